@@ -5,6 +5,7 @@
 #include "../../include/cuhnsw_b200.h"
 #include "engine.h"
 #include "replicas.h"
+#include "table.h"
 
 struct cuhnsw_handle {
   hnsw::Engine engine;         // the index on the first (or only) GPU
@@ -226,6 +227,143 @@ int cuhnsw_merge_topk_gathered_device(const int32_t* d_gathered, const int32_t* 
                                           d_id_offsets, parts, num_queries, topk, d_out_ids, d_out_distances,
                                           d_out_found, reinterpret_cast<cudaStream_t>(cuda_stream));
   return e == cudaSuccess ? CUHNSW_OK : CUHNSW_CUDA_ERROR;
+}
+
+// (no exception can come up in these: they check sizes and launch)
+namespace {
+int status(cudaError_t e) { return e == cudaSuccess ? CUHNSW_OK : CUHNSW_CUDA_ERROR; }
+bool type_ok(int32_t type) { return type == CUHNSW_F32 || type == CUHNSW_F16 || type == CUHNSW_BF16; }
+bool type_aligned(const void* p, int32_t type) { return reinterpret_cast<uintptr_t>(p) % hnsw::type_size(type) == 0; }
+// rows x dims values and their bytes stay far below 2^63
+bool table_ok(int64_t rows, int64_t dims) {
+  return rows >= 0 && rows < 0x7fffffffll && dims >= 1 && dims <= (1 << 24);
+}
+bool group_ok(int64_t group) { return group == 32 || group == 64 || (group >= 128 && group % 128 == 0 && group <= (1 << 24)); }
+bool packed_ok(const void* codes, const void* scales) {
+  return codes && scales && reinterpret_cast<uintptr_t>(codes) % 16 == 0 && reinterpret_cast<uintptr_t>(scales) % 2 == 0;
+}
+}  // namespace
+
+int cuhnsw_lookup_device(const void* d_rows, int64_t row_stride, int64_t num_rows, int64_t num_dims, int32_t type,
+                         const void* d_ids, int32_t ids64, int64_t num_ids, float scale, void* d_out,
+                         void* cuda_stream) {
+  if (!table_ok(num_rows, num_dims) || !type_ok(type) || row_stride < 0 || num_ids < 0 || num_ids >= 0x7fffffffll)
+    return CUHNSW_INVALID_ARGUMENT;
+  if (num_ids == 0) return CUHNSW_OK;
+  if ((num_rows > 0 && !d_rows) || !d_ids || !d_out || !type_aligned(d_rows, type) || !type_aligned(d_out, type) ||
+      reinterpret_cast<uintptr_t>(d_ids) % (ids64 ? 8 : 4) != 0)
+    return CUHNSW_INVALID_ARGUMENT;
+  hnsw::LookupParams p{d_rows, row_stride, num_rows, num_dims, type, d_ids, ids64, num_ids, scale, d_out};
+  return status(hnsw::launch_lookup(p, reinterpret_cast<cudaStream_t>(cuda_stream)));
+}
+
+int64_t cuhnsw_lookup_grad_workspace(int64_t num_ids, int64_t num_rows, int64_t num_dims) {
+  if (!table_ok(num_rows, num_dims) || num_ids < 0 || num_ids >= 0x7fffffffll) return CUHNSW_INVALID_ARGUMENT;
+  return (int64_t)hnsw::lookup_grad_workspace(num_ids, num_rows, num_dims);
+}
+
+int cuhnsw_lookup_grad_device(const void* d_grad, int64_t grad_stride, int32_t type, const void* d_ids, int32_t ids64,
+                              int64_t num_ids, int64_t num_rows, int64_t num_dims, float scale, void* d_out,
+                              int32_t out_type, int32_t accumulate, void* d_workspace, void* cuda_stream) {
+  if (!table_ok(num_rows, num_dims) || !type_ok(type) || (out_type != type && out_type != CUHNSW_F32) ||
+      grad_stride < 0 || num_ids < 0 || num_ids >= 0x7fffffffll)
+    return CUHNSW_INVALID_ARGUMENT;
+  if (num_rows == 0) return CUHNSW_OK;
+  if (!d_out || !type_aligned(d_out, out_type)) return CUHNSW_INVALID_ARGUMENT;
+  if (num_ids > 0 && (!d_grad || !type_aligned(d_grad, type) || !d_ids || !d_workspace ||
+                      reinterpret_cast<uintptr_t>(d_ids) % (ids64 ? 8 : 4) != 0 ||
+                      reinterpret_cast<uintptr_t>(d_workspace) % 256 != 0))
+    return CUHNSW_INVALID_ARGUMENT;
+  hnsw::LookupGradParams p{d_grad, grad_stride, type, d_ids, ids64, num_ids, num_rows, num_dims, scale, d_out, out_type,
+                           accumulate, d_workspace};
+  return status(hnsw::launch_lookup_grad(p, reinterpret_cast<cudaStream_t>(cuda_stream)));
+}
+
+int cuhnsw_pack4_device(const void* d_rows, int64_t row_stride, int32_t type, int64_t num_rows, int64_t num_dims,
+                        int64_t group, void* d_codes, void* d_scales, void* cuda_stream) {
+  if (!table_ok(num_rows, num_dims) || !type_ok(type) || !group_ok(group) || row_stride < 0) return CUHNSW_INVALID_ARGUMENT;
+  if (num_rows == 0) return CUHNSW_OK;
+  if (!d_rows || !type_aligned(d_rows, type) || !packed_ok(d_codes, d_scales)) return CUHNSW_INVALID_ARGUMENT;
+  return status(hnsw::launch_pack4(d_rows, row_stride, type, num_rows, num_dims, group, d_codes, d_scales,
+                                   reinterpret_cast<cudaStream_t>(cuda_stream)));
+}
+
+int cuhnsw_unpack4_device(const void* d_codes, const void* d_scales, int64_t num_rows, int64_t num_dims, int64_t group,
+                          void* d_out, int32_t type, void* cuda_stream) {
+  if (!table_ok(num_rows, num_dims) || !type_ok(type) || !group_ok(group)) return CUHNSW_INVALID_ARGUMENT;
+  if (num_rows == 0) return CUHNSW_OK;
+  if (!packed_ok(d_codes, d_scales) || !d_out || !type_aligned(d_out, type)) return CUHNSW_INVALID_ARGUMENT;
+  return status(hnsw::launch_unpack4(d_codes, d_scales, num_rows, num_dims, group, d_out, type,
+                                     reinterpret_cast<cudaStream_t>(cuda_stream)));
+}
+
+int cuhnsw_scores4_device(const void* d_codes, const void* d_scales, int64_t num_rows, int64_t num_dims, int64_t group,
+                          const void* d_queries, int64_t query_stride, int32_t type, int64_t num_queries,
+                          const float* d_bias, float* d_out, void* cuda_stream) {
+  if (!table_ok(num_rows, num_dims) || !type_ok(type) || !group_ok(group) || query_stride < 0 || num_queries < 0 ||
+      num_queries > (1 << 18))
+    return CUHNSW_INVALID_ARGUMENT;
+  if (num_rows == 0 || num_queries == 0) return CUHNSW_OK;
+  if (!packed_ok(d_codes, d_scales) || !d_queries || !type_aligned(d_queries, type) || !d_out ||
+      !type_aligned(d_out, CUHNSW_F32) || !type_aligned(d_bias, CUHNSW_F32))
+    return CUHNSW_INVALID_ARGUMENT;
+  hnsw::Scores4Params p{d_codes, d_scales, num_rows, num_dims, group, d_queries, query_stride, type, num_queries, d_bias,
+                        d_out};
+  return status(hnsw::launch_scores4(p, reinterpret_cast<cudaStream_t>(cuda_stream)));
+}
+
+namespace {
+bool select_ok(int64_t sequences, int64_t beams, int64_t vocabulary, int32_t keep) {
+  return sequences >= 0 && sequences < 0x7fffffffll && beams >= 1 && beams <= 16384 && vocabulary >= 1 &&
+         vocabulary < 0x7fffffffll && keep >= 1 && keep <= hnsw::kMaxKeep;
+}
+}  // namespace
+
+int64_t cuhnsw_select_workspace(int64_t sequences, int64_t beams, int64_t vocabulary, int32_t keep) {
+  if (!select_ok(sequences, beams, vocabulary, keep)) return CUHNSW_INVALID_ARGUMENT;
+  return (int64_t)hnsw::select_workspace(sequences, beams, vocabulary, keep);
+}
+
+int cuhnsw_select_device(const void* d_scores, int64_t seq_stride, int64_t beam_stride, int32_t type,
+                         const float* d_totals, int64_t sequences, int64_t beams, int64_t vocabulary, int32_t keep,
+                         int32_t log_softmax, int32_t negate, float* d_out_totals, int32_t* d_out_beams,
+                         int32_t* d_out_ids, int32_t* d_out_found, void* d_workspace, void* cuda_stream) {
+  if (!select_ok(sequences, beams, vocabulary, keep) || !type_ok(type) || seq_stride < 0 || beam_stride < 0)
+    return CUHNSW_INVALID_ARGUMENT;
+  if (sequences == 0) return CUHNSW_OK;
+  if (!d_scores || !type_aligned(d_scores, type) || !type_aligned(d_totals, CUHNSW_F32) || !d_out_totals || !d_out_ids ||
+      !d_workspace || reinterpret_cast<uintptr_t>(d_workspace) % 256 != 0)
+    return CUHNSW_INVALID_ARGUMENT;
+  hnsw::SelectParams p{d_scores, type, seq_stride, beam_stride, d_totals, sequences, beams, vocabulary, keep, log_softmax,
+                       d_out_totals, d_out_beams, d_out_ids, d_out_found, negate ? -1.0f : 1.0f, d_workspace};
+  return status(hnsw::launch_select(p, reinterpret_cast<cudaStream_t>(cuda_stream)));
+}
+
+int cuhnsw_reorder_device(const cuhnsw_state* states, int32_t count, const int32_t* d_beams, int64_t sequences,
+                          int64_t beams, int64_t keep, void* cuda_stream) {
+  if (count < 0 || sequences < 0 || beams < 0 || keep < 0 || sequences >= 0x7fffffffll || beams >= 0x7fffffffll ||
+      keep >= 0x7fffffffll || (count > 0 && !states))
+    return CUHNSW_INVALID_ARGUMENT;
+  if (count == 0 || sequences * keep == 0) return CUHNSW_OK;
+  if (!d_beams) return CUHNSW_INVALID_ARGUMENT;
+  for (int32_t i = 0; i < count; ++i) {
+    const cuhnsw_state& s = states[i];
+    if (s.segments < 0 || s.bytes < 0 || s.seq_stride < 0 || s.beam_stride < 0 || s.segment_stride < 0 ||
+        (s.segments * s.bytes > 0 && ((beams > 0 && !s.d_src) || !s.d_dst)))
+      return CUHNSW_INVALID_ARGUMENT;
+  }
+  for (int32_t first = 0; first < count; first += hnsw::kMaxStates) {
+    hnsw::ReorderState block[hnsw::kMaxStates];
+    const int32_t some = count - first < hnsw::kMaxStates ? count - first : hnsw::kMaxStates;
+    for (int32_t i = 0; i < some; ++i) {
+      const cuhnsw_state& s = states[first + i];
+      block[i] = {s.d_src, s.d_dst, s.seq_stride, s.beam_stride, s.segment_stride, s.segments, s.bytes};
+    }
+    const int rc = status(hnsw::launch_reorder(block, some, d_beams, sequences, beams, keep,
+                                               reinterpret_cast<cudaStream_t>(cuda_stream)));
+    if (rc != CUHNSW_OK) return rc;
+  }
+  return CUHNSW_OK;
 }
 
 int cuhnsw_selftest_list_merge(int32_t capacity, const float* distances, const int32_t* ids,

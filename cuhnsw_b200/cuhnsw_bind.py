@@ -17,6 +17,7 @@ LIB_PATH = os.path.join(_HERE, "libcuhnsw_b200.so")
 
 _f32p = ctypes.POINTER(ctypes.c_float)
 _i32p = ctypes.POINTER(ctypes.c_int32)
+_ptr, _i32, _i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
 
 # name -> (restype, argtypes); must list every symbol include/cuhnsw_b200.h declares
 SIGNATURES = {
@@ -62,6 +63,17 @@ SIGNATURES = {
   "cuhnsw_merge_topk_gathered_device": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32,
                                                        ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p,
                                                        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+  "cuhnsw_lookup_device": (ctypes.c_int, [_ptr, _i64, _i64, _i64, _i32, _ptr, _i32, _i64, ctypes.c_float, _ptr, _ptr]),
+  "cuhnsw_lookup_grad_workspace": (_i64, [_i64, _i64, _i64]),
+  "cuhnsw_lookup_grad_device": (ctypes.c_int, [_ptr, _i64, _i32, _ptr, _i32, _i64, _i64, _i64, ctypes.c_float, _ptr,
+                                               _i32, _i32, _ptr, _ptr]),
+  "cuhnsw_pack4_device": (ctypes.c_int, [_ptr, _i64, _i32, _i64, _i64, _i64, _ptr, _ptr, _ptr]),
+  "cuhnsw_unpack4_device": (ctypes.c_int, [_ptr, _ptr, _i64, _i64, _i64, _ptr, _i32, _ptr]),
+  "cuhnsw_scores4_device": (ctypes.c_int, [_ptr, _ptr, _i64, _i64, _i64, _ptr, _i64, _i32, _i64, _ptr, _ptr, _ptr]),
+  "cuhnsw_select_workspace": (_i64, [_i64, _i64, _i64, _i32]),
+  "cuhnsw_select_device": (ctypes.c_int, [_ptr, _i64, _i64, _i32, _ptr, _i64, _i64, _i64, _i32, _i32, _i32, _ptr, _ptr,
+                                          _ptr, _ptr, _ptr, _ptr]),
+  "cuhnsw_reorder_device": (ctypes.c_int, [_ptr, _i32, _ptr, _i64, _i64, _i64, _ptr]),
   "cuhnsw_selftest_list_merge": (ctypes.c_int, [ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                                 ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                                 ctypes.c_void_p, ctypes.c_void_p]),

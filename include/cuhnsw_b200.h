@@ -180,6 +180,83 @@ int cuhnsw_merge_topk_gathered_device(const int32_t* d_gathered, const int32_t* 
                                       int64_t num_queries, int32_t topk, int32_t* d_out_ids, float* d_out_distances,
                                       int32_t* d_out_found, void* cuda_stream);
 
+/* ---- Operators over a table of embeddings -------------------------------------------------------------------------
+ * What a model that keeps its table in an index needs beside the search: rows by number and the gradient of the table,
+ * rows held in 4 bits with their products, and a beam search's selection.  No counterpart in the reference.  All
+ * pointers are device pointers of the current device, all work is enqueued on cuda_stream (which belongs to it) and not
+ * waited for; nothing is allocated, so every call can be captured into a CUDA graph.  Workspaces: the *_workspace functions
+ * say how many bytes (256-byte aligned); their contents need not be kept, but calls that may run at the same time,
+ * captured ones too, need one each.  cuhnsw_b200/table.py is the same for torch tensors. */
+
+/* element types; all sums are fp32 whatever the type */
+enum { CUHNSW_F32 = 0, CUHNSW_F16 = 1, CUHNSW_BF16 = 2 };
+
+/* d_out[t] = scale * d_rows[d_ids[t]], rounded once to the rows' type (scale 1: copied).  d_rows: num_rows rows of num_dims
+ * values, row_stride values apart; d_ids: num_ids int32 or (ids64) int64; d_out: num_ids x num_dims, dense.  An id outside
+ * 0..num_rows-1, e.g. the -1 of an empty result slot, gives zeros.  num_rows up to 2^31 - 2. */
+int cuhnsw_lookup_device(const void* d_rows, int64_t row_stride, int64_t num_rows, int64_t num_dims, int32_t type,
+                         const void* d_ids, int32_t ids64, int64_t num_ids, float scale, void* d_out,
+                         void* cuda_stream);
+
+/* The gradient of that lookup: d_out[r] = scale * sum of d_grad[t] over all t with d_ids[t] = r, for every row of the
+ * table; with `accumulate` it is added to what d_out holds, and rows without ids keep their bits.  d_grad: num_ids rows of num_dims
+ * values of `type`, grad_stride values apart; d_out: num_rows x num_dims, dense, of out_type (`type` or CUHNSW_F32).
+ * The ids are sorted and the sums taken in fp32 in a fixed order: the result does not change from call to call. */
+int64_t cuhnsw_lookup_grad_workspace(int64_t num_ids, int64_t num_rows, int64_t num_dims);
+int cuhnsw_lookup_grad_device(const void* d_grad, int64_t grad_stride, int32_t type, const void* d_ids, int32_t ids64,
+                              int64_t num_ids, int64_t num_rows, int64_t num_dims, float scale, void* d_out,
+                              int32_t out_type, int32_t accumulate, void* d_workspace, void* cuda_stream);
+
+/* Rows in 4 bits.  A value is (code - 8) * scale, with a code of 0..15 per value and a bfloat16 scale per `group` consecutive
+ * dimensions (32, 64 or a multiple of 128; the last group of a row may be shorter):
+ *   scale = bfloat16(largest magnitude of the group * fp32(1 / 7)),  code = round_half_even(value / scale) within -8..7, plus 8
+ * (8 where the scale is 0).  Values have to be finite.
+ * d_scales: num_rows x ceil(num_dims / group).  d_codes: num_rows x 16 * ceil(num_dims / 32) bytes, 16-byte aligned.  A
+ * row's bytes are little-endian 32-bit words of eight codes; blocks of 32 dimensions lie in fours, the last of a row as many
+ * as are left (m of them): word t*m + j of a four (t = 0..3) holds dimensions 8t..8t+7 of its block j, the even ones
+ * in nibbles 0..3 (lowest first), the odd ones in nibbles 4..7.  Codes behind num_dims are 8 when packed here, and not looked
+ * at elsewhere. */
+int cuhnsw_pack4_device(const void* d_rows, int64_t row_stride, int32_t type, int64_t num_rows, int64_t num_dims,
+                        int64_t group, void* d_codes, void* d_scales, void* cuda_stream);
+/* d_out: num_rows x num_dims values of `type`, dense */
+int cuhnsw_unpack4_device(const void* d_codes, const void* d_scales, int64_t num_rows, int64_t num_dims, int64_t group,
+                          void* d_out, int32_t type, void* cuda_stream);
+/* d_out[q, r] = sum over the dimensions of query q times row r, plus d_bias[r] (fp32, may be NULL).  d_queries:
+ * num_queries rows of num_dims values of `type`, query_stride values apart; d_out: num_queries x num_rows fp32, dense.
+ * fp32 queries enter with their 24 bits. */
+int cuhnsw_scores4_device(const void* d_codes, const void* d_scales, int64_t num_rows, int64_t num_dims, int64_t group,
+                          const void* d_queries, int64_t query_stride, int32_t type, int64_t num_queries,
+                          const float* d_bias, float* d_out, void* cuda_stream);
+
+/* The `keep` (up to 256) largest totals of each sequence over its beams and the vocabulary:
+ *   total[b, v] = d_totals[b] + d_scores[b, v] - (log_softmax: log of the sum over u of exp(d_scores[b, u]))
+ * in descending order, equal ones by smaller beam, then smaller v.  d_scores: values of `type`, those of one beam contiguous,
+ * sequences seq_stride and beams beam_stride values apart; d_totals: sequences x beams fp32, or NULL for zeros.  Totals of
+ * -inf or NaN are not chosen; what is left of the `keep` slots holds -inf, -1, -1.  d_out_*: sequences x keep; d_out_beams and
+ * d_out_found (slots in use, per sequence) may be NULL.  negate: the totals are written with the other sign (+inf in empty
+ * slots), the distances of the dot metric.  Totals are compared in 64 bits.  vocabulary below 2^31, beams up to 16384. */
+int64_t cuhnsw_select_workspace(int64_t sequences, int64_t beams, int64_t vocabulary, int32_t keep);
+int cuhnsw_select_device(const void* d_scores, int64_t seq_stride, int64_t beam_stride, int32_t type,
+                         const float* d_totals, int64_t sequences, int64_t beams, int64_t vocabulary, int32_t keep,
+                         int32_t log_softmax, int32_t negate, float* d_out_totals, int32_t* d_out_beams,
+                         int32_t* d_out_ids, int32_t* d_out_found, void* d_workspace, void* cuda_stream);
+
+/* The states of the chosen beams: row (s, k) of state i's output is row (s, d_beams[s, k]) of its input; a number outside
+ * 0..beams-1 gives zeros.  A row is `segments` pieces of `bytes` bytes, segment_stride bytes apart in the input, dense in
+ * the output (a cache of which only the first positions of every head are in use).  `states` is a host array, read before the call
+ * returns.  Inputs and outputs must not overlap. */
+typedef struct cuhnsw_state {
+  const void* d_src;
+  void* d_dst;
+  int64_t seq_stride;   /* bytes between sequences of d_src */
+  int64_t beam_stride;  /* bytes between beams of d_src */
+  int64_t segment_stride;
+  int64_t segments;
+  int64_t bytes;
+} cuhnsw_state;
+int cuhnsw_reorder_device(const cuhnsw_state* states, int32_t count, const int32_t* d_beams, int64_t sequences,
+                          int64_t beams, int64_t keep, void* cuda_stream);
+
 /* Self-tests of the two shared-memory structures every walk uses, for checking them against a host model
  * (host arrays in and out, runs on the current GPU, one warp).  They pin the semantics the reference spreads
  * over PushNodeToSearchPq / CheckAlreadyExists / GetCand (cpp/include/cuda_utils_kernels.cuh:50-151,212-227:
