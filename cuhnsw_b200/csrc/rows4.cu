@@ -133,10 +133,28 @@ cudaError_t pack_t(const T* rows, long long row_stride, long long n, long long d
 // code becomes a half or bfloat16 value exactly, and so do products and the sums of a group in fp32; the scale is applied to
 // a group's sum in fp32.  An fp32 query is three columns of bfloat16, 8 bits of it each, whose sums are added at the end.
 //
-// Bound: HBM bytes of the codes while the columns are few.  Every warp has 16 rows and a share of their blocks; a CTA's warps
-// are `split` shares x 8/split sets of 16 rows.  The queries lie in shared memory.
-constexpr int kScoreWarps = 8;
-constexpr int kScoreThreads = kScoreWarps * 32;
+// Bound: HBM bytes of the codes while the columns are few.  A warp has 32 rows and a share of their dimensions.  It copies its
+// codes asynchronously into a ring of its own in shared memory, two steps of 128 dimensions ahead and across the end of its rows, so
+// that nothing waits for a barrier to keep the copies going; every lane reads back what it copied itself.  A CTA's warps are
+// `split` shares x warps/split sets of 32 rows; all of them read the queries in shared memory.
+constexpr int kRowTiles = 2;                  // operands of 16 rows per warp
+constexpr int kWarpRows = 16 * kRowTiles;
+constexpr int kRowsPerLane = 2 * kRowTiles;   // of the first operand: rows g, g + 8, g + 16, ..
+constexpr int kSumPitch = kWarpRows + 1;
+constexpr int kStages = 3;                    // of the ring
+constexpr int kStageBytes = kWarpRows * 64;
+constexpr int kMostScoreThreads = 512;
+
+template <int Bytes>
+__device__ __forceinline__ void copy_async(unsigned to, const void* from) {
+  if constexpr (Bytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(Bytes) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int Left>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(Left) : "memory"); }
 
 struct PairsF16 {
   // two codes of nibbles `pair` and `pair` + 4 as code - 8
@@ -203,181 +221,365 @@ struct ColumnsF32 {
 };
 
 struct ScoreLayout {
-  int columns;      // 8 * kTiles
-  int queries;      // of a launch's column tile
-  int pitch;        // values per column in shared memory
-  int chunk_fours;  // fours of blocks whose queries are in shared memory at a time
-  int split;        // warps that share 16 rows
+  int queries;       // of a tile of columns: at most 8 * kTiles / parts
+  int pitch;         // values per column in shared memory
+  int chunk_fours;   // fours of blocks whose queries are in shared memory at a time
+  int split;         // warps that share 32 rows
+  int column_tiles;
+  int wide_queries;  // 16-byte loads of queries
+  int wide_scales;   // loads of all scales of four blocks at once
 };
 
-template <class Columns, int kTiles>
-__global__ void __launch_bounds__(kScoreThreads) scores_kernel(Scores4Params p, ScoreLayout l) {
-  using Pairs = typename Columns::Pairs;
-  extern __shared__ __align__(16) unsigned char smem[];
-  unsigned short* xs = reinterpret_cast<unsigned short*>(smem);
-  float* sums = reinterpret_cast<float*>(smem + (size_t)l.columns * l.pitch * 2);  // [warp][column][16 rows + 1]
-  const int warp = threadIdx.x >> 5, lane = lane_id(), g = lane >> 2, t = lane & 3;
-  const int part = warp % l.split, set = warp / l.split, sets = kScoreWarps / l.split;
-  const long long q0 = (long long)blockIdx.y * l.queries;
-  const int nq = (int)min((long long)l.queries, p.nq - q0);
-  const long long blocks = (p.d + kBlock - 1) / kBlock, row_bytes = 16 * blocks;
-  const long long fours = (blocks + 3) / 4, groups = packed_groups_device(p.d, p.group);
-  const int group_blocks = (int)min(p.group / kBlock, 1ll << 30);
-  const unsigned char* codes = static_cast<const unsigned char*>(p.codes);
-  const __nv_bfloat16* scales = static_cast<const __nv_bfloat16*>(p.scales);
-  const typename Columns::In* x = static_cast<const typename Columns::In*>(p.queries);
-  const long long tiles = (p.n + 16 * sets - 1) / (16 * sets);
-  const bool staged_once = fours <= l.chunk_fours;
-  auto stage = [&](long long first_four) {
-    const long long dim0 = first_four * kFour;
-    const int dims = (int)(min((long long)l.chunk_fours, fours - first_four) * kFour);
-    for (int i = threadIdx.x; i < l.columns * dims; i += kScoreThreads) {
-      const int c = i / dims, k = i % dims, q = c / Columns::kParts;
-      unsigned short v = 0;
-      if (q < nq && dim0 + k < p.d) v = Columns::part(x[(q0 + q) * p.query_stride + dim0 + k], c % Columns::kParts);
-      xs[c * l.pitch + k] = v;
-    }
-  };
-  if (staged_once) {
-    stage(0);
-    __syncthreads();
-  }
-  for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const long long row0 = tile * 16 * sets + 16 * set;
-    // rows behind the last one are read as the last one and not written
-    const long long ra = min(row0 + g, p.n - 1), rb = min(row0 + g + 8, p.n - 1);
-    const unsigned char* ca = codes + ra * row_bytes;
-    const unsigned char* cb = codes + rb * row_bytes;
-    const __nv_bfloat16* sa = scales + ra * groups;
-    const __nv_bfloat16* sb = scales + rb * groups;
-    float total[kTiles][4];
+// The queries' values of the dimensions [first, first + count) (a multiple of 8) to shared memory, zeros behind the last one.
+template <class Columns>
+__device__ __forceinline__ void stage_queries(const Scores4Params& p, const ScoreLayout& l, long long q0, int nq,
+                                              long long first, int count, unsigned short* xs) {
+  using In = typename Columns::In;
+  const In* x = static_cast<const In*>(p.queries);
+  const int eights = count / 8;
+  for (int q = 0; q < nq; ++q) {
+    const In* src = x + (q0 + q) * p.query_stride + first;
+    for (int i = threadIdx.x; i < eights; i += blockDim.x) {
+      In v[8];
+      if (l.wide_queries && first + 8 * i + 8 <= p.d) {
+        load_many<In, 8>(src + 8 * i, v);
+      } else {
 #pragma unroll
-    for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) total[i][j] = 0.0f;
-    for (long long chunk = 0; chunk < fours; chunk += l.chunk_fours) {
-      if (!staged_once) {
-        __syncthreads();
-        stage(chunk);
-        __syncthreads();
+        for (int j = 0; j < 8; ++j) v[j] = first + 8 * i + j < p.d ? src[8 * i + j] : from_f32<In>(0.0f);
       }
-      const long long in_chunk = min((long long)l.chunk_fours, fours - chunk);
-      const long long each = (in_chunk + l.split - 1) / l.split;
-      const long long from = chunk + part * each, to = min(chunk + in_chunk, from + each);
-      for (long long four = from; four < to; ++four) {
-        const int m = (int)min(4ll, blocks - 4 * four);
-        unsigned wa[4], wb[4];
-        if (m == 4) {
-          const uint4 a = __ldcs(reinterpret_cast<const uint4*>(ca + 64 * four + 16 * t));
-          const uint4 b = __ldcs(reinterpret_cast<const uint4*>(cb + 64 * four + 16 * t));
-          wa[0] = a.x, wa[1] = a.y, wa[2] = a.z, wa[3] = a.w;
-          wb[0] = b.x, wb[1] = b.y, wb[2] = b.z, wb[3] = b.w;
-        } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            wa[j] = j < m ? *reinterpret_cast<const unsigned*>(ca + 64 * four + 4 * (t * m + j)) : 0x88888888u;
-            wb[j] = j < m ? *reinterpret_cast<const unsigned*>(cb + 64 * four + 4 * (t * m + j)) : 0x88888888u;
+      for (int c = 0; c < Columns::kParts; ++c) {
+        unsigned w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          w[j] = (unsigned)Columns::part(v[2 * j], c) | ((unsigned)Columns::part(v[2 * j + 1], c) << 16);
+        *reinterpret_cast<uint4*>(xs + (c * nq + q) * l.pitch + 8 * i) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ float bf16_low(unsigned pair) { return __uint_as_float(pair << 16); }
+__device__ __forceinline__ float bf16_high(unsigned pair) { return __uint_as_float(pair & 0xffff0000u); }
+
+// The scales of a row for four blocks: pairs of bfloat16
+template <int kGroup>
+struct FourScales;
+template <>
+struct FourScales<1> {
+  uint2 raw;
+  __device__ __forceinline__ void load(const unsigned short* row, int four, int, int groups, bool wide) {
+    if (wide) {
+      raw = *reinterpret_cast<const uint2*>(row + 4 * four);
+    } else {
+      const unsigned short* at = row + 4 * four;
+      const int left = groups - 4 * four;
+      raw.x = at[0] | (left > 1 ? (unsigned)at[1] << 16 : 0);
+      raw.y = (left > 2 ? at[2] : 0) | (left > 3 ? (unsigned)at[3] << 16 : 0);
+    }
+  }
+  __device__ __forceinline__ float get(int j) const {
+    return j == 0 ? bf16_low(raw.x) : j == 1 ? bf16_high(raw.x) : j == 2 ? bf16_low(raw.y) : bf16_high(raw.y);
+  }
+};
+template <>
+struct FourScales<2> {
+  unsigned raw;
+  __device__ __forceinline__ void load(const unsigned short* row, int four, int, int groups, bool wide) {
+    if (wide)
+      raw = *reinterpret_cast<const unsigned*>(row + 2 * four);
+    else
+      raw = row[2 * four] | (groups - 2 * four > 1 ? (unsigned)row[2 * four + 1] << 16 : 0);
+  }
+  __device__ __forceinline__ float get(int j) const { return j == 0 ? bf16_low(raw) : bf16_high(raw); }
+};
+template <>
+struct FourScales<4> {
+  unsigned raw;
+  __device__ __forceinline__ void load(const unsigned short* row, int four, int group_fours, int, bool) {
+    raw = row[group_fours == 1 ? four : four / group_fours];
+  }
+  __device__ __forceinline__ float get(int) const { return bf16_low(raw); }
+};
+
+// kGroup: blocks of 32 dimensions per scale, 4 for four and more.  The parts of an fp32 query are the same column of three
+// operands, so that a lane holds all its sums.
+template <class Columns, int kTiles, int kGroup>
+__global__ void __launch_bounds__(kMostScoreThreads, 1) scores_kernel(const __grid_constant__ Scores4Params p,
+                                                                      const __grid_constant__ ScoreLayout l) {
+  using Pairs = typename Columns::Pairs;
+  constexpr int kOutTiles = kTiles / Columns::kParts;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = lane_id(), g = lane >> 2, t = lane & 3;
+  const int part = warp % l.split, set = warp / l.split, sets = warps / l.split;
+  // the tiles of columns of the same rows run side by side: the second one finds the codes in the L2 cache
+  const long long q0 = (long long)(blockIdx.x % l.column_tiles) * l.queries;
+  const int nq = (int)min((long long)l.queries, p.nq - q0);
+  const int first_unit = blockIdx.x / l.column_tiles, step = gridDim.x / l.column_tiles;
+  // shared memory: the rings, the sums on their way out [warp][8 columns][row], the queries
+  const unsigned ring = (unsigned)__cvta_generic_to_shared(smem) + warp * (kStages * kStageBytes) + 16 * lane;
+  float* sums = reinterpret_cast<float*>(smem + warps * kStages * kStageBytes);
+  unsigned short* xs = reinterpret_cast<unsigned short*>(sums + warps * 8 * kSumPitch);
+  const int blocks = (int)((p.d + kBlock - 1) / kBlock), fours = (blocks + 3) / 4;
+  const int groups = (int)packed_groups_device(p.d, p.group), group_fours = (int)(p.group / kFour);
+  const int row_bytes = 16 * blocks;
+  const unsigned rows = (unsigned)p.n;
+  const unsigned char* codes = static_cast<const unsigned char*>(p.codes);
+  const unsigned short* scales = static_cast<const unsigned short*>(p.scales);
+  const int units = (int)((p.n + kWarpRows * sets - 1) / (kWarpRows * sets));
+
+  for (int chunk = 0; chunk < fours; chunk += l.chunk_fours) {
+    const int in_chunk = min(l.chunk_fours, fours - chunk);
+    const int each = (in_chunk + l.split - 1) / l.split;
+    const int from = chunk + min(part * each, in_chunk), to = min(chunk + in_chunk, from + each);
+    int ahead_unit = first_unit, ahead_four = from;  // what is copied next
+    unsigned ahead_slot = 0;
+    auto copy = [&] {
+      if (ahead_unit < units && from < to) {
+        const unsigned row0 = (unsigned)(ahead_unit * sets + set) * kWarpRows + g;
+        const int m = min(4, blocks - 4 * ahead_four);
+        const int at = 64 * ahead_four + 4 * t * m;
+        const unsigned slot = ring + ahead_slot;
+#pragma unroll
+        for (int i = 0; i < kRowsPerLane; ++i) {
+          // rows behind the last one are read as the last one and not written
+          const unsigned char* src = codes + (long long)min(row0 + 8 * i, rows - 1) * row_bytes + at;
+          if (m == 4) {
+            copy_async<16>(slot + 512 * i, src);
+          } else if (m == 2) {
+            copy_async<8>(slot + 512 * i, src);
+          } else {
+            copy_async<4>(slot + 512 * i, src);
+            if (m == 3) {
+              copy_async<4>(slot + 512 * i + 4, src + 4);
+              copy_async<4>(slot + 512 * i + 8, src + 8);
+            }
           }
         }
-        float sum[kTiles][4];
+        if (++ahead_four == to) {
+          ahead_four = from;
+          ahead_unit += step;
+        }
+      }
+      ahead_slot = ahead_slot == (kStages - 1) * kStageBytes ? 0 : ahead_slot + kStageBytes;
+      copies_end();
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) copy();
+    if (chunk > 0) __syncthreads();
+    stage_queries<Columns>(p, l, q0, nq, (long long)chunk * kFour, in_chunk * kFour, xs);
+    __syncthreads();
+    // lanes of columns that there are not read the last one's and throw the result away
+    const unsigned short* column = xs + 8 * t;
+
+    unsigned slot = 0;
+    FourScales<kGroup> scale[kRowsPerLane];
+    auto load_scales = [&](int unit, int four) {
+      const unsigned row0 = (unsigned)(unit * sets + set) * kWarpRows + g;
+#pragma unroll
+      for (int i = 0; i < kRowsPerLane; ++i)
+        scale[i].load(scales + (long long)min(row0 + 8 * i, rows - 1) * groups, four, group_fours, groups, l.wide_scales);
+    };
+    if (first_unit < units && from < to) load_scales(first_unit, from);
+    for (int unit = first_unit; unit < units; unit += step) {
+      float total[kRowTiles][kTiles][4];
+#pragma unroll
+      for (int r = 0; r < kRowTiles; ++r)
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) total[r][i][j] = 0.0f;
+      for (int four = from; four < to; ++four) {
+        copy();
+        copies_wait<kStages - 1>();
+        FourScales<kGroup> now[kRowsPerLane];
+#pragma unroll
+        for (int i = 0; i < kRowsPerLane; ++i) now[i] = scale[i];
+        if (four + 1 < to)
+          load_scales(unit, four + 1);
+        else if (unit + step < units)
+          load_scales(unit + step, from);
+        uint4 w[kRowsPerLane];
+#pragma unroll
+        for (int i = 0; i < kRowsPerLane; ++i)
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w)
+                       : "r"(ring + slot + 512 * i)
+                       : "memory");
+        slot = slot == (kStages - 1) * kStageBytes ? 0 : slot + kStageBytes;
+        const int m = min(4, blocks - 4 * four);
+        const unsigned short* values = column + (four - chunk) * kFour;
+        float sum[kRowTiles][kTiles][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (j >= m) break;
-          const long long block = 4 * four + j;
-          if (j == 0 || block % group_blocks == 0) {
+          if (j % kGroup == 0) {
 #pragma unroll
-            for (int i = 0; i < kTiles; ++i)
+            for (int r = 0; r < kRowTiles; ++r)
 #pragma unroll
-              for (int k = 0; k < 4; ++k) sum[i][k] = 0.0f;
+              for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) sum[r][i][k] = 0.0f;
           }
-          const unsigned a0[4] = {Pairs::template values<0>(wa[j]), Pairs::template values<0>(wb[j]),
-                                  Pairs::template values<1>(wa[j]), Pairs::template values<1>(wb[j])};
-          const unsigned a1[4] = {Pairs::template values<2>(wa[j]), Pairs::template values<2>(wb[j]),
-                                  Pairs::template values<3>(wa[j]), Pairs::template values<3>(wb[j])};
-          const unsigned short* column = xs + g * l.pitch + (four - chunk) * kFour + j * kBlock + 8 * t;
-#pragma unroll
-          for (int i = 0; i < kTiles; ++i) {
-            const uint4 b = *reinterpret_cast<const uint4*>(column + i * 8 * l.pitch);
-            Pairs::mma(sum[i], a0, b.x, b.y);
-            Pairs::mma(sum[i], a1, b.z, b.w);
-          }
-          if (j == m - 1 || (block + 1) % group_blocks == 0) {
-            const float fa = __bfloat162float(sa[block / group_blocks]), fb = __bfloat162float(sb[block / group_blocks]);
+          if (j < m) {
+            uint4 b[kTiles];
 #pragma unroll
             for (int i = 0; i < kTiles; ++i) {
-              total[i][0] += fa * sum[i][0];
-              total[i][1] += fa * sum[i][1];
-              total[i][2] += fb * sum[i][2];
-              total[i][3] += fb * sum[i][3];
+              const int c = Columns::kParts == 1 ? min(8 * i + g, nq - 1) : i * nq + min(g, nq - 1);
+              b[i] = *reinterpret_cast<const uint4*>(values + c * l.pitch + j * kBlock);
+            }
+#pragma unroll
+            for (int r = 0; r < kRowTiles; ++r) {
+              const uint4& low = w[2 * r];
+              const uint4& high = w[2 * r + 1];
+              const unsigned wa = j == 0 ? low.x : j == 1 ? low.y : j == 2 ? low.z : low.w;
+              const unsigned wb = j == 0 ? high.x : j == 1 ? high.y : j == 2 ? high.z : high.w;
+              const unsigned a0[4] = {Pairs::template values<0>(wa), Pairs::template values<0>(wb),
+                                      Pairs::template values<1>(wa), Pairs::template values<1>(wb)};
+              const unsigned a1[4] = {Pairs::template values<2>(wa), Pairs::template values<2>(wb),
+                                      Pairs::template values<3>(wa), Pairs::template values<3>(wb)};
+#pragma unroll
+              for (int i = 0; i < kTiles; ++i) {
+                Pairs::mma(sum[r][i], a0, b[i].x, b[i].y);
+                Pairs::mma(sum[r][i], a1, b[i].z, b[i].w);
+              }
+            }
+          }
+          if ((j + 1) % kGroup == 0 && j / kGroup * kGroup < m) {
+#pragma unroll
+            for (int r = 0; r < kRowTiles; ++r) {
+              const float fa = now[2 * r].get(j / kGroup), fb = now[2 * r + 1].get(j / kGroup);
+#pragma unroll
+              for (int i = 0; i < kTiles; ++i) {
+                total[r][i][0] += fa * sum[r][i][0];
+                total[r][i][1] += fa * sum[r][i][1];
+                total[r][i][2] += fb * sum[r][i][2];
+                total[r][i][3] += fb * sum[r][i][3];
+              }
             }
           }
         }
       }
-    }
-    // the shares and, of fp32 queries, the parts are added up in shared memory
-    float* mine = sums + warp * l.columns * 17;
+      // through shared memory, eight columns at a time: rows next to each other, the shares added up
+      float* mine = sums + warp * 8 * kSumPitch;
+      const int set_rows = kWarpRows * sets;
 #pragma unroll
-    for (int i = 0; i < kTiles; ++i) {
-      mine[(8 * i + 2 * t) * 17 + g] = total[i][0];
-      mine[(8 * i + 2 * t + 1) * 17 + g] = total[i][1];
-      mine[(8 * i + 2 * t) * 17 + g + 8] = total[i][2];
-      mine[(8 * i + 2 * t + 1) * 17 + g + 8] = total[i][3];
-    }
-    __syncthreads();
-    const int rows = 16 * sets;
-    for (int i = threadIdx.x; i < nq * rows; i += kScoreThreads) {
-      const int q = i / rows, r = i % rows;
-      const long long row = tile * rows + r;
-      if (row >= p.n) continue;
-      float y = 0.0f;
+      for (int i = 0; i < kOutTiles; ++i) {
+        const int some = min(8, nq - 8 * i);
+        if (some <= 0) break;
 #pragma unroll
-      for (int c = Columns::kParts - 1; c >= 0; --c)  // the small parts first
-        for (int s = 0; s < l.split; ++s)
-          y += sums[((r / 16) * l.split + s) * l.columns * 17 + (q * Columns::kParts + c) * 17 + r % 16];
-      if (p.bias) y += p.bias[row];
-      p.out[(q0 + q) * p.n + row] = y;
+        for (int r = 0; r < kRowsPerLane; ++r) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float y = total[r / 2][i * Columns::kParts][2 * (r % 2) + c];
+            if constexpr (Columns::kParts == 3)
+              y += total[r / 2][i * Columns::kParts + 1][2 * (r % 2) + c] +
+                   total[r / 2][i * Columns::kParts + 2][2 * (r % 2) + c];
+            mine[(2 * t + c) * kSumPitch + g + 8 * r] = y;
+          }
+        }
+        auto write = [&](float y, int q, long long row) {
+          float* out = p.out + (q0 + 8 * i + q) * p.n + row;
+          if (chunk > 0)
+            y += *out;
+          else if (p.bias)
+            y += p.bias[row];
+          *out = y;
+        };
+        if (l.split == 1) {
+          __syncwarp();
+          const long long row = (long long)(unit * sets + set) * kWarpRows + lane;
+          if (row < p.n)
+            for (int q = 0; q < some; ++q) write(mine[q * kSumPitch + lane], q, row);
+          __syncwarp();
+        } else {
+          __syncthreads();
+          for (int k = threadIdx.x; k < some * set_rows; k += blockDim.x) {
+            const int q = k / set_rows, r = k % set_rows;
+            const long long row = (long long)unit * set_rows + r;
+            if (row < p.n) {
+              const float* of_set = sums + ((r / kWarpRows) * l.split * 8 + q) * kSumPitch + r % kWarpRows;
+              float y = of_set[0];
+              for (int s = 1; s < l.split; ++s) y += of_set[s * 8 * kSumPitch];
+              write(y, q, row);
+            }
+          }
+          __syncthreads();
+        }
+      }
     }
-    __syncthreads();
+    copies_wait<0>();
   }
 }
 
-template <class Columns, int kTiles>
-cudaError_t scores_t(const Scores4Params& p, cudaStream_t stream) {
-  constexpr int kSpace = 96 * 1024;  // of the queries in shared memory: two CTAs per SM
+template <class Columns, int kTiles, int kGroup>
+cudaError_t scores_t(const Scores4Params& p, int queries, cudaStream_t stream) {
+  constexpr int kMostSpace = 224 * 1024, kHalfSpace = 112 * 1024;  // shared memory of one CTA per SM, of each of two
   ScoreLayout l;
-  l.columns = 8 * kTiles;
-  l.queries = l.columns / Columns::kParts;
-  const long long fours = (p.d + kFour - 1) / kFour;
-  const long long most = kSpace / (l.columns * 2 * kFour);
-  l.chunk_fours = (int)(fours < most ? fours : most);
-  // eight lanes read 16 bytes of two columns and four parts: half a row of banks from column to column
+  l.queries = (int)(p.nq < queries ? p.nq : queries);
+  const int columns = l.queries * Columns::kParts;
+  const int fours = (int)((p.d + kFour - 1) / kFour);
+  auto space = [&](int warps, int in_chunk) {
+    // eight lanes read 16 bytes of two columns and four parts: half a row of banks from column to column
+    return (size_t)columns * (in_chunk * kFour + 32) * 2 + (size_t)warps * (kStages * kStageBytes + 8 * kSumPitch * 4);
+  };
+  // two CTAs of eight warps per SM, or one of as many as the queries leave room for
+  int warps = 8;
+  l.chunk_fours = fours;
+  const bool two = space(8, fours) <= kHalfSpace;
+  if (!two) {
+    warps = 16;
+    while (warps > 8 && space(warps, fours) > kMostSpace) warps -= 4;
+    while (space(warps, l.chunk_fours) > kMostSpace) l.chunk_fours = (l.chunk_fours + 1) / 2;
+  }
   l.pitch = l.chunk_fours * kFour + 32;
-  const long long sets = (p.n + 15) / 16;
+  const size_t smem = space(warps, l.chunk_fours);
+  l.column_tiles = (int)((p.nq + l.queries - 1) / l.queries);
+  // several units for every CTA, and something to do for every warp
+  const long long sets = (p.n + kWarpRows - 1) / kWarpRows;
+  const long long room = (long long)kSMs * (two ? 2 : 1);
   l.split = 1;
-  // rows for at least four CTAs per SM and every warp something to do
-  while (l.split < kScoreWarps && 2 * l.split <= fours && sets * l.split < (long long)kSMs * 4 * kScoreWarps) l.split *= 2;
-  const size_t smem = (size_t)l.columns * l.pitch * 2 + (size_t)kScoreWarps * l.columns * 17 * 4;
-  cudaError_t e = cudaFuncSetAttribute(scores_kernel<Columns, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  while (l.split < (warps == 12 ? 4 : 8) && 2 * l.split <= l.chunk_fours &&
+         sets * l.split * l.column_tiles < 8 * room * warps)
+    l.split *= 2;
+  const long long units = (sets + warps / l.split - 1) / (warps / l.split);
+  long long step = (room + l.column_tiles - 1) / l.column_tiles;
+  if (step > units) step = units;
+  if (step * l.column_tiles > 0x7fffffffll) return cudaErrorInvalidValue;
+  l.wide_queries = word_bytes(reinterpret_cast<uintptr_t>(p.queries) |
+                              (unsigned long long)(p.query_stride * sizeof(typename Columns::In))) == 16;
+  const int per_four = kGroup == 1 ? 4 : kGroup == 2 ? 2 : 1;
+  l.wide_scales = packed_groups(p.d, p.group) % per_four == 0 && reinterpret_cast<uintptr_t>(p.scales) % (2 * per_four) == 0;
+  cudaError_t e = allow_smem<scores_kernel<Columns, kTiles, kGroup>>();
   if (e != cudaSuccess) return e;
-  int per_sm = 0;
-  e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, scores_kernel<Columns, kTiles>, kScoreThreads, smem);
-  if (e != cudaSuccess) return e;
-  const long long tiles = (sets + kScoreWarps / l.split - 1) / (kScoreWarps / l.split);
-  const long long column_tiles = (p.nq + l.queries - 1) / l.queries;
-  if (column_tiles > 65535) return cudaErrorInvalidValue;
-  const long long room = (long long)kSMs * (per_sm > 0 ? per_sm : 1);
-  const long long blocks = tiles < room ? tiles : room;
-  scores_kernel<Columns, kTiles><<<dim3((unsigned)blocks, (unsigned)column_tiles), kScoreThreads, smem, stream>>>(p, l);
+  scores_kernel<Columns, kTiles, kGroup><<<(unsigned)(step * l.column_tiles), 32 * warps, smem, stream>>>(p, l);
   return cudaGetLastError();
+}
+
+template <class Columns, int kTiles>
+cudaError_t scores_group(const Scores4Params& p, int queries, cudaStream_t stream) {
+  if (p.group == kBlock) return scores_t<Columns, kTiles, 1>(p, queries, stream);
+  if (p.group == 2 * kBlock) return scores_t<Columns, kTiles, 2>(p, queries, stream);
+  return scores_t<Columns, kTiles, 4>(p, queries, stream);
 }
 
 template <class Columns>
 cudaError_t scores_columns(const Scores4Params& p, cudaStream_t stream) {
-  const long long columns = p.nq * Columns::kParts;
-  if (columns <= 8) return scores_t<Columns, 1>(p, stream);
-  if (columns <= 16) return scores_t<Columns, 2>(p, stream);
-  if (columns <= 24) return scores_t<Columns, 3>(p, stream);
-  return scores_t<Columns, 4>(p, stream);
+  // as many queries at a time as fit into the operands' columns and, with all their dimensions, into shared memory; then as many
+  // tiles of equal size as that takes
+  constexpr long long kSpace = 132 * 1024;
+  const long long fit = kSpace / (Columns::kParts * 2 * ((p.d + kFour - 1) / kFour * kFour + 32));
+  long long queries = Columns::kParts == 1 ? 32 : 8;
+  if (fit < queries) queries = fit < 1 ? 1 : fit;
+  const long long tiles = (p.nq + queries - 1) / queries;
+  queries = (p.nq + tiles - 1) / tiles;
+  if constexpr (Columns::kParts == 3) {
+    return scores_group<Columns, 3>(p, (int)queries, stream);
+  } else {
+    if (queries <= 8) return scores_group<Columns, 1>(p, (int)queries, stream);
+    if (queries <= 16) return scores_group<Columns, 2>(p, (int)queries, stream);
+    if (queries <= 24) return scores_group<Columns, 3>(p, (int)queries, stream);
+    return scores_group<Columns, 4>(p, (int)queries, stream);
+  }
 }
 
 }  // namespace

@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "table.h"
 
 namespace hnsw {
@@ -95,5 +97,18 @@ inline int next_pow2(long long x, int at_most) {
 }
 
 constexpr int kSMs = 148;
+
+// Lets a kernel have as much shared memory as there is; asked for once per device.
+template <auto kKernel>
+cudaError_t allow_smem() {
+  constexpr int kMost = 227 * 1024 - 2048;  // and what it declares statically
+  static std::atomic<bool> done[64];
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess || (device < 64 && done[device].load(std::memory_order_relaxed))) return e;
+  e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+  if (e == cudaSuccess && device < 64) done[device].store(true, std::memory_order_relaxed);
+  return e;
+}
 
 }  // namespace hnsw
