@@ -389,7 +389,7 @@ cudaError_t launch_select(const SelectParams& p, cudaStream_t stream) {
                   : p.type == kF16 ? pieces_words<__half>(p, plan, best, norms, stream)
                                    : pieces_words<__nv_bfloat16>(p, plan, best, norms, stream);
   if (e != cudaSuccess) return e;
-  e = cudaFuncSetAttribute(sequence_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  e = allow_smem<sequence_kernel>();
   if (e != cudaSuccess) return e;
   sequence_kernel<<<(unsigned)p.sequences, kThreads, smem, stream>>>(p, (int)plan.pieces, best, norms);
   return cudaGetLastError();

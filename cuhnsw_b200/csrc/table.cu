@@ -519,7 +519,7 @@ cudaError_t grad_t(const LookupGradParams& p, cudaStream_t stream) {
   if (p.tokens <= kOneMost) {
     const int items = (int)((p.tokens + kOneThreads - 1) / kOneThreads);
     const size_t smem = (size_t)items * kOneThreads * 6 + (size_t)(kOneThreads / 32) * (1 << sort.digit) * 2;
-    cudaError_t e = cudaFuncSetAttribute(sort_one_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = allow_smem<sort_one_kernel>();
     if (e != cudaSuccess) return e;
     sort_one_kernel<<<1 + zero_blocks, kOneThreads, smem, stream>>>(p, sort, s.keys[0], s.tokens[0], s.joins);
   } else {

@@ -76,6 +76,10 @@ def test_c_abi_has_nothing_to_do():
   assert lib().cuhnsw_reorder_device(None, 0, None, 4, 2, 2, None) == 0
 
 
+def state_of(src, dst, seq_stride, beam_stride, segment_stride, segments, bytes):
+  return (ctypes.c_int64 * 7)(src or 0, dst or 0, seq_stride, beam_stride, segment_stride, segments, bytes)
+
+
 def test_workspaces_and_states_are_checked():
   assert lib().cuhnsw_lookup_grad_workspace(-1, 10, 8) == INVALID
   assert lib().cuhnsw_lookup_grad_workspace(5, 10, 0) == INVALID
@@ -87,13 +91,13 @@ def test_workspaces_and_states_are_checked():
   good = dict(src=A, dst=A, seq_stride=64, beam_stride=32, segment_stride=0, segments=1, bytes=32)
   for bad in (dict(src=None), dict(dst=None), dict(segments=-1), dict(bytes=-4), dict(seq_stride=-1), dict(beam_stride=-1),
               dict(segment_stride=-1)):
-    state = (table._State * 1)(table._State(**dict(good, **bad)))
+    state = state_of(**dict(good, **bad))
     assert lib().cuhnsw_reorder_device(state, 1, A, 2, 2, 2, None) == INVALID, bad
-  state = (table._State * 1)(table._State(**good))
+  state = state_of(**good)
   assert lib().cuhnsw_reorder_device(state, 1, None, 2, 2, 2, None) == INVALID
   assert lib().cuhnsw_reorder_device(None, 1, A, 2, 2, 2, None) == INVALID
   assert lib().cuhnsw_reorder_device(state, -1, A, 2, 2, 2, None) == INVALID
-  assert ctypes.sizeof(table._State) == 56
+  assert ctypes.sizeof(state) == 8 * table._STATE_WORDS
 
 
 def test_torch_layer_refuses_tensors_of_the_host():
