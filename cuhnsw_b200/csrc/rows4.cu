@@ -143,7 +143,8 @@ constexpr int kRowsPerLane = 2 * kRowTiles;   // of the first operand: rows g, g
 constexpr int kSumPitch = kWarpRows + 1;
 constexpr int kStages = 3;                    // of the ring
 constexpr int kStageBytes = kWarpRows * 64;
-constexpr int kMostScoreThreads = 512;
+// A CTA's warps where it has an SM for itself: with three and four tiles of columns sums need more registers than 16 warps leave.
+constexpr int most_score_warps(int tiles) { return tiles >= 3 ? 12 : 16; }
 
 template <int Bytes>
 __device__ __forceinline__ void copy_async(unsigned to, const void* from) {
@@ -156,39 +157,57 @@ __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_gro
 template <int Left>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(Left) : "memory"); }
 
+// (bits & mask) | magic in one instruction: that takes one constant, the other one has to be in a register already
+__device__ __forceinline__ unsigned and_or(unsigned bits, unsigned mask, unsigned magic) {
+  unsigned r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(bits), "r"(mask), "r"(magic));
+  return r;
+}
+__device__ __forceinline__ unsigned in_register(unsigned x) {
+  unsigned r;
+  asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+// c += a * b; `first`: c = a * b
+#define MMA16816(types, c, a, b0, b1, first)                                                                         \
+  if (first)                                                                                                         \
+    asm("mma.sync.aligned.m16n8k16.row.col.f32." types ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};" \
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])                                                             \
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));                                  \
+  else                                                                                                               \
+    asm("mma.sync.aligned.m16n8k16.row.col.f32." types ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"  \
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                                                             \
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1))
+
 struct PairsF16 {
+  unsigned magic = in_register(0x64006400u);  // 1024, the last bit of whose mantissa is one
+  unsigned minus_low = in_register(0xe408e408u), sixteenth = in_register(0x2c002c00u), minus_high = in_register(0xd480d480u);
   // two codes of nibbles `pair` and `pair` + 4 as code - 8
   template <int Pair>
-  static __device__ __forceinline__ unsigned values(unsigned w) {
+  __device__ __forceinline__ unsigned values(unsigned w) const {
     const unsigned u = Pair >= 2 ? w >> 8 : w;
-    if (Pair % 2 == 0) {
-      const unsigned v = (u & 0x000f000fu) | 0x64006400u;  // 1024 + code
-      const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), __half2half2(__ushort_as_half(0x6408)));
-      return *reinterpret_cast<const unsigned*>(&r);
-    }
-    const unsigned v = (u & 0x00f000f0u) | 0x64006400u;    // 1024 + 16 * code
-    const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&v), __half2half2(__ushort_as_half(0x2c00)),
-                              __half2half2(__ushort_as_half(0xd480)));  // / 16 - 72
-    return *reinterpret_cast<const unsigned*>(&r);
+    unsigned r;
+    if (Pair % 2 == 0)  // 1024 + code - 1032
+      asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(and_or(u, 0x000f000fu, magic)), "r"(minus_low));
+    else  // (1024 + 16 * code) / 16 - 72
+      asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(and_or(u, 0x00f000f0u, magic)), "r"(sixteenth), "r"(minus_high));
+    return r;
   }
-  static __device__ __forceinline__ void mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  static __device__ __forceinline__ void mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1, bool first) {
+    MMA16816("f16.f16", c, a, b0, b1, first);
   }
 };
 struct PairsBF16 {
+  unsigned magic = in_register(0x43004300u);  // 128
+  unsigned minus = in_register(0xc308c308u), one = in_register(0x3f803f80u);
   template <int Pair>
-  static __device__ __forceinline__ unsigned values(unsigned w) {
-    const unsigned v = ((w >> (4 * Pair)) & 0x000f000fu) | 0x43004300u;  // 128 + code
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v),
-                                     __bfloat162bfloat162(__ushort_as_bfloat16(0x4308)));
-    return *reinterpret_cast<const unsigned*>(&r);
+  __device__ __forceinline__ unsigned values(unsigned w) const {
+    unsigned r;  // 128 + code - 136
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(and_or(w >> (4 * Pair), 0x000f000fu, magic)), "r"(one), "r"(minus));
+    return r;
   }
-  static __device__ __forceinline__ void mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  static __device__ __forceinline__ void mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1, bool first) {
+    MMA16816("bf16.bf16", c, a, b0, b1, first);
   }
 };
 
@@ -222,39 +241,51 @@ struct ColumnsF32 {
 
 struct ScoreLayout {
   int queries;       // of a tile of columns: at most 8 * kTiles / parts
-  int pitch;         // values per column in shared memory
-  int chunk_fours;   // fours of blocks whose queries are in shared memory at a time
-  int split;         // warps that share 32 rows
+  int pitch;         // values per column of a buffer of queries in shared memory
+  int chunk_fours;   // fours of blocks whose queries are in a buffer: all of them, or there are two buffers in turn
+  int chunks;
+  int chunk_shift;   // logarithm of a chunk's words of eight values, where there are several
+  int split;         // warps that share 32 rows, of every chunk
   int column_tiles;
   int wide_queries;  // 16-byte loads of queries
   int wide_scales;   // loads of all scales of four blocks at once
 };
 
-// The queries' values of the dimensions [first, first + count) (a multiple of 8) to shared memory, zeros behind the last one.
+// The queries' values of the fours [first, first + count) to shared memory, zeros behind the last dimension.  Values that need
+// no change are copied asynchronously (`later`: the caller waits).
 template <class Columns>
-__device__ __forceinline__ void stage_queries(const Scores4Params& p, const ScoreLayout& l, long long q0, int nq,
-                                              long long first, int count, unsigned short* xs) {
+__device__ __forceinline__ void stage_queries(const Scores4Params& p, const ScoreLayout& l, long long q0, int nq, int first,
+                                              int count, bool later, unsigned short* xs) {
   using In = typename Columns::In;
-  const In* x = static_cast<const In*>(p.queries);
-  const int eights = count / 8;
-  for (int q = 0; q < nq; ++q) {
-    const In* src = x + (q0 + q) * p.query_stride + first;
-    for (int i = threadIdx.x; i < eights; i += blockDim.x) {
-      In v[8];
-      if (l.wide_queries && first + 8 * i + 8 <= p.d) {
-        load_many<In, 8>(src + 8 * i, v);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = first + 8 * i + j < p.d ? src[8 * i + j] : from_f32<In>(0.0f);
+  const int eights = count * (kFour / 8), most = l.chunk_fours * (kFour / 8);  // `most`: a power of two for chunks
+  const In* queries = static_cast<const In*>(p.queries) + q0 * p.query_stride + (long long)first * kFour;
+  const long long left = p.d - (long long)first * kFour;
+  for (int k = threadIdx.x; k < nq * most; k += blockDim.x) {
+    const int q = l.chunks > 1 ? k >> l.chunk_shift : k / most, i = k - q * most;
+    if (i >= eights) continue;
+    const In* src = queries + q * p.query_stride + 8 * i;
+    const bool whole = l.wide_queries && 8 * i + 8 <= left;
+    unsigned short* to = xs + q * l.pitch + 8 * i;
+    if constexpr (Columns::kParts == 1) {
+      if (later && whole) {
+        copy_async<16>((unsigned)__cvta_generic_to_shared(to), src);
+        continue;
       }
+    }
+    In v[8];
+    if (whole) {
+      load_many<In, 8>(src, v);
+    } else {
 #pragma unroll
-      for (int c = 0; c < Columns::kParts; ++c) {
-        unsigned w[4];
+      for (int j = 0; j < 8; ++j) v[j] = 8 * i + j < left ? src[j] : from_f32<In>(0.0f);
+    }
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          w[j] = (unsigned)Columns::part(v[2 * j], c) | ((unsigned)Columns::part(v[2 * j + 1], c) << 16);
-        *reinterpret_cast<uint4*>(xs + (c * nq + q) * l.pitch + 8 * i) = make_uint4(w[0], w[1], w[2], w[3]);
-      }
+    for (int c = 0; c < Columns::kParts; ++c) {
+      unsigned w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        w[j] = (unsigned)Columns::part(v[2 * j], c) | ((unsigned)Columns::part(v[2 * j + 1], c) << 16);
+      *reinterpret_cast<uint4*>(to + c * nq * l.pitch) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
 }
@@ -262,50 +293,40 @@ __device__ __forceinline__ void stage_queries(const Scores4Params& p, const Scor
 __device__ __forceinline__ float bf16_low(unsigned pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float bf16_high(unsigned pair) { return __uint_as_float(pair & 0xffff0000u); }
 
-// The scales of a row for four blocks: pairs of bfloat16
+// The scales of a row for four blocks: bfloat16, one to four of them.  `at`: the first one; left: how many there are from there on.
 template <int kGroup>
-struct FourScales;
-template <>
-struct FourScales<1> {
-  uint2 raw;
-  __device__ __forceinline__ void load(const unsigned short* row, int four, int, int groups, bool wide) {
-    if (wide) {
-      raw = *reinterpret_cast<const uint2*>(row + 4 * four);
+struct FourScales {
+  unsigned low = 0, high = 0;
+  __device__ __forceinline__ void load(const unsigned short* at, int left, bool wide) {
+    if constexpr (kGroup == 4) {
+      low = *at;
+    } else if constexpr (kGroup == 2) {
+      low = wide ? *reinterpret_cast<const unsigned*>(at) : at[0] | (left > 1 ? (unsigned)at[1] << 16 : 0);
+    } else if (wide) {
+      const uint2 both = *reinterpret_cast<const uint2*>(at);
+      low = both.x;
+      high = both.y;
     } else {
-      const unsigned short* at = row + 4 * four;
-      const int left = groups - 4 * four;
-      raw.x = at[0] | (left > 1 ? (unsigned)at[1] << 16 : 0);
-      raw.y = (left > 2 ? at[2] : 0) | (left > 3 ? (unsigned)at[3] << 16 : 0);
+      low = at[0] | (left > 1 ? (unsigned)at[1] << 16 : 0);
+      high = (left > 2 ? at[2] : 0) | (left > 3 ? (unsigned)at[3] << 16 : 0);
     }
   }
+  __device__ __forceinline__ FourScales of_lane(int lane) const {
+    FourScales r;
+    r.low = __shfl_sync(FULL, low, lane);
+    if (kGroup == 1) r.high = __shfl_sync(FULL, high, lane);
+    return r;
+  }
   __device__ __forceinline__ float get(int j) const {
-    return j == 0 ? bf16_low(raw.x) : j == 1 ? bf16_high(raw.x) : j == 2 ? bf16_low(raw.y) : bf16_high(raw.y);
+    const unsigned pair = j < 2 ? low : high;
+    return j % 2 == 0 ? bf16_low(pair) : bf16_high(pair);
   }
-};
-template <>
-struct FourScales<2> {
-  unsigned raw;
-  __device__ __forceinline__ void load(const unsigned short* row, int four, int, int groups, bool wide) {
-    if (wide)
-      raw = *reinterpret_cast<const unsigned*>(row + 2 * four);
-    else
-      raw = row[2 * four] | (groups - 2 * four > 1 ? (unsigned)row[2 * four + 1] << 16 : 0);
-  }
-  __device__ __forceinline__ float get(int j) const { return j == 0 ? bf16_low(raw) : bf16_high(raw); }
-};
-template <>
-struct FourScales<4> {
-  unsigned raw;
-  __device__ __forceinline__ void load(const unsigned short* row, int four, int group_fours, int, bool) {
-    raw = row[group_fours == 1 ? four : four / group_fours];
-  }
-  __device__ __forceinline__ float get(int) const { return bf16_low(raw); }
 };
 
 // kGroup: blocks of 32 dimensions per scale, 4 for four and more.  The parts of an fp32 query are the same column of three
 // operands, so that a lane holds all its sums.
 template <class Columns, int kTiles, int kGroup>
-__global__ void __launch_bounds__(kMostScoreThreads, 1) scores_kernel(const __grid_constant__ Scores4Params p,
+__global__ void __launch_bounds__(32 * most_score_warps(kTiles), 1) scores_kernel(const __grid_constant__ Scores4Params p,
                                                                       const __grid_constant__ ScoreLayout l) {
   using Pairs = typename Columns::Pairs;
   constexpr int kOutTiles = kTiles / Columns::kParts;
@@ -320,195 +341,221 @@ __global__ void __launch_bounds__(kMostScoreThreads, 1) scores_kernel(const __gr
   const unsigned ring = (unsigned)__cvta_generic_to_shared(smem) + warp * (kStages * kStageBytes) + 16 * lane;
   float* sums = reinterpret_cast<float*>(smem + warps * kStages * kStageBytes);
   unsigned short* xs = reinterpret_cast<unsigned short*>(sums + warps * 8 * kSumPitch);
+  const int buffer = l.queries * Columns::kParts * l.pitch;  // of the second buffer of queries
   const int blocks = (int)((p.d + kBlock - 1) / kBlock), fours = (blocks + 3) / 4;
   const int groups = (int)packed_groups_device(p.d, p.group), group_fours = (int)(p.group / kFour);
   const int row_bytes = 16 * blocks;
   const unsigned rows = (unsigned)p.n;
-  const unsigned char* codes = static_cast<const unsigned char*>(p.codes);
-  const unsigned short* scales = static_cast<const unsigned short*>(p.scales);
   const int units = (int)((p.n + kWarpRows * sets - 1) / (kWarpRows * sets));
-
-  for (int chunk = 0; chunk < fours; chunk += l.chunk_fours) {
-    const int in_chunk = min(l.chunk_fours, fours - chunk);
-    const int each = (in_chunk + l.split - 1) / l.split;
-    const int from = chunk + min(part * each, in_chunk), to = min(chunk + in_chunk, from + each);
-    int ahead_unit = first_unit, ahead_four = from;  // what is copied next
-    unsigned ahead_slot = 0;
-    auto copy = [&] {
-      if (ahead_unit < units && from < to) {
-        const unsigned row0 = (unsigned)(ahead_unit * sets + set) * kWarpRows + g;
-        const int m = min(4, blocks - 4 * ahead_four);
-        const int at = 64 * ahead_four + 4 * t * m;
-        const unsigned slot = ring + ahead_slot;
+  // a warp's last rows are the table's last 32: some of them are another warp's as well, which writes them
+  const unsigned last_start = max(rows, (unsigned)kWarpRows) - kWarpRows;
+  auto first_row = [&](int unit) { return min((unsigned)(unit * sets + set) * kWarpRows, last_start); };
+  int row_at[kRowsPerLane];
 #pragma unroll
+  for (int i = 0; i < kRowsPerLane; ++i) row_at[i] = (int)min((unsigned)(g + 8 * i), rows - 1) * row_bytes + 16 * t;
+  // the lanes of a row load the scales of a row each: t those of row g + 8 * t
+  const int scale_at = (int)min((unsigned)(g + 8 * t), rows - 1) * groups;
+  const Pairs pairs;
+
+  // The way through the rows: the fours of this warp's share of every chunk, unit after unit, two ahead of the sums.
+  const int share = (l.chunk_fours + l.split - 1) / l.split, first_four = part * share;
+  int ahead_unit = first_four < min(l.chunk_fours, fours) ? first_unit : units;
+  int ahead_four = first_four, ahead_left = min(share, fours - first_four);  // until the share of this chunk ends
+  unsigned ahead_slot = ring;
+  const unsigned char* src = nullptr;
+  const unsigned short* scale_src = nullptr;
+  FourScales<kGroup> scale, scale_1, scale_2;  // of the next four, of the one after it, ..
+  auto start_unit = [&] {
+    src = static_cast<const unsigned char*>(p.codes) + (long long)first_row(ahead_unit) * row_bytes + 64 * ahead_four;
+    scale_src = static_cast<const unsigned short*>(p.scales) + (long long)first_row(ahead_unit) * groups + scale_at;
+  };
+  if (ahead_unit < units) start_unit();
+  auto copy = [&] {
+    if (ahead_unit < units) {
+      if (4 * ahead_four + 4 <= blocks) {
+#pragma unroll
+        for (int i = 0; i < kRowsPerLane; ++i) copy_async<16>(ahead_slot + 512 * i, src + row_at[i]);
+      } else {
+        const int m = blocks - 4 * ahead_four;
+        const unsigned char* from = src + 4 * t * m - 16 * t;
         for (int i = 0; i < kRowsPerLane; ++i) {
-          // rows behind the last one are read as the last one and not written
-          const unsigned char* src = codes + (long long)min(row0 + 8 * i, rows - 1) * row_bytes + at;
-          if (m == 4) {
-            copy_async<16>(slot + 512 * i, src);
-          } else if (m == 2) {
-            copy_async<8>(slot + 512 * i, src);
+          if (m == 2) {
+            copy_async<8>(ahead_slot + 512 * i, from + row_at[i]);
           } else {
-            copy_async<4>(slot + 512 * i, src);
-            if (m == 3) {
-              copy_async<4>(slot + 512 * i + 4, src + 4);
-              copy_async<4>(slot + 512 * i + 8, src + 8);
-            }
+            for (int j = 0; j < m; ++j) copy_async<4>(ahead_slot + 512 * i + 4 * j, from + row_at[i] + 4 * j);
           }
         }
-        if (++ahead_four == to) {
-          ahead_four = from;
-          ahead_unit += step;
-        }
       }
-      ahead_slot = ahead_slot == (kStages - 1) * kStageBytes ? 0 : ahead_slot + kStageBytes;
-      copies_end();
-    };
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) copy();
-    if (chunk > 0) __syncthreads();
-    stage_queries<Columns>(p, l, q0, nq, (long long)chunk * kFour, in_chunk * kFour, xs);
-    __syncthreads();
-    // lanes of columns that there are not read the last one's and throw the result away
-    const unsigned short* column = xs + 8 * t;
+      const int at = kGroup < 4 ? ahead_four * (4 / kGroup) : group_fours == 1 ? ahead_four : ahead_four / group_fours;
+      scale_2.load(scale_src + at, groups - at, l.wide_scales);
+      ++ahead_four;
+      src += 64;
+      if (--ahead_left == 0) {
+        ahead_four += l.chunk_fours - share;
+        src += 64 * (l.chunk_fours - share);
+        if (ahead_four >= fours) {
+          ahead_four = first_four;
+          ahead_unit += step;
+          if (ahead_unit < units) start_unit();
+        }
+        ahead_left = min(share, fours - ahead_four);
+      }
+    }
+    ahead_slot = ahead_slot == ring + (kStages - 1) * kStageBytes ? ring : ahead_slot + kStageBytes;
+    copies_end();
+  };
+  static_assert(kStages == 3, "scale, scale_1 and scale_2");
+  copy();
+  scale = scale_2;
+  copy();
+  scale_1 = scale_2;
+  stage_queries<Columns>(p, l, q0, nq, 0, min(l.chunk_fours, fours), false, xs);
 
-    unsigned slot = 0;
-    FourScales<kGroup> scale[kRowsPerLane];
-    auto load_scales = [&](int unit, int four) {
-      const unsigned row0 = (unsigned)(unit * sets + set) * kWarpRows + g;
+  // lanes of columns that there are not read the last one's and throw the result away
+  int column[kTiles];
 #pragma unroll
-      for (int i = 0; i < kRowsPerLane; ++i)
-        scale[i].load(scales + (long long)min(row0 + 8 * i, rows - 1) * groups, four, group_fours, groups, l.wide_scales);
-    };
-    if (first_unit < units && from < to) load_scales(first_unit, from);
-    for (int unit = first_unit; unit < units; unit += step) {
-      float total[kRowTiles][kTiles][4];
+  for (int i = 0; i < kTiles; ++i)
+    column[i] = (Columns::kParts == 1 ? min(8 * i + g, nq - 1) : i * nq + min(g, nq - 1)) * l.pitch + 8 * t;
+  unsigned slot = ring;
+  int current = 0;  // buffer of the queries
+  __syncthreads();
+
+  for (int unit = first_unit; unit < units; unit += step) {
+    float total[kRowTiles][kTiles][4];
 #pragma unroll
-      for (int r = 0; r < kRowTiles; ++r)
+    for (int r = 0; r < kRowTiles; ++r)
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i)
+      for (int i = 0; i < kTiles; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) total[r][i][j] = 0.0f;
-      for (int four = from; four < to; ++four) {
+        for (int j = 0; j < 4; ++j) total[r][i][j] = 0.0f;
+    for (int chunk = 0; chunk < l.chunks; ++chunk) {
+      const int base = chunk * l.chunk_fours;
+      const int from = base + first_four, to = min(min(fours, base + l.chunk_fours), from + share);
+      if (l.chunks > 1 && (chunk + 1 < l.chunks || unit + step < units)) {
+        const int next = chunk + 1 < l.chunks ? base + l.chunk_fours : 0;
+        stage_queries<Columns>(p, l, q0, nq, next, min(l.chunk_fours, fours - next), true, xs + (current ^ 1) * buffer);
+      }
+      const unsigned short* values = xs + current * buffer + first_four * kFour;
+#pragma unroll 1
+      for (int four = from; four < to; ++four, values += kFour) {
         copy();
         copies_wait<kStages - 1>();
-        FourScales<kGroup> now[kRowsPerLane];
-#pragma unroll
-        for (int i = 0; i < kRowsPerLane; ++i) now[i] = scale[i];
-        if (four + 1 < to)
-          load_scales(unit, four + 1);
-        else if (unit + step < units)
-          load_scales(unit + step, from);
         uint4 w[kRowsPerLane];
 #pragma unroll
         for (int i = 0; i < kRowsPerLane; ++i)
           asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
                        : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w)
-                       : "r"(ring + slot + 512 * i)
+                       : "r"(slot + 512 * i)
                        : "memory");
-        slot = slot == (kStages - 1) * kStageBytes ? 0 : slot + kStageBytes;
-        const int m = min(4, blocks - 4 * four);
-        const unsigned short* values = column + (four - chunk) * kFour;
+        slot = slot == ring + (kStages - 1) * kStageBytes ? ring : slot + kStageBytes;
+        FourScales<kGroup> use[kRowsPerLane];
+#pragma unroll
+        for (int i = 0; i < kRowsPerLane; ++i) use[i] = scale.of_lane((lane & ~3) + i);
+        scale = scale_1;
+        scale_1 = scale_2;
         float sum[kRowTiles][kTiles][4];
+        auto block = [&](int j) {
+          uint4 b[kTiles];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (j % kGroup == 0) {
+          for (int i = 0; i < kTiles; ++i) b[i] = *reinterpret_cast<const uint4*>(values + column[i] + j * kBlock);
 #pragma unroll
-            for (int r = 0; r < kRowTiles; ++r)
+          for (int r = 0; r < kRowTiles; ++r) {
+            const uint4& low = w[2 * r];
+            const uint4& high = w[2 * r + 1];
+            const unsigned wa = j == 0 ? low.x : j == 1 ? low.y : j == 2 ? low.z : low.w;
+            const unsigned wb = j == 0 ? high.x : j == 1 ? high.y : j == 2 ? high.z : high.w;
+            const unsigned a0[4] = {pairs.template values<0>(wa), pairs.template values<0>(wb),
+                                    pairs.template values<1>(wa), pairs.template values<1>(wb)};
+            const unsigned a1[4] = {pairs.template values<2>(wa), pairs.template values<2>(wb),
+                                    pairs.template values<3>(wa), pairs.template values<3>(wb)};
 #pragma unroll
-              for (int i = 0; i < kTiles; ++i)
+            for (int i = 0; i < kTiles; ++i) Pairs::mma(sum[r][i], a0, b[i].x, b[i].y, j % kGroup == 0);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) sum[r][i][k] = 0.0f;
+            for (int i = 0; i < kTiles; ++i) Pairs::mma(sum[r][i], a1, b[i].z, b[i].w, false);
           }
-          if (j < m) {
-            uint4 b[kTiles];
+        };
+        auto add = [&](int j) {
+#pragma unroll
+          for (int r = 0; r < kRowTiles; ++r) {
+            const float fa = use[2 * r].get(j / kGroup), fb = use[2 * r + 1].get(j / kGroup);
 #pragma unroll
             for (int i = 0; i < kTiles; ++i) {
-              const int c = Columns::kParts == 1 ? min(8 * i + g, nq - 1) : i * nq + min(g, nq - 1);
-              b[i] = *reinterpret_cast<const uint4*>(values + c * l.pitch + j * kBlock);
-            }
-#pragma unroll
-            for (int r = 0; r < kRowTiles; ++r) {
-              const uint4& low = w[2 * r];
-              const uint4& high = w[2 * r + 1];
-              const unsigned wa = j == 0 ? low.x : j == 1 ? low.y : j == 2 ? low.z : low.w;
-              const unsigned wb = j == 0 ? high.x : j == 1 ? high.y : j == 2 ? high.z : high.w;
-              const unsigned a0[4] = {Pairs::template values<0>(wa), Pairs::template values<0>(wb),
-                                      Pairs::template values<1>(wa), Pairs::template values<1>(wb)};
-              const unsigned a1[4] = {Pairs::template values<2>(wa), Pairs::template values<2>(wb),
-                                      Pairs::template values<3>(wa), Pairs::template values<3>(wb)};
-#pragma unroll
-              for (int i = 0; i < kTiles; ++i) {
-                Pairs::mma(sum[r][i], a0, b[i].x, b[i].y);
-                Pairs::mma(sum[r][i], a1, b[i].z, b[i].w);
-              }
+              total[r][i][0] += fa * sum[r][i][0];
+              total[r][i][1] += fa * sum[r][i][1];
+              total[r][i][2] += fb * sum[r][i][2];
+              total[r][i][3] += fb * sum[r][i][3];
             }
           }
-          if ((j + 1) % kGroup == 0 && j / kGroup * kGroup < m) {
+        };
+        if (4 * four + 4 <= blocks) {
 #pragma unroll
-            for (int r = 0; r < kRowTiles; ++r) {
-              const float fa = now[2 * r].get(j / kGroup), fb = now[2 * r + 1].get(j / kGroup);
+          for (int j = 0; j < 4; ++j) {
+            block(j);
+            if ((j + 1) % kGroup == 0) add(j);
+          }
+        } else {
+          const int m = blocks - 4 * four;
 #pragma unroll
-              for (int i = 0; i < kTiles; ++i) {
-                total[r][i][0] += fa * sum[r][i][0];
-                total[r][i][1] += fa * sum[r][i][1];
-                total[r][i][2] += fb * sum[r][i][2];
-                total[r][i][3] += fb * sum[r][i][3];
-              }
+          for (int j = 0; j < 3; ++j) {
+            if (j < m) {
+              block(j);
+              if ((j + 1) % kGroup == 0 || j == m - 1) add(j);
             }
           }
         }
       }
-      // through shared memory, eight columns at a time: rows next to each other, the shares added up
-      float* mine = sums + warp * 8 * kSumPitch;
-      const int set_rows = kWarpRows * sets;
-#pragma unroll
-      for (int i = 0; i < kOutTiles; ++i) {
-        const int some = min(8, nq - 8 * i);
-        if (some <= 0) break;
-#pragma unroll
-        for (int r = 0; r < kRowsPerLane; ++r) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float y = total[r / 2][i * Columns::kParts][2 * (r % 2) + c];
-            if constexpr (Columns::kParts == 3)
-              y += total[r / 2][i * Columns::kParts + 1][2 * (r % 2) + c] +
-                   total[r / 2][i * Columns::kParts + 2][2 * (r % 2) + c];
-            mine[(2 * t + c) * kSumPitch + g + 8 * r] = y;
-          }
-        }
-        auto write = [&](float y, int q, long long row) {
-          float* out = p.out + (q0 + 8 * i + q) * p.n + row;
-          if (chunk > 0)
-            y += *out;
-          else if (p.bias)
-            y += p.bias[row];
-          *out = y;
-        };
-        if (l.split == 1) {
-          __syncwarp();
-          const long long row = (long long)(unit * sets + set) * kWarpRows + lane;
-          if (row < p.n)
-            for (int q = 0; q < some; ++q) write(mine[q * kSumPitch + lane], q, row);
-          __syncwarp();
-        } else {
-          __syncthreads();
-          for (int k = threadIdx.x; k < some * set_rows; k += blockDim.x) {
-            const int q = k / set_rows, r = k % set_rows;
-            const long long row = (long long)unit * set_rows + r;
-            if (row < p.n) {
-              const float* of_set = sums + ((r / kWarpRows) * l.split * 8 + q) * kSumPitch + r % kWarpRows;
-              float y = of_set[0];
-              for (int s = 1; s < l.split; ++s) y += of_set[s * 8 * kSumPitch];
-              write(y, q, row);
-            }
-          }
-          __syncthreads();
-        }
+      if (l.chunks > 1) {
+        // the next queries were copied with the first of this chunk's codes: three steps later they have arrived
+        if (to - from < kStages) copies_end(), copies_wait<0>();
+        __syncthreads();
+        current ^= 1;
       }
     }
-    copies_wait<0>();
+    // through shared memory, eight columns at a time: rows next to each other, the shares added up
+    float* mine = sums + warp * 8 * kSumPitch;
+#pragma unroll
+    for (int i = 0; i < kOutTiles; ++i) {
+      const int some = min(8, nq - 8 * i);
+      if (some <= 0) break;
+#pragma unroll
+      for (int r = 0; r < kRowsPerLane; ++r) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float y = total[r / 2][i * Columns::kParts][2 * (r % 2) + c];
+          if constexpr (Columns::kParts == 3)
+            y += total[r / 2][i * Columns::kParts + 1][2 * (r % 2) + c] +
+                 total[r / 2][i * Columns::kParts + 2][2 * (r % 2) + c];
+          mine[(2 * t + c) * kSumPitch + g + 8 * r] = y;
+        }
+      }
+      float* out = p.out + (q0 + 8 * i) * p.n;
+      if (l.split == 1) {
+        __syncwarp();
+        const unsigned row = first_row(unit) + lane;
+        if (row < rows && row >= (unsigned)(unit * sets + set) * kWarpRows) {
+          const float bias = p.bias ? p.bias[row] : 0.0f;
+          for (int q = 0; q < some; ++q) out[q * p.n + row] = mine[q * kSumPitch + lane] + bias;
+        }
+        __syncwarp();
+      } else {
+        __syncthreads();
+        // a warp takes a set's 32 rows of one column at a time
+        for (int k = warp; k < some * sets; k += warps) {
+          const int q = k / sets, s = k % sets;
+          const unsigned nominal = (unsigned)(unit * sets + s) * kWarpRows;
+          const unsigned row = min(nominal, last_start) + lane;
+          if (row < rows && row >= nominal) {
+            const float* of_set = sums + (s * l.split * 8 + q) * kSumPitch + lane;
+            float y = of_set[0];
+            for (int other = 1; other < l.split; ++other) y += of_set[other * 8 * kSumPitch];
+            out[q * p.n + row] = y + (p.bias ? p.bias[row] : 0.0f);
+          }
+        }
+        __syncthreads();
+      }
+    }
   }
+  copies_wait<0>();
 }
 
 template <class Columns, int kTiles, int kGroup>
@@ -518,32 +565,48 @@ cudaError_t scores_t(const Scores4Params& p, int queries, cudaStream_t stream) {
   l.queries = (int)(p.nq < queries ? p.nq : queries);
   const int columns = l.queries * Columns::kParts;
   const int fours = (int)((p.d + kFour - 1) / kFour);
+  l.column_tiles = (int)((p.nq + l.queries - 1) / l.queries);
   auto space = [&](int warps, int in_chunk) {
     // eight lanes read 16 bytes of two columns and four parts: half a row of banks from column to column
-    return (size_t)columns * (in_chunk * kFour + 32) * 2 + (size_t)warps * (kStages * kStageBytes + 8 * kSumPitch * 4);
+    return (size_t)columns * (in_chunk * kFour + 32) * 2 * (in_chunk < fours ? 2 : 1) +
+           (size_t)warps * (kStages * kStageBytes + 8 * kSumPitch * 4);
   };
-  // two CTAs of eight warps per SM, or one of as many as the queries leave room for
-  int warps = 8;
+  // two CTAs of eight warps per SM, or one of as many as the queries leave room for; queries that do not fit pass through
+  // shared memory in chunks, for all warps of a CTA together
+  const long long sets = (p.n + kWarpRows - 1) / kWarpRows;
+  int warps = 8, per_sm = 2;
   l.chunk_fours = fours;
-  const bool two = space(8, fours) <= kHalfSpace;
-  if (!two) {
-    warps = 16;
+  if (kTiles >= 3 || space(8, fours) > kHalfSpace) {
+    per_sm = 1;
+    warps = most_score_warps(kTiles);
     while (warps > 8 && space(warps, fours) > kMostSpace) warps -= 4;
-    while (space(warps, l.chunk_fours) > kMostSpace) l.chunk_fours = (l.chunk_fours + 1) / 2;
+    if (space(warps, fours) > kMostSpace) {
+      warps = most_score_warps(kTiles);
+      l.chunk_fours = 4;
+    }
   }
+  // How many warps share 32 rows: what takes the CTA with the most units the least time, in steps of four blocks.  The end of a
+  // unit takes about two of them, four where sums of several warps are added up.
+  const long long room = ((long long)kSMs * per_sm + l.column_tiles - 1) / l.column_tiles;
+  const bool chunked = l.chunk_fours < fours;
+  long long least = 0;
+  l.split = 1;
+  for (int split = 1; split <= (warps == 12 ? 4 : 8) && split <= fours; split *= 2) {
+    if (chunked && (split > 4 || space(warps, 4 * split) > kMostSpace)) break;
+    const long long units = (sets + warps / split - 1) / (warps / split), steps = (fours + split - 1) / split;
+    const long long time = (units + room - 1) / room * (steps + (split == 1 ? 2 : 4));
+    if (split == 1 || time < least) {
+      least = time;
+      l.split = split;
+    }
+  }
+  if (chunked) l.chunk_fours = 4 * l.split;
+  l.chunk_shift = 6 + (l.split == 4 ? 2 : l.split == 2 ? 1 : 0);
+  l.chunks = (fours + l.chunk_fours - 1) / l.chunk_fours;
   l.pitch = l.chunk_fours * kFour + 32;
   const size_t smem = space(warps, l.chunk_fours);
-  l.column_tiles = (int)((p.nq + l.queries - 1) / l.queries);
-  // several units for every CTA, and something to do for every warp
-  const long long sets = (p.n + kWarpRows - 1) / kWarpRows;
-  const long long room = (long long)kSMs * (two ? 2 : 1);
-  l.split = 1;
-  while (l.split < (warps == 12 ? 4 : 8) && 2 * l.split <= l.chunk_fours &&
-         sets * l.split * l.column_tiles < 8 * room * warps)
-    l.split *= 2;
   const long long units = (sets + warps / l.split - 1) / (warps / l.split);
-  long long step = (room + l.column_tiles - 1) / l.column_tiles;
-  if (step > units) step = units;
+  const long long step = room < units ? room : units;
   if (step * l.column_tiles > 0x7fffffffll) return cudaErrorInvalidValue;
   l.wide_queries = word_bytes(reinterpret_cast<uintptr_t>(p.queries) |
                               (unsigned long long)(p.query_stride * sizeof(typename Columns::In))) == 16;
@@ -564,12 +627,11 @@ cudaError_t scores_group(const Scores4Params& p, int queries, cudaStream_t strea
 
 template <class Columns>
 cudaError_t scores_columns(const Scores4Params& p, cudaStream_t stream) {
-  // as many queries at a time as fit into the operands' columns and, with all their dimensions, into shared memory; then as many
-  // tiles of equal size as that takes
+  // as many queries at a time as the operands have columns, in tiles of equal size.  (fp32 queries are taken apart on
+  // their way into shared memory, which is better done once: fewer at a time where that makes them fit.)
   constexpr long long kSpace = 132 * 1024;
   const long long fit = kSpace / (Columns::kParts * 2 * ((p.d + kFour - 1) / kFour * kFour + 32));
-  long long queries = Columns::kParts == 1 ? 32 : 8;
-  if (fit < queries) queries = fit < 1 ? 1 : fit;
+  long long queries = Columns::kParts == 1 ? 32 : fit >= 4 && fit < 8 ? fit : 8;
   const long long tiles = (p.nq + queries - 1) / queries;
   queries = (p.nq + tiles - 1) / tiles;
   if constexpr (Columns::kParts == 3) {
