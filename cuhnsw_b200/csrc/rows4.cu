@@ -19,10 +19,9 @@ constexpr int kFour = 4 * kBlock;      // of four blocks
 __device__ __forceinline__ long long packed_groups_device(long long d, long long group) { return (d + group - 1) / group; }
 
 // Byte offset in a row of the word that holds dimensions 8 * index .. 8 * index + 7
-__device__ __forceinline__ long long word_offset(long long index, long long blocks) {
-  const long long four = index / 16, block = index / 4, t = index % 4;
-  const int m = (int)min(4ll, blocks - 4 * four);
-  return 64 * four + 4 * (t * m + (block - 4 * four));
+__device__ __forceinline__ int word_offset(int index, int blocks) {
+  const int four = index >> 4, block = (index >> 2) & 3, t = index & 3;
+  return 64 * four + 4 * (t * min(4, blocks - 4 * four) + block);
 }
 
 // ---- packing --------------------------------------------------------------------------------------------------------
@@ -30,99 +29,218 @@ __device__ __forceinline__ long long word_offset(long long index, long long bloc
 constexpr int kPackThreads = 256;
 
 template <class T, int N>
-__device__ __forceinline__ void load_eight(const T* row, long long dim, long long d, float (&v)[8]) {
+__device__ __forceinline__ void load_eight(const T* row, int dim, int d, T (&v)[8]) {
   if (dim + 8 <= d) {
 #pragma unroll
     for (int i = 0; i < 8; i += N) {
       T w[N];
       load_many<T, N>(row + dim + i, w);
 #pragma unroll
-      for (int j = 0; j < N; ++j) v[i + j] = to_f32(w[j]);
+      for (int j = 0; j < N; ++j) v[i + j] = w[j];
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = dim + i < d ? to_f32(row[dim + i]) : 0.0f;
-  }
-}
-
-// `lanes` lanes (a power of two, at most a warp) share a row, eight dimensions each at a time.  Bound: HBM bytes.
-template <class T, int N>
-__global__ void __launch_bounds__(kPackThreads) pack_kernel(const T* rows, long long row_stride, long long n, long long d,
-                                                            long long group, unsigned char* codes,
-                                                            __nv_bfloat16* scales, int lanes) {
-  const int lane = threadIdx.x % lanes;
-  const long long row = (long long)blockIdx.x * (kPackThreads / lanes) + threadIdx.x / lanes;
-  if ((threadIdx.x & ~31) / lanes + (long long)blockIdx.x * (kPackThreads / lanes) >= n) return;  // the whole warp
-  const bool live = row < n;
-  const T* src = rows + (live ? row : 0) * row_stride;
-  const long long blocks = (d + kBlock - 1) / kBlock, words = 4 * blocks, groups = packed_groups_device(d, group);
-  unsigned char* dst = codes + row * 16 * blocks;
-  const long long group_words = group / 8;
-  const int span = (int)min((long long)lanes, group_words);  // lanes that share a group at a time
-  for (long long first = 0; first < words; first += group_words > lanes ? group_words : lanes) {
-    // the largest magnitude of each group
-    const long long until = group_words > lanes ? min(first + group_words, words) : min(first + lanes, words);
-    float most = 0.0f, v[8];
-    for (long long w = first + lane; w < until; w += lanes) {
-      load_eight<T, N>(src, 8 * w, d, v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[i]));
-    }
-    for (int off = 1; off < span; off <<= 1) most = fmaxf(most, __shfl_xor_sync(FULL, most, off));
-    const __nv_bfloat16 scale = __float2bfloat16_rn(__fmul_rn(most, 1.0f / 7.0f));
-    const float step = __bfloat162float(scale);
-    for (long long w = first + lane; w < until; w += lanes) {
-      if (until - first > lanes) load_eight<T, N>(src, 8 * w, d, v);
-      unsigned word = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float q = step > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(v[i], step)), -8.0f), 7.0f) : 0.0f;
-        const unsigned code = (unsigned)((int)q + 8);
-        word |= code << (4 * ((i >> 1) + 4 * (i & 1)));
-      }
-      if (live) *reinterpret_cast<unsigned*>(dst + word_offset(w, blocks)) = word;
-      if (live && w % group_words == 0 && w / group_words < groups) scales[row * groups + w / group_words] = scale;
-    }
+    for (int i = 0; i < 8; ++i) v[i] = dim + i < d ? row[dim + i] : from_f32<T>(0.0f);
   }
 }
 
 template <class T>
-__global__ void __launch_bounds__(kPackThreads) unpack_kernel(const unsigned char* codes, const __nv_bfloat16* scales,
-                                                              long long n, long long d, long long group, T* out) {
-  const long long blocks = (d + kBlock - 1) / kBlock, words = (d + 7) / 8, groups = packed_groups_device(d, group);
-  const long long step = (long long)gridDim.x * kPackThreads;
-  for (long long at = (long long)blockIdx.x * kPackThreads + threadIdx.x; at < n * words; at += step) {
-    const long long row = at / words, w = at % words;
-    const unsigned word = *reinterpret_cast<const unsigned*>(codes + row * 16 * blocks + word_offset(w, blocks));
-    const float scale = __bfloat162float(scales[row * groups + 8 * w / group]);
-    T* to = out + row * d + 8 * w;
+__device__ __forceinline__ float largest(const T (&v)[8], float most) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int code = (word >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15;
-      if (8 * w + i < d) to[i] = from_f32<T>((float)(code - 8) * scale);
+  for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(to_f32(v[i])));
+  return most;
+}
+
+__device__ __forceinline__ __nv_bfloat16 scale_of(float most) { return __float2bfloat16_rn(__fmul_rn(most, 1.0f / 7.0f)); }
+
+template <class T>
+__device__ __forceinline__ unsigned codes_of(const T (&v)[8], float step) {
+  // A product with the reciprocal is off by 2^-21 at most: only where it comes that near to the middle of two codes does the
+  // quotient itself have to be rounded (and for steps whose reciprocal is no ordinary number).
+  const bool plain = step > 1e-36f && step < 1e36f;
+  const float inverse = plain ? __frcp_rn(step) : 0.0f;
+  unsigned word = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float x = to_f32(v[i]);
+    const float quotient = x * inverse;
+    float q = rintf(quotient);
+    if (fabsf(fabsf(quotient - q) - 0.5f) < 1e-5f || !plain) q = step > 0.0f ? rintf(__fdiv_rn(x, step)) : 0.0f;
+    const int code = (int)fminf(fmaxf(q, -8.0f), 7.0f) + 8;
+    word |= (unsigned)code << (4 * ((i >> 1) + 4 * (i & 1)));
+  }
+  return word;
+}
+
+// `lanes` lanes (a power of two, at most a warp) take as many words of eight dimensions of a row at a time, whole groups; kAt times
+// in a row before they look at the first.  Bound: HBM bytes.
+template <class T, int N, int kAt>
+__global__ void __launch_bounds__(kPackThreads) pack_kernel(const T* rows, long long row_stride, long long n, int d,
+                                                            int group_words, unsigned char* codes, __nv_bfloat16* scales,
+                                                            int lanes) {
+  const int lane = threadIdx.x & (lanes - 1);
+  const int blocks = (d + kBlock - 1) / kBlock, words = 4 * blocks, pieces = (words + lanes - 1) / lanes;
+  const int groups = (d + 8 * group_words - 1) / (8 * group_words);
+  const int span = min(lanes, group_words);
+  const long long first = ((long long)blockIdx.x * (kPackThreads / lanes) + threadIdx.x / lanes) * kAt;
+  long long row = first / pieces;
+  int piece = (int)(first - row * pieces);
+  T v[kAt][8];
+  long long row_of[kAt];
+  int word_of[kAt];
+#pragma unroll
+  for (int k = 0; k < kAt; ++k) {
+    row_of[k] = row;
+    word_of[k] = piece * lanes + lane;
+    if (row < n) {
+      load_eight<T, N>(rows + row * row_stride, 8 * word_of[k], d, v[k]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[k][i] = from_f32<T>(0.0f);
+    }
+    if (++piece == pieces) {
+      piece = 0;
+      ++row;
     }
   }
+#pragma unroll
+  for (int k = 0; k < kAt; ++k) {
+    float most = largest(v[k], 0.0f);
+    for (int off = 1; off < span; off <<= 1) most = fmaxf(most, __shfl_xor_sync(FULL, most, off));
+    const __nv_bfloat16 scale = scale_of(most);
+    const int w = word_of[k];
+    if (row_of[k] < n && w < words) {
+      const unsigned word = codes_of(v[k], __bfloat162float(scale));
+      *reinterpret_cast<unsigned*>(codes + row_of[k] * (16ll * blocks) + word_offset(w, blocks)) = word;
+      if ((w & (group_words - 1)) == 0 && w / group_words < groups) scales[row_of[k] * groups + w / group_words] = scale;
+    }
+  }
+}
+
+// Groups that are more than a warp's words: a warp per row, every group read twice.
+template <class T, int N>
+__global__ void __launch_bounds__(kPackThreads) pack_wide_kernel(const T* rows, long long row_stride, long long n, int d,
+                                                                 int group, unsigned char* codes, __nv_bfloat16* scales) {
+  const int lane = lane_id();
+  const long long row = (long long)blockIdx.x * (kPackThreads / 32) + (threadIdx.x >> 5);
+  if (row >= n) return;
+  const T* src = rows + row * row_stride;
+  const int blocks = (d + kBlock - 1) / kBlock, words = 4 * blocks, group_words = group / 8, groups = (d + group - 1) / group;
+  for (int g = 0; g < groups; ++g) {
+    const int first = g * group_words, until = min(first + group_words, words);
+    float most = 0.0f;
+    T v[8];
+    for (int w = first + lane; w < until; w += 32) {
+      load_eight<T, N>(src, 8 * w, d, v);
+      most = largest(v, most);
+    }
+    for (int off = 1; off < 32; off <<= 1) most = fmaxf(most, __shfl_xor_sync(FULL, most, off));
+    const __nv_bfloat16 scale = scale_of(most);
+    for (int w = first + lane; w < until; w += 32) {
+      load_eight<T, N>(src, 8 * w, d, v);
+      const unsigned word = codes_of(v, __bfloat162float(scale));
+      *reinterpret_cast<unsigned*>(codes + row * (16ll * blocks) + word_offset(w, blocks)) = word;
+    }
+    if (lane == 0) scales[row * groups + g] = scale;
+  }
+}
+
+// `lanes` threads share kUnpackRows rows, V neighbouring values of each at a time (V divides 8).
+constexpr int kUnpackRows = 4;
+template <class T, int V>
+__global__ void __launch_bounds__(kPackThreads) unpack_kernel(const unsigned char* codes, const __nv_bfloat16* scales,
+                                                              long long n, int d, int group, int group_shift, T* out,
+                                                              int lanes) {
+  const int lane = threadIdx.x & (lanes - 1);
+  const long long first = ((long long)blockIdx.x * (kPackThreads / lanes) + threadIdx.x / lanes) * kUnpackRows;
+  const int blocks = (d + kBlock - 1) / kBlock, groups = (d + group - 1) / group;
+  for (int dim = lane * V; dim < d; dim += lanes * V) {
+    const int at = word_offset(dim >> 3, blocks), g = group_shift >= 0 ? dim >> group_shift : dim / group;
+    unsigned word[kUnpackRows];
+    float scale[kUnpackRows];
+#pragma unroll
+    for (int r = 0; r < kUnpackRows; ++r) {
+      if (first + r < n) {
+        word[r] = __ldg(reinterpret_cast<const unsigned*>(codes + (first + r) * (16ll * blocks) + at));
+        scale[r] = __bfloat162float(scales[(first + r) * groups + g]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kUnpackRows; ++r) {
+      if (first + r < n) {
+        T v[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const int k = (dim & 7) + i;
+          const int code = (word[r] >> (4 * ((k >> 1) + 4 * (k & 1)))) & 15;
+          v[i] = from_f32<T>((float)(code - 8) * scale[r]);
+        }
+        store_many<T, V>(out + (first + r) * d + dim, v);
+      }
+    }
+  }
+}
+
+template <class T, int N>
+cudaError_t pack_n(const T* rows, long long row_stride, long long n, int d, long long group, void* codes, void* scales,
+                   cudaStream_t stream) {
+  const int words = 4 * ((d + kBlock - 1) / kBlock);
+  const int lanes = next_pow2(words, 32);
+  unsigned char* c = static_cast<unsigned char*>(codes);
+  __nv_bfloat16* s = static_cast<__nv_bfloat16*>(scales);
+  if (group / 8 > lanes && words > lanes) {
+    const long long blocks = (n + kPackThreads / 32 - 1) / (kPackThreads / 32);
+    if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
+    pack_wide_kernel<T, N><<<(unsigned)blocks, kPackThreads, 0, stream>>>(rows, row_stride, n, d, (int)group, c, s);
+    return cudaGetLastError();
+  }
+  // a group that is longer than the row is as good as one of all its words
+  const int group_words = group / 8 > lanes ? lanes : (int)(group / 8);
+  const long long pieces = n * ((words + lanes - 1) / lanes);
+  const bool many = pieces > (long long)4 * kSMs * (kPackThreads / lanes);
+  const long long per = (kPackThreads / lanes) * (many ? 4 : 1), blocks = (pieces + per - 1) / per;
+  if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
+  if (many)
+    pack_kernel<T, N, 4><<<(unsigned)blocks, kPackThreads, 0, stream>>>(rows, row_stride, n, d, group_words, c, s, lanes);
+  else
+    pack_kernel<T, N, 1><<<(unsigned)blocks, kPackThreads, 0, stream>>>(rows, row_stride, n, d, group_words, c, s, lanes);
+  return cudaGetLastError();
 }
 
 template <class T>
 cudaError_t pack_t(const T* rows, long long row_stride, long long n, long long d, long long group, void* codes,
                    void* scales, cudaStream_t stream) {
-  const int lanes = next_pow2(4 * ((d + kBlock - 1) / kBlock), 32);
-  const long long blocks = (n * lanes + kPackThreads - 1) / kPackThreads;
-  if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
   const int w = word_bytes(reinterpret_cast<uintptr_t>(rows) | (unsigned long long)(row_stride * sizeof(T)));
-#define PACK(N) pack_kernel<T, N><<<(unsigned)blocks, kPackThreads, 0, stream>>>( \
-    rows, row_stride, n, d, group, static_cast<unsigned char*>(codes), static_cast<__nv_bfloat16*>(scales), lanes)
-  if (w == 16)
-    PACK(16 / sizeof(T));
-  else if (w == 8)
-    PACK(8 / sizeof(T));
-  else if (w == 4)
-    PACK(4 / sizeof(T));
-  else
-    PACK(1);
-#undef PACK
+  if (w == 16) return pack_n<T, 16 / sizeof(T)>(rows, row_stride, n, (int)d, group, codes, scales, stream);
+  if (w == 8) return pack_n<T, 8 / sizeof(T)>(rows, row_stride, n, (int)d, group, codes, scales, stream);
+  if (w == 4) return pack_n<T, 4 / sizeof(T)>(rows, row_stride, n, (int)d, group, codes, scales, stream);
+  return pack_n<T, 1>(rows, row_stride, n, (int)d, group, codes, scales, stream);
+}
+
+template <class T, int V>
+cudaError_t unpack_v(const unsigned char* codes, const __nv_bfloat16* scales, long long n, int d, int group, T* out,
+                     cudaStream_t stream) {
+  const int lanes = next_pow2((d + V - 1) / V, kPackThreads);
+  const long long per = (long long)(kPackThreads / lanes) * kUnpackRows, blocks = (n + per - 1) / per;
+  if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
+  int shift = 0;
+  while ((1 << shift) < group) ++shift;
+  unpack_kernel<T, V><<<(unsigned)blocks, kPackThreads, 0, stream>>>(codes, scales, n, d, group,
+                                                                    (1 << shift) == group ? shift : -1, out, lanes);
   return cudaGetLastError();
+}
+
+template <class T>
+cudaError_t unpack_t(const void* codes, const void* scales, long long n, long long d, long long group, void* out,
+                     cudaStream_t stream) {
+  const unsigned char* c = static_cast<const unsigned char*>(codes);
+  const __nv_bfloat16* s = static_cast<const __nv_bfloat16*>(scales);
+  T* to = static_cast<T*>(out);
+  const int w = word_bytes(reinterpret_cast<uintptr_t>(out) | (unsigned long long)(d * sizeof(T)));
+  if (w == 16) return unpack_v<T, 16 / sizeof(T)>(c, s, n, (int)d, (int)group, to, stream);
+  if (w == 8) return unpack_v<T, 8 / sizeof(T)>(c, s, n, (int)d, (int)group, to, stream);
+  if (w == 4) return unpack_v<T, 4 / sizeof(T)>(c, s, n, (int)d, (int)group, to, stream);
+  return unpack_v<T, 1>(c, s, n, (int)d, (int)group, to, stream);
 }
 
 // ---- products -------------------------------------------------------------------------------------------------------
@@ -244,7 +362,6 @@ struct ScoreLayout {
   int pitch;         // values per column of a buffer of queries in shared memory
   int chunk_fours;   // fours of blocks whose queries are in a buffer: all of them, or there are two buffers in turn
   int chunks;
-  int chunk_shift;   // logarithm of a chunk's words of eight values, where there are several
   int split;         // warps that share 32 rows, of every chunk
   int column_tiles;
   int wide_queries;  // 16-byte loads of queries
@@ -257,27 +374,23 @@ template <class Columns>
 __device__ __forceinline__ void stage_queries(const Scores4Params& p, const ScoreLayout& l, long long q0, int nq, int first,
                                               int count, bool later, unsigned short* xs) {
   using In = typename Columns::In;
-  const int eights = count * (kFour / 8), most = l.chunk_fours * (kFour / 8);  // `most`: a power of two for chunks
+  const int eights = count * (kFour / 8), warps = blockDim.x >> 5;
   const In* queries = static_cast<const In*>(p.queries) + q0 * p.query_stride + (long long)first * kFour;
   const long long left = p.d - (long long)first * kFour;
-  for (int k = threadIdx.x; k < nq * most; k += blockDim.x) {
-    const int q = l.chunks > 1 ? k >> l.chunk_shift : k / most, i = k - q * most;
-    if (i >= eights) continue;
-    const In* src = queries + q * p.query_stride + 8 * i;
+  auto eight = [&](const In* src, unsigned short* to, int i) {
     const bool whole = l.wide_queries && 8 * i + 8 <= left;
-    unsigned short* to = xs + q * l.pitch + 8 * i;
     if constexpr (Columns::kParts == 1) {
       if (later && whole) {
-        copy_async<16>((unsigned)__cvta_generic_to_shared(to), src);
-        continue;
+        copy_async<16>((unsigned)__cvta_generic_to_shared(to + 8 * i), src + 8 * i);
+        return;
       }
     }
     In v[8];
     if (whole) {
-      load_many<In, 8>(src, v);
+      load_many<In, 8>(src + 8 * i, v);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = 8 * i + j < left ? src[j] : from_f32<In>(0.0f);
+      for (int j = 0; j < 8; ++j) v[j] = 8 * i + j < left ? src[8 * i + j] : from_f32<In>(0.0f);
     }
 #pragma unroll
     for (int c = 0; c < Columns::kParts; ++c) {
@@ -285,8 +398,18 @@ __device__ __forceinline__ void stage_queries(const Scores4Params& p, const Scor
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         w[j] = (unsigned)Columns::part(v[2 * j], c) | ((unsigned)Columns::part(v[2 * j + 1], c) << 16);
-      *reinterpret_cast<uint4*>(to + c * nq * l.pitch) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(to + c * nq * l.pitch + 8 * i) = make_uint4(w[0], w[1], w[2], w[3]);
     }
+  };
+  if (nq * 2 > warps) {  // a warp per query
+    for (int q = threadIdx.x >> 5; q < nq; q += warps) {
+      const In* src = queries + q * p.query_stride;
+      unsigned short* to = xs + q * l.pitch;
+      for (int i = lane_id(); i < eights; i += 32) eight(src, to, i);
+    }
+  } else {  // all warps for each query
+    for (int q = 0; q < nq; ++q)
+      for (int i = threadIdx.x; i < eights; i += blockDim.x) eight(queries + q * p.query_stride, xs + q * l.pitch, i);
   }
 }
 
@@ -421,6 +544,10 @@ __global__ void __launch_bounds__(32 * most_score_warps(kTiles), 1) scores_kerne
   __syncthreads();
 
   for (int unit = first_unit; unit < units; unit += step) {
+    // the row that this lane writes if its warp has rows for itself; its bias is on the way meanwhile
+    const unsigned mine_row = first_row(unit) + lane;
+    const bool writes = mine_row < rows && mine_row >= (unsigned)(unit * sets + set) * kWarpRows;
+    const float bias = p.bias && writes ? __ldg(p.bias + mine_row) : 0.0f;
     float total[kRowTiles][kTiles][4];
 #pragma unroll
     for (int r = 0; r < kRowTiles; ++r)
@@ -531,10 +658,11 @@ __global__ void __launch_bounds__(32 * most_score_warps(kTiles), 1) scores_kerne
       float* out = p.out + (q0 + 8 * i) * p.n;
       if (l.split == 1) {
         __syncwarp();
-        const unsigned row = first_row(unit) + lane;
-        if (row < rows && row >= (unsigned)(unit * sets + set) * kWarpRows) {
-          const float bias = p.bias ? p.bias[row] : 0.0f;
-          for (int q = 0; q < some; ++q) out[q * p.n + row] = mine[q * kSumPitch + lane] + bias;
+        if (writes) {
+          float* to_out = out + mine_row;
+          const float* from_sums = mine + lane;
+#pragma unroll 4
+          for (int q = 0; q < some; ++q, to_out += p.n, from_sums += kSumPitch) *to_out = *from_sums + bias;
         }
         __syncwarp();
       } else {
@@ -548,7 +676,7 @@ __global__ void __launch_bounds__(32 * most_score_warps(kTiles), 1) scores_kerne
             const float* of_set = sums + (s * l.split * 8 + q) * kSumPitch + lane;
             float y = of_set[0];
             for (int other = 1; other < l.split; ++other) y += of_set[other * 8 * kSumPitch];
-            out[q * p.n + row] = y + (p.bias ? p.bias[row] : 0.0f);
+            out[q * p.n + row] = y + (p.bias ? __ldg(p.bias + row) : 0.0f);
           }
         }
         __syncthreads();
@@ -585,23 +713,28 @@ cudaError_t scores_t(const Scores4Params& p, int queries, cudaStream_t stream) {
       l.chunk_fours = 4;
     }
   }
-  // How many warps share 32 rows: what takes the CTA with the most units the least time, in steps of four blocks.  The end of a
-  // unit takes about two of them, four where sums of several warps are added up.
+  // How many warps share 32 rows, and how many an SM's only CTA has: what takes the CTA with the most units the least time, in
+  // steps of four blocks of all its warps.  The end of a unit takes about two of them, four where sums of several warps are
+  // added up; chunks of queries are as many bytes as the codes of `columns` rows, for fewer rows the more warps share them.
   const long long room = ((long long)kSMs * per_sm + l.column_tiles - 1) / l.column_tiles;
   const bool chunked = l.chunk_fours < fours;
+  const int most_warps = warps;
   long long least = 0;
-  l.split = 1;
-  for (int split = 1; split <= (warps == 12 ? 4 : 8) && split <= fours; split *= 2) {
-    if (chunked && (split > 4 || space(warps, 4 * split) > kMostSpace)) break;
-    const long long units = (sets + warps / split - 1) / (warps / split), steps = (fours + split - 1) / split;
-    const long long time = (units + room - 1) / room * (steps + (split == 1 ? 2 : 4));
-    if (split == 1 || time < least) {
-      least = time;
-      l.split = split;
+  for (int w = most_warps; w >= (per_sm == 1 ? 8 : 6); --w) {
+    for (int split = 1; split <= 8 && split <= fours; split *= 2) {
+      if (w % split != 0 || (chunked && (split > 4 || space(w, 4 * split) > kMostSpace))) continue;
+      const long long units = (sets + w / split - 1) / (w / split), steps = (fours + split - 1) / split;
+      const long long time = (units + room - 1) / room * w *
+                             (steps + (chunked ? steps * columns * split / (32 * w) : 0) + (split == 1 ? 2 : 4));
+      // (fewer warps hide less: only for a gain of a twentieth)
+      if (least == 0 || (w == warps ? time < least : 20 * time < 19 * least)) {
+        least = time;
+        l.split = split;
+        warps = w;
+      }
     }
   }
   if (chunked) l.chunk_fours = 4 * l.split;
-  l.chunk_shift = 6 + (l.split == 4 ? 2 : l.split == 2 ? 1 : 0);
   l.chunks = (fours + l.chunk_fours - 1) / l.chunk_fours;
   l.pitch = l.chunk_fours * kFour + 32;
   const size_t smem = space(warps, l.chunk_fours);
@@ -657,18 +790,9 @@ cudaError_t launch_pack4(const void* rows, long long row_stride, int type, long 
 cudaError_t launch_unpack4(const void* codes, const void* scales, long long n, long long d, long long group, void* out,
                            int type, cudaStream_t stream) {
   if (n <= 0 || d <= 0) return cudaSuccess;
-  const unsigned char* c = static_cast<const unsigned char*>(codes);
-  const __nv_bfloat16* s = static_cast<const __nv_bfloat16*>(scales);
-  const long long items = n * ((d + 7) / 8);
-  const long long wanted = (items + kPackThreads - 1) / kPackThreads, room = kSMs * 32;
-  const unsigned blocks = (unsigned)(wanted < room ? wanted : room);
-  if (type == kF32)
-    unpack_kernel<float><<<blocks, kPackThreads, 0, stream>>>(c, s, n, d, group, static_cast<float*>(out));
-  else if (type == kF16)
-    unpack_kernel<__half><<<blocks, kPackThreads, 0, stream>>>(c, s, n, d, group, static_cast<__half*>(out));
-  else
-    unpack_kernel<__nv_bfloat16><<<blocks, kPackThreads, 0, stream>>>(c, s, n, d, group, static_cast<__nv_bfloat16*>(out));
-  return cudaGetLastError();
+  if (type == kF32) return unpack_t<float>(codes, scales, n, d, group, out, stream);
+  if (type == kF16) return unpack_t<__half>(codes, scales, n, d, group, out, stream);
+  return unpack_t<__nv_bfloat16>(codes, scales, n, d, group, out, stream);
 }
 
 cudaError_t launch_scores4(const Scores4Params& p, cudaStream_t stream) {
