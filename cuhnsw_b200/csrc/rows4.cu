@@ -55,65 +55,72 @@ __device__ __forceinline__ __nv_bfloat16 scale_of(float most) { return __float2b
 
 template <class T>
 __device__ __forceinline__ unsigned codes_of(const T (&v)[8], float step) {
-  // A product with the reciprocal is off by 2^-21 at most: only where it comes that near to the middle of two codes does the
-  // quotient itself have to be rounded (and for steps whose reciprocal is no ordinary number).
-  const bool plain = step > 1e-36f && step < 1e36f;
+  constexpr int kNibble[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+  // Added to a small number, this leaves its nearest whole number (the even one of two) in the last bits.
+  constexpr float kWhole = 12582912.0f;
+  constexpr unsigned kWholeBits = 0x4b400000u;
+  const bool plain = step > 1e-30f && step < 1e30f;
   const float inverse = plain ? __frcp_rn(step) : 0.0f;
   unsigned word = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float x = to_f32(v[i]);
-    const float quotient = x * inverse;
-    float q = rintf(quotient);
-    if (fabsf(fabsf(quotient - q) - 0.5f) < 1e-5f || !plain) q = step > 0.0f ? rintf(__fdiv_rn(x, step)) : 0.0f;
-    const int code = (int)fminf(fmaxf(q, -8.0f), 7.0f) + 8;
-    word |= (unsigned)code << (4 * ((i >> 1) + 4 * (i & 1)));
+    // The quotient, correctly rounded (16-bit values are halfway between two codes often enough): with a correctly rounded
+    // reciprocal one correction by the exact remainder does it (Markstein, Computation of elementary functions on the IBM RISC
+    // System/6000 processor, 1990).  Its magnitude is below 7.1, as the scale is the largest value's.
+    const float near = x * inverse;
+    const float quotient = __fmaf_rn(__fmaf_rn(-near, step, x), inverse, near);
+    word += (__float_as_uint(quotient + kWhole) - kWholeBits + 8) << (4 * kNibble[i]);
+  }
+  if (!plain) {  // no scale, or one whose reciprocal is no ordinary number
+    word = 0;
+    for (int i = 0; i < 8; ++i) {
+      const float q = step > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(to_f32(v[i]), step)), -8.0f), 7.0f) : 0.0f;
+      word |= (unsigned)((int)q + 8) << (4 * ((i >> 1) + 4 * (i & 1)));
+    }
   }
   return word;
 }
 
 // `lanes` lanes (a power of two, at most a warp) take as many words of eight dimensions of a row at a time, whole groups; kAt times
-// in a row before they look at the first.  Bound: HBM bytes.
-template <class T, int N, int kAt>
+// in a row before they look at the first: of kAt rows that are no longer than that, or of one row.  Bound: HBM bytes.
+template <class T, int N, int kAt, bool kLong>
 __global__ void __launch_bounds__(kPackThreads) pack_kernel(const T* rows, long long row_stride, long long n, int d,
-                                                            int group_words, unsigned char* codes, __nv_bfloat16* scales,
-                                                            int lanes) {
+                                                            int group_shift, int groups, unsigned char* codes,
+                                                            __nv_bfloat16* scales, int lanes) {
   const int lane = threadIdx.x & (lanes - 1);
-  const int blocks = (d + kBlock - 1) / kBlock, words = 4 * blocks, pieces = (words + lanes - 1) / lanes;
-  const int groups = (d + 8 * group_words - 1) / (8 * group_words);
-  const int span = min(lanes, group_words);
-  const long long first = ((long long)blockIdx.x * (kPackThreads / lanes) + threadIdx.x / lanes) * kAt;
-  long long row = first / pieces;
-  int piece = (int)(first - row * pieces);
-  T v[kAt][8];
-  long long row_of[kAt];
-  int word_of[kAt];
+  const int blocks = (d + kBlock - 1) / kBlock, words = 4 * blocks, span = min(lanes, 1 << group_shift);
+  const long long team = (long long)blockIdx.x * (kPackThreads / lanes) + threadIdx.x / lanes;
+  const long long row = kLong ? team : team * kAt;
+  const T* src = rows + row * row_stride;
+  unsigned char* dst = codes + row * (16ll * blocks);
+  __nv_bfloat16* to_scales = scales + row * groups;
+  for (int first = lane; first - lane < words; first += kAt * lanes) {
+    T v[kAt][8];
 #pragma unroll
-  for (int k = 0; k < kAt; ++k) {
-    row_of[k] = row;
-    word_of[k] = piece * lanes + lane;
-    if (row < n) {
-      load_eight<T, N>(rows + row * row_stride, 8 * word_of[k], d, v[k]);
-    } else {
+    for (int k = 0; k < kAt; ++k) {
+      const int w = kLong ? first + k * lanes : first;
+      if (row + (kLong ? 0 : k) < n && 8 * w < d) {
+        load_eight<T, N>(src + (kLong ? 0 : k * row_stride), 8 * w, d, v[k]);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[k][i] = from_f32<T>(0.0f);
+        for (int i = 0; i < 8; ++i) v[k][i] = from_f32<T>(0.0f);
+      }
     }
-    if (++piece == pieces) {
-      piece = 0;
-      ++row;
-    }
-  }
 #pragma unroll
-  for (int k = 0; k < kAt; ++k) {
-    float most = largest(v[k], 0.0f);
-    for (int off = 1; off < span; off <<= 1) most = fmaxf(most, __shfl_xor_sync(FULL, most, off));
-    const __nv_bfloat16 scale = scale_of(most);
-    const int w = word_of[k];
-    if (row_of[k] < n && w < words) {
-      const unsigned word = codes_of(v[k], __bfloat162float(scale));
-      *reinterpret_cast<unsigned*>(codes + row_of[k] * (16ll * blocks) + word_offset(w, blocks)) = word;
-      if ((w & (group_words - 1)) == 0 && w / group_words < groups) scales[row_of[k] * groups + w / group_words] = scale;
+    for (int k = 0; k < kAt; ++k) {
+      const int w = kLong ? first + k * lanes : first;
+      float most = largest(v[k], 0.0f);
+      for (int off = 1; off < span; off <<= 1) most = fmaxf(most, __shfl_xor_sync(FULL, most, off));
+      const __nv_bfloat16 scale = scale_of(most);
+      if (row + (kLong ? 0 : k) < n && w < words) {
+        const unsigned word = codes_of(v[k], __bfloat162float(scale));
+        *reinterpret_cast<unsigned*>(dst + (kLong ? 0 : k * (16ll * blocks)) + word_offset(w, blocks)) = word;
+        const int g = w >> group_shift;
+        if (g << group_shift == w && g < groups) to_scales[(kLong ? 0 : k * groups) + g] = scale;
+      }
     }
+    if (!kLong) break;
   }
 }
 
@@ -145,38 +152,35 @@ __global__ void __launch_bounds__(kPackThreads) pack_wide_kernel(const T* rows, 
   }
 }
 
-// `lanes` threads share kUnpackRows rows, V neighbouring values of each at a time (V divides 8).
-constexpr int kUnpackRows = 4;
+// `lanes` threads share `each` rows, V neighbouring values of each (V divides 8): where they are in a row is worked out once.
 template <class T, int V>
 __global__ void __launch_bounds__(kPackThreads) unpack_kernel(const unsigned char* codes, const __nv_bfloat16* scales,
                                                               long long n, int d, int group, int group_shift, T* out,
-                                                              int lanes) {
+                                                              int lanes, int each) {
   const int lane = threadIdx.x & (lanes - 1);
-  const long long first = ((long long)blockIdx.x * (kPackThreads / lanes) + threadIdx.x / lanes) * kUnpackRows;
-  const int blocks = (d + kBlock - 1) / kBlock, groups = (d + group - 1) / group;
+  const long long first = ((long long)blockIdx.x * (kPackThreads / lanes) + threadIdx.x / lanes) * each;
+  const int rows = (int)min((long long)each, n - first);
+  const int blocks = (d + kBlock - 1) / kBlock, groups = (d + group - 1) / group, row_bytes = 16 * blocks;
   for (int dim = lane * V; dim < d; dim += lanes * V) {
-    const int at = word_offset(dim >> 3, blocks), g = group_shift >= 0 ? dim >> group_shift : dim / group;
-    unsigned word[kUnpackRows];
-    float scale[kUnpackRows];
+    const unsigned char* word_at = codes + first * row_bytes + word_offset(dim >> 3, blocks);
+    const __nv_bfloat16* scale_at = scales + first * groups + (group_shift >= 0 ? dim >> group_shift : dim / group);
+    T* to = out + first * d + dim;
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r) {
+      const unsigned word = __ldg(reinterpret_cast<const unsigned*>(word_at));
+      const float scale = __bfloat162float(*scale_at);
+      T v[V];
 #pragma unroll
-    for (int r = 0; r < kUnpackRows; ++r) {
-      if (first + r < n) {
-        word[r] = __ldg(reinterpret_cast<const unsigned*>(codes + (first + r) * (16ll * blocks) + at));
-        scale[r] = __bfloat162float(scales[(first + r) * groups + g]);
+      for (int i = 0; i < V; ++i) {
+        const int k = (V == 8 ? 0 : dim & 7) + i;
+        // 2^23 + code, and 2^23 + 8 taken away: exact
+        const float code = __uint_as_float(((word >> (4 * ((k >> 1) + 4 * (k & 1)))) & 15) | 0x4b000000u) - 8388616.0f;
+        v[i] = from_f32<T>(code * scale);
       }
-    }
-#pragma unroll
-    for (int r = 0; r < kUnpackRows; ++r) {
-      if (first + r < n) {
-        T v[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int k = (dim & 7) + i;
-          const int code = (word[r] >> (4 * ((k >> 1) + 4 * (k & 1)))) & 15;
-          v[i] = from_f32<T>((float)(code - 8) * scale[r]);
-        }
-        store_many<T, V>(out + (first + r) * d + dim, v);
-      }
+      store_many<T, V>(to, v);
+      word_at += row_bytes;
+      scale_at += groups;
+      to += d;
     }
   }
 }
@@ -196,14 +200,18 @@ cudaError_t pack_n(const T* rows, long long row_stride, long long n, int d, long
   }
   // a group that is longer than the row is as good as one of all its words
   const int group_words = group / 8 > lanes ? lanes : (int)(group / 8);
-  const long long pieces = n * ((words + lanes - 1) / lanes);
-  const bool many = pieces > (long long)4 * kSMs * (kPackThreads / lanes);
-  const long long per = (kPackThreads / lanes) * (many ? 4 : 1), blocks = (pieces + per - 1) / per;
+  int shift = 0;
+  while ((1 << shift) < group_words) ++shift;
+  const int teams = kPackThreads / lanes, groups = (int)((d + group - 1) / group);
+  const bool longer = words > lanes, many = longer || n > (long long)4 * kSMs * teams;
+  const long long per = longer || !many ? teams : 4 * teams, blocks = (n + per - 1) / per;
   if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
-  if (many)
-    pack_kernel<T, N, 4><<<(unsigned)blocks, kPackThreads, 0, stream>>>(rows, row_stride, n, d, group_words, c, s, lanes);
+  if (longer)
+    pack_kernel<T, N, 4, true><<<(unsigned)blocks, kPackThreads, 0, stream>>>(rows, row_stride, n, d, shift, groups, c, s, lanes);
+  else if (many)
+    pack_kernel<T, N, 4, false><<<(unsigned)blocks, kPackThreads, 0, stream>>>(rows, row_stride, n, d, shift, groups, c, s, lanes);
   else
-    pack_kernel<T, N, 1><<<(unsigned)blocks, kPackThreads, 0, stream>>>(rows, row_stride, n, d, group_words, c, s, lanes);
+    pack_kernel<T, N, 1, false><<<(unsigned)blocks, kPackThreads, 0, stream>>>(rows, row_stride, n, d, shift, groups, c, s, lanes);
   return cudaGetLastError();
 }
 
@@ -221,12 +229,15 @@ template <class T, int V>
 cudaError_t unpack_v(const unsigned char* codes, const __nv_bfloat16* scales, long long n, int d, int group, T* out,
                      cudaStream_t stream) {
   const int lanes = next_pow2((d + V - 1) / V, kPackThreads);
-  const long long per = (long long)(kPackThreads / lanes) * kUnpackRows, blocks = (n + per - 1) / per;
+  // 16 rows, fewer while there are not four CTAs per SM
+  int each = 16;
+  while (each > 1 && n / ((long long)(kPackThreads / lanes) * each) < 4 * kSMs) each /= 2;
+  const long long per = (long long)(kPackThreads / lanes) * each, blocks = (n + per - 1) / per;
   if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
   int shift = 0;
   while ((1 << shift) < group) ++shift;
-  unpack_kernel<T, V><<<(unsigned)blocks, kPackThreads, 0, stream>>>(codes, scales, n, d, group,
-                                                                    (1 << shift) == group ? shift : -1, out, lanes);
+  unpack_kernel<T, V><<<(unsigned)blocks, kPackThreads, 0, stream>>>(
+    codes, scales, n, d, group, (1 << shift) == group ? shift : -1, out, lanes, each);
   return cudaGetLastError();
 }
 
