@@ -19,8 +19,8 @@ __device__ __forceinline__ long long id_at(const void* ids, int ids64, long long
 
 constexpr int kLookupThreads = 256;
 
-// `lanes` threads take kRows tokens at once, so that kRows loads of each are in flight.  Bound: HBM bytes.
-template <class T, int N, int kRows>
+// `lanes` threads take kRows tokens at once and kAt words of each, so that so many loads of each are in flight.  Bound: HBM bytes.
+template <class T, int N, int kRows, int kAt>
 __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(LookupParams p, int lanes) {
   const int group = threadIdx.x / lanes, lane = threadIdx.x % lanes, groups = kLookupThreads / lanes;
   const long long first = ((long long)blockIdx.x * groups + group) * kRows;
@@ -33,32 +33,44 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(LookupParams p, 
     id[r] = first + r < p.tokens ? id_at(p.ids, p.ids64, first + r) : -1;
     if (id[r] >= p.n) id[r] = -1;
   }
-  for (long long c = (long long)lane * N; c < p.d; c += (long long)lanes * N) {
-    Vec<T, N> v[kRows];
+  const int step = lanes * N, d = (int)p.d;
+  for (int begin = lane * N; begin < d; begin += kAt * step) {
+    Vec<T, N> v[kRows][kAt];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      if (id[r] >= 0) {
-        v[r] = load_vec<T, N>(rows + id[r] * p.row_stride + c);
-      } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[r].v[i] = from_f32<T>(0.0f);
+      for (int k = 0; k < kAt; ++k) {
+        const int c = begin + k * step;
+        if (id[r] >= 0 && c < d) {
+          v[r][k] = load_vec<T, N>(rows + id[r] * p.row_stride + c);
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; ++i) v[r][k].v[i] = from_f32<T>(0.0f);
+        }
       }
     }
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       if (first + r >= p.tokens) break;
-      if (id[r] >= 0 && p.scale != 1.0f) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[r].v[i] = from_f32<T>(to_f32(v[r].v[i]) * p.scale);
+      for (int k = 0; k < kAt; ++k) {
+        const int c = begin + k * step;
+        if (c >= d) break;
+        if (id[r] >= 0 && p.scale != 1.0f) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) v[r][k].v[i] = from_f32<T>(to_f32(v[r][k].v[i]) * p.scale);
+        }
+        store_vec<T, N>(out + (first + r) * p.d + c, v[r][k]);
       }
-      store_vec<T, N>(out + (first + r) * p.d + c, v[r]);
     }
   }
 }
 
 template <class T, int N>
 cudaError_t lookup_t(const LookupParams& p, cudaStream_t stream) {
-  const int lanes = next_pow2((p.d + N - 1) / N, kLookupThreads);
+  // narrow words: four of each row
+  constexpr int kAt = N * sizeof(T) >= 8 ? 1 : 4;
+  const int lanes = next_pow2((p.d + kAt * N - 1) / (kAt * N), kLookupThreads);
   const int groups = kLookupThreads / lanes;
   // four rows at a time, unless there are too few tokens to give every SM work
   const bool many = p.tokens > (long long)4 * groups * kSMs;
@@ -66,9 +78,9 @@ cudaError_t lookup_t(const LookupParams& p, cudaStream_t stream) {
   const long long blocks = (p.tokens + per - 1) / per;
   if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
   if (many)
-    lookup_kernel<T, N, 4><<<(unsigned)blocks, kLookupThreads, 0, stream>>>(p, lanes);
+    lookup_kernel<T, N, 4, kAt><<<(unsigned)blocks, kLookupThreads, 0, stream>>>(p, lanes);
   else
-    lookup_kernel<T, N, 1><<<(unsigned)blocks, kLookupThreads, 0, stream>>>(p, lanes);
+    lookup_kernel<T, N, 1, kAt><<<(unsigned)blocks, kLookupThreads, 0, stream>>>(p, lanes);
   return cudaGetLastError();
 }
 
@@ -84,31 +96,175 @@ cudaError_t lookup_words(const LookupParams& p, cudaStream_t stream) {
 
 // ---- gradient: the tokens sorted by id ------------------------------------------------------------------------------
 
-// A least-significant-digit radix sort of (id, token): stable, so the tokens of a row stay in their order and its sum does
-// not depend on the launch.  Ids outside the table become n, the largest key.
-constexpr int kOneThreads = 1024;       // one CTA sorts up to kOneMost tokens in shared memory
-constexpr int kOneItems = 16;
-constexpr int kOneMost = kOneThreads * kOneItems;
-constexpr int kTileThreads = 256;       // more: tiles of kTile tokens, one launch per step
-constexpr int kTileItems = 16;
-constexpr int kTile = kTileThreads * kTileItems;
-constexpr int kMaxDigit = 8;
+// Tokens sorted by id, those of a row in their order, so that its sum does not depend on the launch.  Ids outside the table
+// become n, the largest key.  The launches that sort are short chains of dependent steps; on the SMs beside them the zeros of the
+// rows without tokens are written (`zeros`: that part of `out`, by the CTAs behind `first`).
 
-struct SortPlan {
-  int bits, passes, digit;
+struct ZeroPart {
+  int first;                          // CTAs from here on, kZeroWords each
+  unsigned long long begin, words;    // of 16 bytes, from the first 16-byte boundary in `out`
+  unsigned char* out;
+  unsigned long long bytes;           // of all of `out`
 };
-SortPlan sort_plan(long long n) {
-  SortPlan s;
-  s.bits = 1;
-  while (s.bits < 32 && (n >> s.bits) > 0) ++s.bits;  // keys 0..n
-  s.passes = (s.bits + kMaxDigit - 1) / kMaxDigit;
-  s.digit = (s.bits + s.passes - 1) / s.passes;
-  return s;
+
+// Many CTAs with a few words each: 1 GB in 147 us; 592 CTAs that go through it in strides take 174.
+constexpr int kZeroThreads = 256;
+constexpr int kZeroWords = 4 * kZeroThreads;
+
+__device__ __forceinline__ void write_zeros(const ZeroPart& z) {
+  // whole words of 16 bytes, and with the first ones single bytes before and behind them all
+  const unsigned long long head = min(z.bytes, (unsigned long long)(-reinterpret_cast<uintptr_t>(z.out) & 15));
+  if ((int)blockIdx.x == z.first && z.begin == 0) {
+    const unsigned long long all = (z.bytes - head) / 16, tail = (z.bytes - head) % 16;
+    if (threadIdx.x < head) z.out[threadIdx.x] = 0;
+    if (threadIdx.x < tail) z.out[head + all * 16 + threadIdx.x] = 0;
+  }
+  uint4* to = reinterpret_cast<uint4*>(z.out + head) + z.begin;
+  const unsigned long long at = (unsigned long long)(blockIdx.x - z.first) * kZeroWords + threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < kZeroWords / kZeroThreads; ++i)
+    if (at + i * kZeroThreads < z.words) to[at + i * kZeroThreads] = make_uint4(0, 0, 0, 0);
 }
 
 __device__ __forceinline__ unsigned key_at(const LookupGradParams& p, long long t) {
   const long long id = id_at(p.ids, p.ids64, t);
   return id < 0 || id >= p.n ? (unsigned)p.n : (unsigned)id;
+}
+
+// Up to kRankMost tokens: every token's place is the number of smaller keys and of equal ones before it, counted against all
+// tokens: no pass depends on another one.  16 384 tokens take 17 us spread over all SMs, 511 about 2.
+constexpr int kRankMost = 16384;
+constexpr int kRankThreads = kZeroThreads;
+constexpr int kRankTokens = 64;                                // of a CTA
+constexpr int kRankShares = kRankThreads / kRankTokens;        // threads that share a token
+constexpr int kRankTile = 2048;                                // keys in shared memory at a time
+
+__global__ void __launch_bounds__(kRankThreads) sort_rank_kernel(LookupGradParams p, ZeroPart zeros, unsigned* keys_out,
+                                                                 unsigned* tokens_out, unsigned* joins) {
+  next_launch_may_start();
+  if ((int)blockIdx.x >= zeros.first) {
+    write_zeros(zeros);
+    return;
+  }
+  __shared__ __align__(16) unsigned keys[kRankTile];
+  __shared__ unsigned counts[kRankShares][kRankTokens];
+  const int count = (int)p.tokens, mine = threadIdx.x % kRankTokens, share = threadIdx.x / kRankTokens;
+  const int first = blockIdx.x * kRankTokens, token = first + mine;
+  const unsigned key = token < count ? key_at(p, token) : 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *joins = 0;
+  unsigned below = 0;
+  unsigned next[kRankTile / kRankThreads];  // the next tile, on its way while this one is compared
+  auto load = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < kRankTile / kRankThreads; ++i) {
+      const int at = tile + i * kRankThreads + threadIdx.x;
+      next[i] = at < count ? key_at(p, at) : 0xffffffffu;  // (keys behind the last one are smaller than none)
+    }
+  };
+  load(0);
+  for (int tile = 0; tile < count; tile += kRankTile) {
+    const int held = min(kRankTile, count - tile);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kRankTile / kRankThreads; ++i) keys[i * kRankThreads + threadIdx.x] = next[i];
+    __syncthreads();
+    if (tile + kRankTile < count) load(tile + kRankTile);
+    // four keys at a time, the shares in turn: those of tokens before this CTA's (equal ones come first), its own, and the rest
+    const int own = min(max(first - tile, 0), held), after = min(max(first + kRankTokens - tile, 0), held);
+    constexpr int kStep = 4 * kRankShares;
+    int i = 4 * share;
+#pragma unroll 4
+    for (; i < own; i += kStep) {
+      const uint4 k = *reinterpret_cast<const uint4*>(keys + i);
+      below += (k.x <= key) + (k.y <= key) + (k.z <= key) + (k.w <= key);
+    }
+    for (; i < after; i += kStep) {
+      const uint4 k = *reinterpret_cast<const uint4*>(keys + i);
+      const int at = tile + i;
+      below += (k.x < key || (k.x == key && at < token)) + (k.y < key || (k.y == key && at + 1 < token)) +
+               (k.z < key || (k.z == key && at + 2 < token)) + (k.w < key || (k.w == key && at + 3 < token));
+    }
+#pragma unroll 4
+    for (; i < held; i += kStep) {
+      const uint4 k = *reinterpret_cast<const uint4*>(keys + i);
+      below += (k.x < key) + (k.y < key) + (k.z < key) + (k.w < key);
+    }
+  }
+  counts[share][mine] = below;
+  __syncthreads();
+  if (share == 0 && token < count) {
+#pragma unroll
+    for (int s = 1; s < kRankShares; ++s) below += counts[s][mine];
+    keys_out[below] = key;
+    tokens_out[below] = token;
+  }
+}
+
+// More tokens: a least-significant-digit radix sort.  At most kParts CTAs have a contiguous part of the tokens each; a pass
+// counts the digits of each part, and then every part finds out where its tokens of each digit begin and puts them there, tile by
+// tile.
+constexpr int kParts = 2 * kSMs;
+constexpr int kTileThreads = kZeroThreads;
+constexpr int kTileWarps = kTileThreads / 32;
+constexpr int kMaxDigit = 8;
+
+struct SortPlan {
+  int passes, digit;      // bits
+  int items;              // tokens of a tile per thread: 4 or 16
+  int parts;
+  long long part;         // tokens, whole tiles
+};
+SortPlan sort_plan(long long tokens, long long n) {
+  SortPlan s;
+  int bits = 1;
+  while (bits < 32 && (n >> bits) > 0) ++bits;  // keys 0..n
+  s.passes = (bits + kMaxDigit - 1) / kMaxDigit;
+  s.digit = (bits + s.passes - 1) / s.passes;
+  if (s.digit < 2) s.digit = 2;  // (four counts are read at a time)
+  // small tiles while they are enough for a part each: more CTAs that take less time
+  s.items = tokens <= (long long)kParts * kTileThreads * 4 ? 4 : 16;
+  const long long tile = kTileThreads * s.items, tiles = (tokens + tile - 1) / tile;
+  s.part = (tiles + kParts - 1) / kParts * tile;
+  s.parts = (int)((tokens + s.part - 1) / s.part);
+  return s;
+}
+
+// counts[part * digits + digit]
+template <int kTileItems>
+__global__ void __launch_bounds__(kTileThreads) sort_count_kernel(LookupGradParams p, ZeroPart zeros, SortPlan plan,
+                                                                  const unsigned* keys, int shift, unsigned* counts,
+                                                                  unsigned* joins) {
+  next_launch_may_start();
+  if ((int)blockIdx.x >= zeros.first) {
+    write_zeros(zeros);
+    return;
+  }
+  constexpr int kTile = kTileThreads * kTileItems;
+  const int digits = 1 << plan.digit;
+  __shared__ unsigned bins[1 << kMaxDigit];
+  for (int i = threadIdx.x; i < digits; i += kTileThreads) bins[i] = 0;
+  if (keys) wait_for_launch_before();
+  if (joins && blockIdx.x == 0 && threadIdx.x == 0) *joins = 0;
+  __syncthreads();
+  const long long begin = blockIdx.x * plan.part, end = min(begin + plan.part, p.tokens);
+  for (long long tile = begin; tile < end; tile += kTile) {
+    unsigned key[kTileItems];
+#pragma unroll
+    for (int i = 0; i < kTileItems; ++i) {
+      const long long at = tile + i * kTileThreads + threadIdx.x;
+      key[i] = at >= end ? 0 : keys ? keys[at] : key_at(p, at);
+    }
+#pragma unroll
+    for (int i = 0; i < kTileItems; ++i) {
+      const bool live = tile + i * kTileThreads + threadIdx.x < end;
+      const unsigned digit = live ? (key[i] >> shift) & (digits - 1) : 0xffffffffu;
+      // one addition for all lanes with the same digit: a frequent token would serialise them
+      const unsigned peers = __match_any_sync(FULL, digit);
+      if (live && (peers & ((1u << lane_id()) - 1)) == 0) atomicAdd(bins + digit, __popc(peers));
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < digits; i += kTileThreads) counts[blockIdx.x * digits + i] = bins[i];
 }
 
 // Rank of each of a warp's keys (lane l holds items l, 32 + l, ..) among the earlier keys of the warp with the same
@@ -131,203 +287,92 @@ __device__ __forceinline__ void warp_ranks(const unsigned (&key)[Items], int shi
   }
 }
 
-// Exclusive sum of one value per thread over the CTA.
-template <int Threads>
-__device__ __forceinline__ unsigned block_exclusive(unsigned x, unsigned* scratch /* Threads / 32 */) {
-  const int lane = lane_id(), warp = threadIdx.x >> 5;
-  unsigned sum = x;
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const unsigned y = __shfl_up_sync(FULL, sum, off);
-    if (lane >= off) sum += y;
-  }
-  if (lane == 31) scratch[warp] = sum;
-  __syncthreads();
-  unsigned before = 0;
-  for (int w = 0; w < warp; ++w) before += scratch[w];
-  __syncthreads();
-  return before + sum - x;
-}
-
-// Zeros in all of `out`, by the CTAs [first, gridDim.x) of a launch.
-__device__ __forceinline__ void zero_out(const LookupGradParams& p, int first) {
-  unsigned char* out = static_cast<unsigned char*>(p.out);
-  const unsigned long long bytes = (unsigned long long)p.n * p.d * (p.out_type == kF32 ? 4 : 2);
-  // whole words of 16 bytes, and single bytes before and behind them
-  const unsigned long long head = min(bytes, (unsigned long long)(-reinterpret_cast<uintptr_t>(out) & 15));
-  const unsigned long long words = (bytes - head) / 16, tail = (bytes - head) % 16;
-  if ((int)blockIdx.x == first) {
-    if (threadIdx.x < head) out[threadIdx.x] = 0;
-    if (threadIdx.x < tail) out[head + words * 16 + threadIdx.x] = 0;
-  }
-  const unsigned long long step = (unsigned long long)(gridDim.x - first) * blockDim.x;
-  uint4* to = reinterpret_cast<uint4*>(out + head);
-  for (unsigned long long at = (unsigned long long)(blockIdx.x - first) * blockDim.x + threadIdx.x; at < words; at += step)
-    __stcs(to + at, make_uint4(0, 0, 0, 0));
-}
-
-// CTA 0 sorts all tokens in shared memory; the others meanwhile write the zeros of the rows that nobody looked up.
-__global__ void __launch_bounds__(kOneThreads) sort_one_kernel(LookupGradParams p, SortPlan plan, unsigned* keys_out,
-                                                               unsigned* tokens_out, unsigned* joins) {
-  if (blockIdx.x > 0) {
-    zero_out(p, 1);
-    return;
-  }
-  extern __shared__ __align__(16) unsigned char smem[];
-  constexpr int kWarps = kOneThreads / 32;
-  const int digits = 1 << plan.digit, count = (int)p.tokens;
-  const int items = (count + kOneThreads - 1) / kOneThreads;
-  unsigned* keys = reinterpret_cast<unsigned*>(smem);
-  unsigned short* places = reinterpret_cast<unsigned short*>(keys + items * kOneThreads);
-  unsigned short* counts = places + items * kOneThreads;
-  __shared__ unsigned scratch[kWarps];
-  const int warp = threadIdx.x >> 5, lane = lane_id();
-  const int begin = min(warp * items * 32, count), valid = min(items * 32, count - begin);
-  if (threadIdx.x == 0) *joins = 0;
-  for (int t = threadIdx.x; t < count; t += kOneThreads) {
-    keys[t] = key_at(p, t);
-    places[t] = (unsigned short)t;
-  }
-  for (int pass = 0; pass < plan.passes; ++pass) {
-    const int shift = pass * plan.digit;
-    for (int i = threadIdx.x; i < kWarps * digits; i += kOneThreads) counts[i] = 0;
-    __syncthreads();
-    unsigned key[kOneItems], rank[kOneItems];
-    unsigned short place[kOneItems];
-#pragma unroll
-    for (int i = 0; i < kOneItems; ++i) {
-      if (i * 32 + lane < valid) {
-        key[i] = keys[begin + i * 32 + lane];
-        place[i] = places[begin + i * 32 + lane];
-      }
-    }
-    warp_ranks<kOneItems>(key, shift, digits - 1, valid, counts + warp * digits, rank);
-    __syncthreads();
-    unsigned total = 0;
-    if (threadIdx.x < digits) {
-      for (int w = 0; w < kWarps; ++w) {
-        const unsigned c = counts[w * digits + threadIdx.x];
-        counts[w * digits + threadIdx.x] = (unsigned short)total;
-        total += c;
-      }
-    }
-    const unsigned base = block_exclusive<kOneThreads>(total, scratch);
-    if (threadIdx.x < digits)
-      for (int w = 0; w < kWarps; ++w) counts[w * digits + threadIdx.x] += (unsigned short)base;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kOneItems; ++i) {
-      if (i * 32 + lane < valid) {
-        const unsigned at = counts[warp * digits + ((key[i] >> shift) & (digits - 1))] + rank[i];
-        if (pass + 1 < plan.passes) {
-          keys[at] = key[i];
-          places[at] = place[i];
-        } else {
-          keys_out[at] = key[i];
-          tokens_out[at] = place[i];
-        }
-      }
-    }
-    __syncthreads();
-  }
-}
-
-// Tokens of each digit in each tile, digit by digit: counts[digit * tiles + tile].  In the first pass the CTAs behind the
-// tiles write the zeros.
-__global__ void __launch_bounds__(kTileThreads) sort_count_kernel(LookupGradParams p, const unsigned* keys, int shift,
-                                                                  int digits, int tiles, unsigned* counts,
-                                                                  unsigned* joins) {
-  if ((int)blockIdx.x >= tiles) {
-    zero_out(p, tiles);
-    return;
-  }
-  __shared__ unsigned bins[1 << kMaxDigit];
-  for (int i = threadIdx.x; i < digits; i += kTileThreads) bins[i] = 0;
-  if (joins && blockIdx.x == 0 && threadIdx.x == 0) *joins = 0;
-  __syncthreads();
-  const long long begin = (long long)blockIdx.x * kTile;
-  const int valid = (int)min((long long)kTile, p.tokens - begin);
-  for (int from = threadIdx.x & ~31; from < valid; from += kTileThreads) {
-    const int i = from + lane_id();
-    const bool live = i < valid;
-    const unsigned key = !live ? 0 : keys ? keys[begin + i] : key_at(p, begin + i);
-    const unsigned digit = live ? (key >> shift) & (digits - 1) : 0xffffffffu;
-    // one addition for all lanes with the same digit: a frequent token would serialise them
-    const unsigned peers = __match_any_sync(FULL, digit);
-    if (live && (peers & ((1u << lane_id()) - 1)) == 0) atomicAdd(bins + digit, __popc(peers));
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < digits; i += kTileThreads) counts[(size_t)i * tiles + blockIdx.x] = bins[i];
-}
-
-// Exclusive sum of all counts, by one CTA.
-__global__ void __launch_bounds__(kOneThreads) sort_scan_kernel(unsigned* counts, long long total) {
-  __shared__ unsigned scratch[kOneThreads / 32];
-  __shared__ unsigned carry;
-  if (threadIdx.x == 0) carry = 0;
-  __syncthreads();
-  constexpr int kEach = 16;
-  for (long long begin = 0; begin < total; begin += kOneThreads * kEach) {
-    const long long mine = begin + (long long)threadIdx.x * kEach;
-    unsigned c[kEach], sum = 0;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      c[i] = mine + i < total ? counts[mine + i] : 0;
-      sum += c[i];
-    }
-    unsigned before = block_exclusive<kOneThreads>(sum, scratch) + carry;
-    const unsigned after = before + sum;
-    __syncthreads();
-    if (threadIdx.x == kOneThreads - 1) carry = after;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      if (mine + i < total) counts[mine + i] = before;
-      before += c[i];
-    }
-    __syncthreads();
-  }
-}
-
-// Every tile's tokens to their places.
-__global__ void __launch_bounds__(kTileThreads) sort_place_kernel(LookupGradParams p, const unsigned* keys,
-                                                                  const unsigned* tokens, int shift, int digits,
-                                                                  int tiles, const unsigned* counts, unsigned* keys_out,
+template <int kTileItems>
+__global__ void __launch_bounds__(kTileThreads) sort_place_kernel(LookupGradParams p, ZeroPart zeros, SortPlan plan,
+                                                                  const unsigned* keys, const unsigned* tokens,
+                                                                  int shift, const unsigned* counts, unsigned* keys_out,
                                                                   unsigned* tokens_out) {
-  constexpr int kWarps = kTileThreads / 32;
-  __shared__ unsigned short warp_counts[kWarps << kMaxDigit];
-  __shared__ unsigned bases[kWarps << kMaxDigit];
-  const int warp = threadIdx.x >> 5, lane = lane_id();
-  for (int i = threadIdx.x; i < kWarps * digits; i += kTileThreads) warp_counts[i] = 0;
+  next_launch_may_start();
+  if ((int)blockIdx.x >= zeros.first) {
+    write_zeros(zeros);
+    return;
+  }
+  constexpr int kTile = kTileThreads * kTileItems;
+  constexpr int kDigits = 1 << kMaxDigit;
+  static_assert(kDigits == kTileThreads, "a digit per thread");
+  __shared__ unsigned short warp_counts[kTileWarps * kDigits];
+  __shared__ unsigned bases[kTileWarps * kDigits], starts[kDigits], before[kDigits], scratch[kTileWarps];
+  const int digits = 1 << plan.digit, warp = threadIdx.x >> 5, lane = lane_id(), parts = plan.parts;
+  // tokens of each digit in all parts, and in the ones before this: every warp takes some of the parts, a lane four digits
+  for (int i = threadIdx.x; i < digits; i += kTileThreads) starts[i] = before[i] = 0;
+  wait_for_launch_before();
   __syncthreads();
-  const long long tile_begin = (long long)blockIdx.x * kTile;
-  const long long begin = min(tile_begin + warp * 32 * kTileItems, p.tokens);
-  const int valid = (int)min((long long)(32 * kTileItems), p.tokens - begin);
-  unsigned key[kTileItems], token[kTileItems], rank[kTileItems];
+  for (int d = 4 * lane; d < digits; d += 128) {
+    unsigned all[4] = {0, 0, 0, 0}, earlier[4] = {0, 0, 0, 0};
+#pragma unroll 8
+    for (int i = warp; i < parts; i += kTileWarps) {
+      const uint4 c = *reinterpret_cast<const uint4*>(counts + i * digits + d);
+      const bool earlier_part = i < (int)blockIdx.x;
+      all[0] += c.x, all[1] += c.y, all[2] += c.z, all[3] += c.w;
+      earlier[0] += earlier_part ? c.x : 0, earlier[1] += earlier_part ? c.y : 0;
+      earlier[2] += earlier_part ? c.z : 0, earlier[3] += earlier_part ? c.w : 0;
+    }
 #pragma unroll
-  for (int i = 0; i < kTileItems; ++i) {
-    if (i * 32 + lane < valid) {
-      const long long at = begin + i * 32 + lane;
-      key[i] = keys ? keys[at] : key_at(p, at);
-      token[i] = tokens ? tokens[at] : (unsigned)at;
+    for (int k = 0; k < 4; ++k) {
+      atomicAdd(starts + d + k, all[k]);
+      atomicAdd(before + d + k, earlier[k]);
     }
   }
-  warp_ranks<kTileItems>(key, shift, digits - 1, valid, warp_counts + warp * digits, rank);
   __syncthreads();
-  for (int i = threadIdx.x; i < digits; i += kTileThreads) {
-    unsigned base = counts[(size_t)i * tiles + blockIdx.x];
-    for (int w = 0; w < kWarps; ++w) {
-      bases[w * digits + i] = base;
-      base += warp_counts[w * digits + i];
-    }
-  }
-  __syncthreads();
+  {
+    const unsigned x = (int)threadIdx.x < digits ? starts[threadIdx.x] : 0;
+    unsigned sum = x;
 #pragma unroll
-  for (int i = 0; i < kTileItems; ++i) {
-    if (i * 32 + lane < valid) {
-      const unsigned at = bases[warp * digits + ((key[i] >> shift) & (digits - 1))] + rank[i];
-      keys_out[at] = key[i];
-      tokens_out[at] = token[i];
+    for (int off = 1; off < 32; off <<= 1) {
+      const unsigned y = __shfl_up_sync(FULL, sum, off);
+      if (lane >= off) sum += y;
     }
+    if (lane == 31) scratch[warp] = sum;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) sum += scratch[w];
+    if ((int)threadIdx.x < digits) starts[threadIdx.x] = sum - x + before[threadIdx.x];
+  }
+  const long long part_begin = blockIdx.x * plan.part, part_end = min(part_begin + plan.part, p.tokens);
+  for (long long tile = part_begin; tile < part_end; tile += kTile) {
+    for (int i = threadIdx.x; i < kTileWarps * digits / 2; i += kTileThreads) reinterpret_cast<unsigned*>(warp_counts)[i] = 0;
+    const long long begin = min(tile + warp * 32 * kTileItems, part_end);
+    const int valid = (int)min((long long)(32 * kTileItems), part_end - begin);
+    unsigned key[kTileItems], token[kTileItems], rank[kTileItems];
+#pragma unroll
+    for (int i = 0; i < kTileItems; ++i) {
+      if (i * 32 + lane < valid) {
+        const long long at = begin + i * 32 + lane;
+        key[i] = keys ? keys[at] : key_at(p, at);
+        token[i] = tokens ? tokens[at] : (unsigned)at;
+      }
+    }
+    __syncthreads();
+    warp_ranks<kTileItems>(key, shift, digits - 1, valid, warp_counts + warp * digits, rank);
+    __syncthreads();
+    if ((int)threadIdx.x < digits) {
+      unsigned base = starts[threadIdx.x];
+#pragma unroll
+      for (int w = 0; w < kTileWarps; ++w) {
+        bases[w * digits + threadIdx.x] = base;
+        base += warp_counts[w * digits + threadIdx.x];
+      }
+      starts[threadIdx.x] = base;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kTileItems; ++i) {
+      if (i * 32 + lane < valid) {
+        const unsigned at = bases[warp * digits + ((key[i] >> shift) & (digits - 1))] + rank[i];
+        keys_out[at] = key[i];
+        tokens_out[at] = token[i];
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -339,125 +384,238 @@ __global__ void __launch_bounds__(kTileThreads) sort_place_kernel(LookupGradPara
 // join_kernel adds those up.
 constexpr int kSumThreads = 256;
 constexpr int kInFlight = 8;
+constexpr int kMostChunk = 64;
+constexpr int kSumLanes = 8;   // threads of a chunk at least
 
 struct SumPlan {
-  int chunk;         // tokens
+  int chunk;         // tokens, a multiple of kInFlight
   long long chunks;
 };
 SumPlan sum_plan(long long tokens, long long d) {
   SumPlan s;
-  // about 2048 values per SM and chunk of 64 tokens keep all SMs busy; short batches take shorter chunks
-  s.chunk = 64;
-  while (s.chunk > 8 && tokens / s.chunk * d < (long long)kSMs * 4096) s.chunk /= 2;
+  // chunks of 64 tokens where that leaves every SM some 14 000 values to add side by side, shorter ones for fewer tokens (but
+  // the shorter they are the more partial sums there are)
+  s.chunk = kMostChunk;
+  const int least = tokens > 8192 ? 2 * kInFlight : kInFlight;
+  while (s.chunk > least && tokens / s.chunk * d < (long long)kSMs * 14'000) s.chunk /= 2;
   s.chunks = (tokens + s.chunk - 1) / s.chunk;
   return s;
 }
 
-template <class G, class O, int N>
+template <class O, int N>
 __device__ __forceinline__ void write_row(const LookupGradParams& p, unsigned row, long long c, const float (&sum)[N]) {
   O* at = static_cast<O*>(p.out) + (long long)row * p.d + c;
   O v[N];
-  if (p.accumulate) load_many<O, N>(at, v);
+  if (p.accumulate) {
+    load_many<O, N>(at, v);
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = from_f32<O>(p.accumulate ? to_f32(v[i]) + sum[i] * p.scale : sum[i] * p.scale);
+    for (int i = 0; i < N; ++i) v[i] = from_f32<O>(to_f32(v[i]) + sum[i] * p.scale);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = from_f32<O>(sum[i] * p.scale);
+  }
   store_many<O, N>(at, v);
 }
 
-template <class G, class O, int N>
-__global__ void __launch_bounds__(kSumThreads) sum_kernel(LookupGradParams p, SumPlan plan, const unsigned* keys,
+// `lanes` threads have a chunk (of up to lanes * N dimensions); kInFlight rows of the gradient are on their way to each.  A
+// thread has N neighbouring values or, of rows that are no whole words (kApart), N values `lanes` apart.
+template <class G, class O, int N, bool kApart>
+__global__ void __launch_bounds__(kSumThreads, 3) sum_kernel(LookupGradParams p, SumPlan plan, const unsigned* keys,
                                                           const unsigned* tokens, float* heads, float* tails,
                                                           unsigned* joins, unsigned* join_list, int lanes) {
   const int group = threadIdx.x / lanes, lane = threadIdx.x % lanes, groups = kSumThreads / lanes;
   const long long chunk = (long long)blockIdx.x * groups + group;
-  if (chunk >= plan.chunks) return;
-  const long long begin = chunk * plan.chunk, end = min(begin + plan.chunk, p.tokens);
-  const long long c = ((long long)blockIdx.y * lanes + lane) * N;
-  if (c >= p.d) return;
+  next_launch_may_start();
+  wait_for_launch_before();
+  __shared__ __align__(16) unsigned chunk_keys[kSumThreads / kSumLanes][kMostChunk], chunk_tokens[kSumThreads / kSumLanes][kMostChunk];
   const unsigned none = (unsigned)p.n;
-  const G* grad = static_cast<const G*>(p.grad);
+  const long long begin = chunk * plan.chunk, end = min(begin + plan.chunk, p.tokens);
+  for (int i = lane; i < plan.chunk; i += lanes) {  // (the end of the last chunk as empty slots)
+    chunk_keys[group][i] = begin + i < end ? keys[begin + i] : none;
+    chunk_tokens[group][i] = begin + i < end ? tokens[begin + i] : 0;
+  }
+  __syncthreads();
+  if (chunk >= plan.chunks) return;
+  const long long c = (long long)blockIdx.y * lanes * N + (kApart ? lane : lane * N);
+  if (c >= p.d) return;
+  const int held = kApart ? (int)min((long long)N, (p.d - c + lanes - 1) / lanes) : N;  // values
+  const G* grad = static_cast<const G*>(p.grad) + c;
   const unsigned before = begin > 0 ? keys[begin - 1] : none, after = end < p.tokens ? keys[end] : none;
-  unsigned row = keys[begin];
-  bool first = true;  // the row that the chunk begins with
+  unsigned row = chunk_keys[group][0];
+  bool head = row == before;  // the row that the chunk begins with is another chunk's as well
   float sum[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) sum[i] = 0.0f;
-  auto finish = [&](bool last) {
-    if (row == none) return;
-    float* partial = nullptr;
-    if (first && row == before)
-      partial = heads + chunk * p.d + c;
-    else if (last && row == after)
-      partial = tails + chunk * p.d + c;
-    if (partial) {
-      store_many<float, N>(partial, sum);
-      if (last && row == after && !(first && row == before) && c == 0) join_list[atomicAdd(joins, 1u)] = (unsigned)chunk;
+  auto partial = [&](float* to) {
+    to += chunk * p.d + c;
+    if constexpr (kApart) {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (j < held) to[j * lanes] = sum[j];
     } else {
-      write_row<G, O, N>(p, row, c, sum);
+      store_many<float, N>(to, sum);
     }
   };
-  for (long long t = begin; t < end; t += kInFlight) {
+  auto write = [&] {
+    if constexpr (kApart) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float one[1] = {sum[j]};
+        if (j < held) write_row<O, 1>(p, row, c + j * lanes, one);
+      }
+    } else {
+      write_row<O, N>(p, row, c, sum);
+    }
+  };
+  for (int t = 0; t < plan.chunk; t += kInFlight) {
     unsigned key[kInFlight];
-    Vec<G, N> v[kInFlight];
+#pragma unroll
+    for (int i = 0; i < kInFlight; i += 4) {
+      const uint4 k = *reinterpret_cast<const uint4*>(chunk_keys[group] + t + i);
+      key[i] = k.x, key[i + 1] = k.y, key[i + 2] = k.z, key[i + 3] = k.w;
+    }
+    // (whole words: a value of 16 bits that waits by itself takes a register)
+    using Word = typename WordOf<kApart ? sizeof(G) : sizeof(G) * N>::type;
+    constexpr int kWords = kApart ? N : 1;
+    Word word[kInFlight][kWords];
 #pragma unroll
     for (int i = 0; i < kInFlight; ++i) {
-      key[i] = t + i < end ? keys[t + i] : none;
-      if (key[i] != none) v[i] = load_stream<G, N>(grad + (long long)tokens[t + i] * p.grad_stride + c);
+      if (key[i] == none) continue;
+      const G* from = grad + (long long)chunk_tokens[group][t + i] * p.grad_stride;
+#pragma unroll
+      for (int j = 0; j < kWords; ++j)
+        if (!kApart || j < held) word[i][j] = __ldcs(reinterpret_cast<const Word*>(from + (kApart ? j * lanes : 0)));
     }
 #pragma unroll
     for (int i = 0; i < kInFlight; ++i) {
-      if (t + i >= end) break;
       if (key[i] != row) {
-        finish(false);
+        if (key[i] == none) break;  // nothing but empty slots from here on, or the end
+        if (head)
+          partial(heads);
+        else
+          write();
+        head = false;
         row = key[i];
-        first = false;
 #pragma unroll
         for (int j = 0; j < N; ++j) sum[j] = 0.0f;
       }
-      if (row == none) return;  // nothing but empty slots from here on
+      if (row == none) return;  // a chunk of empty slots
+      if constexpr (kApart) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) sum[j] += to_f32(v[i].v[j]);
+        for (int j = 0; j < N; ++j) sum[j] += to_f32(*reinterpret_cast<const G*>(&word[i][j]));
+      } else {
+        const Vec<G, N> v = *reinterpret_cast<const Vec<G, N>*>(&word[i][0]);
+#pragma unroll
+        for (int j = 0; j < N; ++j) sum[j] += to_f32(v.v[j]);
+      }
     }
   }
-  finish(true);
+  if (head) {
+    partial(heads);
+  } else if (row == after) {
+    partial(tails);
+    if (c == 0) join_list[atomicAdd(joins, 1u)] = (unsigned)chunk;
+  } else {
+    write();
+  }
 }
 
-// Rows that cross borders of chunks: 8 warps add up an eighth of the partial sums each.
+// Rows that cross borders of chunks.  A warp takes one of them and kJoinDims dimensions; of a row with many partial sums the
+// CTA's warps add up a share each.
 constexpr int kJoinWarps = 8;
-template <class G, class O>
+constexpr int kJoinDims = 128;
+constexpr long long kJoinAlone = 48;  // partial sums that a warp adds up by itself
+
+template <class O>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(LookupGradParams p, SumPlan plan, const unsigned* keys,
                                                                const float* heads, const float* tails,
                                                                const unsigned* joins, const unsigned* join_list) {
-  __shared__ float sums[kJoinWarps][32];
+  __shared__ float sums[kJoinWarps][kJoinDims];
+  __shared__ long long first_of[kJoinWarps], parts_of[kJoinWarps];
+  __shared__ unsigned row_of[kJoinWarps];
+  constexpr int kEach = kJoinDims / 32;
   const int warp = threadIdx.x >> 5, lane = lane_id();
-  const unsigned count = *joins;
-  const long long c = (long long)blockIdx.y * 32 + lane;
-  for (unsigned i = blockIdx.x; i < count; i += gridDim.x) {
-    const long long chunk = join_list[i];
-    const unsigned row = keys[(chunk + 1) * plan.chunk];
-    // the last chunk that the row reaches: its first key is the row's
-    long long low = chunk + 1, high = plan.chunks - 1;
-    while (low < high) {
-      const long long mid = (low + high + 1) / 2;
-      if (keys[mid * plan.chunk] == row)
-        low = mid;
-      else
-        high = mid - 1;
+  wait_for_launch_before();
+  const long long count = *joins, items = count * ((p.d + kJoinDims - 1) / kJoinDims);
+  for (long long base = (long long)blockIdx.x * kJoinWarps; base < items; base += (long long)gridDim.x * kJoinWarps) {
+    const long long item = base + warp;
+    long long chunk = 0, parts = 0;
+    unsigned row = 0;
+    if (item < items) {
+      chunk = join_list[item % count];  // (a CTA's warps take different rows: the longest ones are not all its own)
+      row = keys[(chunk + 1) * plan.chunk];
+      // the last chunk that begins with the row: 32 candidates at a time, the next ones first
+      long long low = chunk + 1, step = 1;
+      for (;;) {
+        const long long at = low + (lane + 1) * step;
+        const unsigned same = __ballot_sync(FULL, at < plan.chunks && keys[min(at, plan.chunks - 1) * plan.chunk] == row);
+        const int reached = __popc(same);  // they are the first ones
+        low += reached * step;
+        if (reached == 32) {
+          step *= 32;
+        } else if (step == 1) {
+          break;
+        } else {
+          step /= 32;
+        }
+      }
+      parts = low - chunk + 1;  // one tail, the rest heads
     }
-    const long long parts = low - chunk + 1;  // one tail, the rest heads
-    const long long each = (parts + kJoinWarps - 1) / kJoinWarps;
-    float sum = 0.0f;
-    if (c < p.d) {
-      const long long to = min(parts, (warp + 1) * each);
-#pragma unroll 8
-      for (long long k = warp * each; k < to; ++k) sum += (k == 0 ? tails : heads)[(chunk + k) * p.d + c];
-    }
-    sums[warp][lane] = sum;
-    __syncthreads();
-    if (warp == 0 && c < p.d) {
-      float total[1] = {sums[0][lane]};
+    auto add = [&](long long from_chunk, long long from, long long to, long long column, float (&sum)[kEach]) {
 #pragma unroll
-      for (int w = 1; w < kJoinWarps; ++w) total[0] += sums[w][lane];
-      write_row<G, O, 1>(p, row, c, total);
+      for (int i = 0; i < kEach; ++i) sum[i] = 0.0f;
+      if (from == 0 && to > 0) {
+        const float* tail = tails + from_chunk * p.d + column * kJoinDims + lane;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+          if (column * kJoinDims + lane + 32 * i < p.d) sum[i] = tail[32 * i];
+        ++from;
+      }
+      const float* head = heads + (from_chunk + from) * p.d + column * kJoinDims + lane;
+#pragma unroll 8
+      for (long long k = from; k < to; ++k, head += p.d) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+          if (column * kJoinDims + lane + 32 * i < p.d) sum[i] += head[32 * i];
+      }
+    };
+    auto write = [&](unsigned to_row, long long column, const float (&sum)[kEach]) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const long long c = column * kJoinDims + lane + 32 * i;
+        const float one[1] = {sum[i]};
+        if (c < p.d) write_row<O, 1>(p, to_row, c, one);
+      }
+    };
+    if (item < items && parts <= kJoinAlone) {
+      float sum[kEach];
+      add(chunk, 0, parts, item / count, sum);
+      write(row, item / count, sum);
+    }
+    if (lane == 0) {
+      first_of[warp] = chunk;
+      parts_of[warp] = parts;
+      row_of[warp] = row;
+    }
+    __syncthreads();
+    for (int w = 0; w < kJoinWarps; ++w) {
+      if (parts_of[w] <= kJoinAlone) continue;
+      const long long share = (parts_of[w] + kJoinWarps - 1) / kJoinWarps, column = (base + w) / count;
+      float sum[kEach];
+      add(first_of[w], warp * share, min(parts_of[w], (warp + 1) * share), column, sum);
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) sums[warp][lane + 32 * i] = sum[i];
+      __syncthreads();
+      if (warp == 0) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          sum[i] = sums[0][lane + 32 * i];
+#pragma unroll
+          for (int v = 1; v < kJoinWarps; ++v) sum[i] += sums[v][lane + 32 * i];
+        }
+        write(row_of[w], column, sum);
+      }
+      __syncthreads();
     }
     __syncthreads();
   }
@@ -483,13 +641,13 @@ GradSpace grad_space(long long tokens, long long n, long long d, void* base) {
     return here;
   };
   const SumPlan sums = sum_plan(tokens, d);
-  const SortPlan plan = sort_plan(n);
-  const bool one = tokens <= kOneMost;
-  for (int i = 0; i < 2; ++i) {
-    s.keys[i] = reinterpret_cast<unsigned*>(take(one && i ? 0 : tokens));
-    s.tokens[i] = reinterpret_cast<unsigned*>(take(one && i ? 0 : tokens));
+  const SortPlan plan = sort_plan(tokens, n);
+  const bool ranked = tokens <= kRankMost;
+  for (int i = 0; i < 2; ++i) {  // sum_kernel reads up to kInFlight - 1 words more
+    s.keys[i] = reinterpret_cast<unsigned*>(take(ranked && i ? 0 : tokens + kInFlight));
+    s.tokens[i] = reinterpret_cast<unsigned*>(take(ranked && i ? 0 : tokens + kInFlight));
   }
-  s.counts = reinterpret_cast<unsigned*>(take(one ? 0 : ((tokens + kTile - 1) / kTile) << plan.digit));
+  s.counts = reinterpret_cast<unsigned*>(take(ranked ? 0 : (long long)plan.parts << plan.digit));
   s.joins = reinterpret_cast<unsigned*>(take(1));
   s.join_list = reinterpret_cast<unsigned*>(take(sums.chunks));
   s.heads = reinterpret_cast<float*>(take(sums.chunks * d));
@@ -498,65 +656,76 @@ GradSpace grad_space(long long tokens, long long n, long long d, void* base) {
   return s;
 }
 
-template <class G, class O, int N>
+template <class G, class O, int N, bool kApart>
 cudaError_t sum_t(const LookupGradParams& p, const SumPlan& plan, const GradSpace& s, int at, cudaStream_t stream) {
-  const int lanes = next_pow2((p.d + N - 1) / N, kSumThreads);
+  int lanes = next_pow2((p.d + N - 1) / N, kSumThreads);
+  if (lanes < kSumLanes) lanes = kSumLanes;
   const int groups = kSumThreads / lanes;
   const long long blocks = (plan.chunks + groups - 1) / groups, columns = (p.d + (long long)lanes * N - 1) / ((long long)lanes * N);
   if (blocks > 0x7fffffffll || columns > 65535) return cudaErrorInvalidValue;
-  sum_kernel<G, O, N><<<dim3((unsigned)blocks, (unsigned)columns), kSumThreads, 0, stream>>>(
-    p, plan, s.keys[at], s.tokens[at], s.heads, s.tails, s.joins, s.join_list, lanes);
-  return cudaGetLastError();
+  const dim3 grid((unsigned)blocks, (unsigned)columns);
+  return launch_after(p.tokens > kRankMost, sum_kernel<G, O, N, kApart>, grid, kSumThreads, stream, p, plan, s.keys[at],
+                      s.tokens[at], s.heads, s.tails, s.joins, s.join_list, lanes);
 }
 
 template <class G, class O>
 cudaError_t grad_t(const LookupGradParams& p, cudaStream_t stream) {
   const SumPlan plan = sum_plan(p.tokens, p.d);
-  const SortPlan sort = sort_plan(p.n);
   const GradSpace s = grad_space(p.tokens, p.n, p.d, p.workspace);
-  const int zero_blocks = p.accumulate ? 0 : kSMs;
+  // the zeros in equal parts with each of the sort's launches, by four CTAs per SM
+  const unsigned long long bytes = p.accumulate ? 0 : (unsigned long long)p.n * p.d * sizeof(O);
+  const unsigned long long words = (bytes - (bytes < 16 ? bytes : -reinterpret_cast<uintptr_t>(p.out) & 15)) / 16;
+  auto zeros = [&](int first, int launch, int launches) {
+    ZeroPart z;
+    z.first = first;
+    z.begin = words / launches * launch;
+    z.words = launch + 1 == launches ? words - z.begin : words / launches;
+    z.out = static_cast<unsigned char*>(p.out);
+    z.bytes = bytes;
+    return z;
+  };
+  // (a CTA is there for the single bytes even if there are no words)
+  auto zero_blocks = [&](const ZeroPart& z) { return bytes == 0 ? 0 : z.words / kZeroWords + 1; };
+  cudaError_t e;
   int at = 0;
-  if (p.tokens <= kOneMost) {
-    const int items = (int)((p.tokens + kOneThreads - 1) / kOneThreads);
-    const size_t smem = (size_t)items * kOneThreads * 6 + (size_t)(kOneThreads / 32) * (1 << sort.digit) * 2;
-    cudaError_t e = allow_smem<sort_one_kernel>();
+  if (p.tokens <= kRankMost) {
+    const ZeroPart z = zeros((int)((p.tokens + kRankTokens - 1) / kRankTokens), 0, 1);
+    sort_rank_kernel<<<(unsigned)(z.first + zero_blocks(z)), kRankThreads, 0, stream>>>(p, z, s.keys[0], s.tokens[0], s.joins);
+    e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    sort_one_kernel<<<1 + zero_blocks, kOneThreads, smem, stream>>>(p, sort, s.keys[0], s.tokens[0], s.joins);
   } else {
-    const long long tiles = (p.tokens + kTile - 1) / kTile;
-    const int digits = 1 << sort.digit;
+    const SortPlan sort = sort_plan(p.tokens, p.n);
     for (int pass = 0; pass < sort.passes; ++pass) {
       const unsigned* keys = pass ? s.keys[at] : nullptr;
       const unsigned* tokens = pass ? s.tokens[at] : nullptr;
-      const int to = pass ? 1 - at : 0;
-      sort_count_kernel<<<(unsigned)(tiles + (pass ? 0 : 4 * zero_blocks)), kTileThreads, 0, stream>>>(
-        p, keys, pass * sort.digit, digits, (int)tiles, s.counts, pass ? nullptr : s.joins);
-      sort_scan_kernel<<<1, kOneThreads, 0, stream>>>(s.counts, tiles * digits);
-      sort_place_kernel<<<(unsigned)tiles, kTileThreads, 0, stream>>>(p, keys, tokens, pass * sort.digit, digits,
-                                                                     (int)tiles, s.counts, s.keys[to], s.tokens[to]);
+      const int to = pass ? 1 - at : 0, shift = pass * sort.digit;
+      const ZeroPart first = zeros(sort.parts, 2 * pass, 2 * sort.passes), second = zeros(sort.parts, 2 * pass + 1, 2 * sort.passes);
+      auto* count = sort.items == 4 ? sort_count_kernel<4> : sort_count_kernel<16>;
+      auto* place = sort.items == 4 ? sort_place_kernel<4> : sort_place_kernel<16>;
+      unsigned* joins = pass ? nullptr : s.joins;
+      const dim3 grid((unsigned)(first.first + zero_blocks(first)));
+      // (the first one starts when what came before on the stream is complete)
+      e = launch_after(pass > 0, count, grid, kTileThreads, stream, p, first, sort, keys, shift, s.counts, joins);
+      if (e != cudaSuccess) return e;
+      e = launch_after(true, place, dim3((unsigned)(second.first + zero_blocks(second))), kTileThreads, stream, p, second,
+                       sort, keys, tokens, shift, s.counts, s.keys[to], s.tokens[to]);
+      if (e != cudaSuccess) return e;
       at = to;
     }
   }
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
   const int w = word_bytes(reinterpret_cast<uintptr_t>(p.grad) | (unsigned long long)(p.grad_stride * sizeof(G)) |
                            (unsigned long long)(p.d * sizeof(G)));
   const int to = word_bytes(reinterpret_cast<uintptr_t>(p.out)) / (int)sizeof(O) * (int)sizeof(G);
   if (w == 16 && to * sizeof(O) >= 16 * sizeof(G))
-    e = sum_t<G, O, 16 / sizeof(G)>(p, plan, s, at, stream);
+    e = sum_t<G, O, 16 / sizeof(G), false>(p, plan, s, at, stream);
   else if (w >= 8 && to >= 8)
-    e = sum_t<G, O, 8 / sizeof(G)>(p, plan, s, at, stream);
-  else if (w >= 4 && to >= 4)
-    e = sum_t<G, O, 4 / sizeof(G)>(p, plan, s, at, stream);
+    e = sum_t<G, O, 8 / sizeof(G), false>(p, plan, s, at, stream);
   else
-    e = sum_t<G, O, 1>(p, plan, s, at, stream);
+    e = sum_t<G, O, 4, true>(p, plan, s, at, stream);
   if (e != cudaSuccess || plan.chunks < 2) return e;
-  const long long columns = (p.d + 31) / 32;
-  if (columns > 65535) return cudaErrorInvalidValue;
-  const long long rows = plan.chunks < 4 * kSMs ? plan.chunks : 4 * kSMs;
-  join_kernel<G, O><<<dim3((unsigned)rows, (unsigned)columns), kJoinWarps * 32, 0, stream>>>(
-    p, plan, s.keys[at], s.heads, s.tails, s.joins, s.join_list);
-  return cudaGetLastError();
+  const long long items = plan.chunks * ((p.d + kJoinDims - 1) / kJoinDims), wanted = (items + kJoinWarps - 1) / kJoinWarps;
+  return launch_after(p.tokens > kRankMost, join_kernel<O>, dim3((unsigned)(wanted < 6 * kSMs ? wanted : 6 * kSMs)),
+                      kJoinWarps * 32, stream, p, plan, s.keys[at], s.heads, s.tails, s.joins, s.join_list);
 }
 
 }  // namespace
