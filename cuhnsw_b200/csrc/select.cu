@@ -48,6 +48,11 @@ __device__ __forceinline__ bool none(const TotalKey& k) { return k.total == 0; }
 __device__ __forceinline__ void clear(ScoreKey& k) { k = 0; }
 __device__ __forceinline__ void clear(TotalKey& k) { k = {0, 0, 0}; }
 
+__device__ __forceinline__ ScoreKey from_lane(ScoreKey k, int lane) { return shfl64(k, lane); }
+__device__ __forceinline__ TotalKey from_lane(const TotalKey& k, int lane) {
+  return {shfl64(k.total, lane), __shfl_sync(FULL, k.place, lane), __shfl_sync(FULL, k.beam, lane)};
+}
+
 // Candidates of a CTA in shared memory, in any order; `sort` puts them in descending order.
 template <class Key>
 struct Pool {
@@ -57,11 +62,25 @@ struct Pool {
 
   __device__ void push(const Key& k) { keys[atomicAdd(count, 1)] = k; }
 
-  // Bitonic over the smallest power of two that holds them; all threads.
+  // All threads.  Up to a warp's worth are ranked by one warp; more go through a bitonic network over the smallest power of two
+  // that holds them.
   __device__ void sort() {
     __syncthreads();
     const int held = *count;
-    int size = 2;
+    if (held <= 32) {
+      if (threadIdx.x < 32) {
+        Key mine;
+        clear(mine);
+        if ((int)threadIdx.x < held) mine = keys[threadIdx.x];
+        int rank = 0;
+        for (int i = 0; i < held; ++i) rank += above(from_lane(mine, i), mine);
+        __syncwarp();
+        if ((int)threadIdx.x < held) keys[rank] = mine;
+      }
+      __syncthreads();
+      return;
+    }
+    int size = 64;
     while (size < held) size <<= 1;
     for (int i = held + threadIdx.x; i < size; i += kThreads) clear(keys[i]);
     for (int span = 2; span <= size; span <<= 1) {
@@ -98,119 +117,114 @@ struct Pool {
 
 // Every thread holds kEach scores.  The CTA's `keep` best: a bound that at least `keep` of them reach (groups of threads
 // are at least that many, and the smallest of the groups' largest scores is reached once in each), everything from there on
-// into a pool, the pool in order.  Also the piece's largest score and its sum of exponentials.
+// into a pool, the pool in order.  Also the piece's largest score and its sum of exponentials.  Bound: HBM bytes, and the
+// instructions for every score: its part in the maximum, in the sum, and one comparison.
 constexpr int kPoolScores = 2048;
+constexpr int kWarps = kThreads / 32;
+
+__device__ __forceinline__ float exp2_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 template <class T, int N, int kEach>
 __global__ void __launch_bounds__(kThreads) piece_kernel(SelectParams p, int pieces, ScoreKey* best, float2* norms) {
   __shared__ ScoreKey pool_keys[kPoolScores];
   __shared__ int pool_count;
-  __shared__ ScoreKey firsts[kThreads];
-  __shared__ float warp_max[kThreads / 32], warp_sum[kThreads / 32];
+  __shared__ float firsts[kThreads];
+  __shared__ float warp_max[kWarps], warp_sum[kWarps];
   const int warp = threadIdx.x >> 5, lane = lane_id();
   const long long row = blockIdx.y + (long long)blockIdx.z * 65535;
   if (row >= p.sequences * p.beams) return;
   const long long seq = row / p.beams, beam = row % p.beams;
   const T* scores = static_cast<const T*>(p.scores) + seq * p.seq_stride + beam * p.beam_stride;
-  const long long begin = (long long)blockIdx.x * kThreads * kEach;
+  const int vocabulary = (int)p.vocabulary;
+  const unsigned begin = blockIdx.x * (unsigned)(kThreads * kEach);  // (below 2^31, and so is the vocabulary)
+  auto place = [&](int i) { return begin + (unsigned)((i / N * kThreads + threadIdx.x) * N + i % N); };
+  if (threadIdx.x == 0) pool_count = 0;
   float x[kEach];
 #pragma unroll
   for (int i = 0; i < kEach; i += N) {
-    const long long at = begin + (long long)(i / N * kThreads + threadIdx.x) * N;
-    if (at + N <= p.vocabulary) {
+    const unsigned at = place(i);
+    if (at + N <= (unsigned)vocabulary) {
       const Vec<T, N> v = load_stream<T, N>(scores + at);
 #pragma unroll
       for (int j = 0; j < N; ++j) x[i + j] = to_f32(v.v[j]);
     } else {
 #pragma unroll
-      for (int j = 0; j < N; ++j) x[i + j] = at + j < p.vocabulary ? to_f32(scores[at + j]) : -INFINITY;
+      for (int j = 0; j < N; ++j) x[i + j] = at + j < (unsigned)vocabulary ? to_f32(scores[at + j]) : -INFINITY;
     }
   }
-  auto place = [&](int i) { return (unsigned)(begin + (long long)(i / N * kThreads + threadIdx.x) * N + i % N); };
-  float top = -INFINITY;
+  float top = x[0];
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) top = fmaxf(top, x[i]);
-  ScoreKey mine = 0;
+  for (int i = 1; i < kEach; ++i) top = fmaxf(top, x[i]);
+  // groups of `lanes` threads, at least `keep` of them; their largest scores
+  int lanes = kThreads;
+  while (lanes > 1 && kThreads / lanes < p.keep) lanes >>= 1;
+  float of_group = top, of_warp = top;
 #pragma unroll
-  for (int i = kEach - 1; i >= 0; --i)
-    if (x[i] == top) mine = score_key(top, place(i));
+  for (int off = 1; off < 32; off <<= 1) {
+    of_warp = fmaxf(of_warp, __shfl_xor_sync(FULL, of_warp, off));
+    if (off < lanes) of_group = of_warp;
+  }
+  firsts[threadIdx.x] = of_group;
+  if (lane == 0) warp_max[warp] = of_warp;
+  __syncthreads();
+  float most = -FLT_MAX, least = INFINITY;  // (of a row of -inf the exponentials are zeros)
+  if (lanes <= 32) {
+    for (int i = lane * lanes; i < kThreads; i += 32 * lanes) least = fminf(least, firsts[i]);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) least = fminf(least, __shfl_xor_sync(FULL, least, off));
+  } else {
+    for (int w = 0; w < kWarps; w += lanes / 32) {
+      float of_warps = warp_max[w];
+      for (int v = 1; v < lanes / 32; ++v) of_warps = fmaxf(of_warps, warp_max[w + v]);
+      least = fminf(least, of_warps);
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) most = fmaxf(most, warp_max[w]);
   if (p.log_softmax) {
-    float most = top;
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(FULL, most, off));
-    if (lane == 0) warp_max[warp] = most;
-    __syncthreads();
-    most = -FLT_MAX;  // (of a row of -inf the exponentials are zeros)
-    for (int w = 0; w < kThreads / 32; ++w) most = fmaxf(most, warp_max[w]);
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) sum += __expf(x[i] - most);
+    for (int i = 0; i < kEach; ++i) sum += exp2_of((x[i] - most) * 1.44269504f);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(FULL, sum, off);
     if (lane == 0) warp_sum[warp] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      float all = 0.0f;
-      for (int w = 0; w < kThreads / 32; ++w) all += warp_sum[w];
-      norms[row * pieces + blockIdx.x] = make_float2(most, all);
-    }
   }
-  // the bound: groups of `lanes` threads
-  int lanes = kThreads;
-  while (lanes > 1 && kThreads / lanes < p.keep) lanes >>= 1;
-  ScoreKey bound = mine;
-  for (int off = 1; off < lanes && off < 32; off <<= 1) {
-    const ScoreKey other = shfl64(bound, lane ^ off);
-    bound = other > bound ? other : bound;
-  }
-  firsts[threadIdx.x] = bound;
-  if (threadIdx.x == 0) pool_count = 0;
-  __syncthreads();
-  const int stride = min(lanes, 32);
-  if (lanes > 32) {
-    // a group is several warps
-    ScoreKey of_group = 0;
-    const int from = threadIdx.x / lanes * lanes;
-    for (int i = from; i < from + lanes; i += 32) of_group = firsts[i] > of_group ? firsts[i] : of_group;
-    bound = of_group;
-    __syncthreads();
-    firsts[threadIdx.x] = bound;
-    __syncthreads();
-  }
-  // the smallest over the groups
-  ScoreKey least = ~0ull;
-  for (int i = lane * stride; i < kThreads; i += 32 * stride) least = firsts[i] < least ? firsts[i] : least;
-  for (int off = 16; off > 0; off >>= 1) {
-    const ScoreKey other = shfl64(least, lane ^ off);
-    least = other < least ? other : least;
-  }
+  // -inf and NaN are no candidates: neither is at least the lowest number.  (A group without scores has no largest one.)
+  const float bound = fmaxf(least, -FLT_MAX);
   int passing = 0;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const ScoreKey k = score_key(x[i], place(i));
-    passing += k != 0 && k >= least;
-  }
+  for (int i = 0; i < kEach; ++i) passing += x[i] >= bound;
   Pool<ScoreKey> pool{pool_keys, &pool_count, kPoolScores};
-  if (__syncthreads_count(passing > 0) == 0) {
-    // nothing to choose from
-  } else if (__syncthreads_or(passing > kPoolScores / kThreads) == 0) {
+  if (__syncthreads_or(passing > kPoolScores / kThreads) == 0) {
+    if (passing > 0) {
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const ScoreKey k = score_key(x[i], place(i));
-      if (k != 0 && k >= least) pool.push(k);
+      for (int i = 0; i < kEach; ++i)
+        if (x[i] >= bound) pool.push(score_key(x[i], place(i)));
     }
   } else {
+    // so many that they may not fit: a score of each thread at a time
+    ScoreKey from = 0;
 #pragma unroll 1
     for (int i = 0; i < kEach; ++i) {
-      pool.make_room(p.keep, least);
+      pool.make_room(p.keep, from);
       float xi = x[0];
 #pragma unroll
       for (int j = 1; j < kEach; ++j) xi = j == i ? x[j] : xi;
       const ScoreKey k = score_key(xi, place(i));
-      if (k != 0 && k >= least) pool.push(k);
+      if (xi >= bound && k >= from) pool.push(k);
     }
   }
   pool.sort();
+  if (p.log_softmax && threadIdx.x == 0) {
+    float all = warp_sum[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) all += warp_sum[w];
+    norms[row * pieces + blockIdx.x] = make_float2(most, all);
+  }
   ScoreKey* to = best + (row * pieces + blockIdx.x) * p.keep;
   const int held = min(pool_count, p.keep);
   for (int i = threadIdx.x; i < p.keep; i += kThreads) to[i] = i < held ? pool_keys[i] : 0;
@@ -220,8 +234,8 @@ __global__ void __launch_bounds__(kThreads) piece_kernel(SelectParams p, int pie
 
 constexpr int kPoolTotals = 2048;
 
-// One CTA per sequence: all pieces' lists in order of rank, so that the best of every list come first and the bound rises
-// at once.
+// One CTA per sequence.  The lists of the pieces are in order: of their first totals the `keep`-th is a bound that as many
+// candidates reach, and from there on there are few.
 __global__ void __launch_bounds__(kThreads) sequence_kernel(SelectParams p, int pieces, const ScoreKey* best,
                                                             const float2* norms) {
   extern __shared__ __align__(16) unsigned char smem[];
@@ -231,17 +245,21 @@ __global__ void __launch_bounds__(kThreads) sequence_kernel(SelectParams p, int 
   const int lane = lane_id(), warp = threadIdx.x >> 5;
   const long long seq = blockIdx.x;
   const int beams = (int)p.beams;
+  const long long lists = (long long)beams * pieces, total = lists * p.keep;
+  const ScoreKey* mine = best + seq * total;
   if (threadIdx.x == 0) pool_count = 0;
-  for (int b = warp; b < beams; b += kThreads / 32) {
+  const ScoreKey first = (long long)threadIdx.x < lists ? mine[threadIdx.x * p.keep] : 0;  // on its way meanwhile
+  for (int b = warp; b < beams; b += kWarps) {
     double offset = p.totals ? (double)p.totals[seq * beams + b] : 0.0;
     if (p.log_softmax) {
       const float2* of_row = norms + (seq * beams + b) * pieces;
-      float most = -FLT_MAX;
-      for (int i = lane; i < pieces; i += 32) most = fmaxf(most, of_row[i].x);
+      const float2 norm = lane < pieces ? of_row[lane] : make_float2(-FLT_MAX, 0.0f);
+      float most = norm.x;
+      for (int i = lane + 32; i < pieces; i += 32) most = fmaxf(most, of_row[i].x);
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(FULL, most, off));
-      double sum = 0.0;
-      for (int i = lane; i < pieces; i += 32) sum += of_row[i].y * exp((double)of_row[i].x - (double)most);
+      double sum = norm.y * exp((double)norm.x - (double)most);
+      for (int i = lane + 32; i < pieces; i += 32) sum += of_row[i].y * exp((double)of_row[i].x - (double)most);
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(FULL, sum, off);
       offset -= (double)most + log(sum);
@@ -249,30 +267,50 @@ __global__ void __launch_bounds__(kThreads) sequence_kernel(SelectParams p, int 
     if (lane == 0) offsets[b] = offset;
   }
   __syncthreads();
+  auto total_key = [&](long long list, ScoreKey k) {
+    TotalKey key = {0, 0, 0};
+    if (k == 0) return key;
+    const unsigned beam = (unsigned)list / (unsigned)pieces;
+    const double value = offsets[beam] + (double)key_score(k);
+    if (value > -INFINITY) key = {d2ord(value), key_place(k), beam};
+    return key;
+  };
   Pool<TotalKey> pool{pool_keys, &pool_count, kPoolTotals};
   TotalKey least = {0, 0, 0};
-  const long long lists = (long long)beams * pieces, total = lists * p.keep;
-  const ScoreKey* mine = best + seq * total;
+  if (lists >= p.keep && total > kThreads) {
+    // the best first total of each thread's lists, the `keep`-th of them all
+    TotalKey top = total_key(threadIdx.x, first);
+    for (long long list = threadIdx.x + kThreads; list < lists; list += kThreads) {
+      const TotalKey key = total_key(list, mine[list * p.keep]);
+      if (above(key, top)) top = key;
+    }
+    pool_keys[threadIdx.x] = top;
+    __syncthreads();
+    const int held = (int)min((long long)kThreads, lists);
+    int rank = 0;
+    if (!none(top))
+      for (int i = 0; i < held; ++i) rank += above(pool_keys[i], top);
+    __syncthreads();
+    if (!none(top) && rank == p.keep - 1) pool_keys[0] = top;
+    const bool there = __syncthreads_or(!none(top) && rank == p.keep - 1);
+    if (there) least = pool_keys[0];
+    __syncthreads();
+  }
+  // list by list of the same rank: the best ones first
   for (long long begin = 0; begin < total; begin += kThreads) {
     pool.make_room(p.keep, least);
     const long long i = begin + threadIdx.x;
     if (i < total) {
-      const long long list = i % lists, rank = i / lists;
-      const ScoreKey k = mine[list * p.keep + rank];
-      if (k != 0) {
-        const unsigned beam = (unsigned)(list / pieces);
-        const double value = offsets[beam] + (double)key_score(k);
-        if (value > -INFINITY) {
-          const TotalKey key = {d2ord(value), key_place(k), beam};
-          if (none(least) || !above(least, key)) pool.push(key);
-        }
-      }
+      const unsigned long long list = total < (1ll << 32) ? (unsigned)i % (unsigned)lists : i % lists;
+      const unsigned long long rank = total < (1ll << 32) ? (unsigned)i / (unsigned)lists : i / lists;
+      const TotalKey key = total_key(list, mine[list * p.keep + rank]);
+      if (!none(key) && !above(least, key)) pool.push(key);
     }
   }
   pool.sort();
   const int found = min(pool_count, p.keep);
   for (int i = threadIdx.x; i < p.keep; i += kThreads) {
-    const TotalKey k = pool_keys[min(i, kPoolTotals - 1)];
+    const TotalKey k = pool_keys[i];
     const long long at = seq * p.keep + i;
     p.out_totals[at] = p.sign * (i < found ? (float)ord2d(k.total) : -INFINITY);
     if (p.out_beams) p.out_beams[at] = i < found ? (int)k.beam : -1;

@@ -132,16 +132,15 @@ __device__ __forceinline__ unsigned key_at(const LookupGradParams& p, long long 
 }
 
 // Up to kRankMost tokens: every token's place is the number of smaller keys and of equal ones before it, counted against all
-// tokens: no pass depends on another one.  16 384 tokens take 17 us spread over all SMs, 511 about 2.
-constexpr int kRankMost = 16384;
+// tokens: no pass depends on another one.  8192 tokens take 14 us, 2048 seven, 511 three.
+constexpr int kRankMost = 8192;
 constexpr int kRankThreads = kZeroThreads;
 constexpr int kRankTokens = 64;                                // of a CTA
 constexpr int kRankShares = kRankThreads / kRankTokens;        // threads that share a token
 constexpr int kRankTile = 2048;                                // keys in shared memory at a time
 
-__global__ void __launch_bounds__(kRankThreads) sort_rank_kernel(LookupGradParams p, ZeroPart zeros, unsigned* keys_out,
-                                                                 unsigned* tokens_out, unsigned* joins) {
-  next_launch_may_start();
+__global__ void __launch_bounds__(kRankThreads) sort_rank_kernel(LookupGradParams p, ZeroPart zeros, uint2* sorted,
+                                                                 unsigned* joins) {
   if ((int)blockIdx.x >= zeros.first) {
     write_zeros(zeros);
     return;
@@ -195,15 +194,14 @@ __global__ void __launch_bounds__(kRankThreads) sort_rank_kernel(LookupGradParam
   if (share == 0 && token < count) {
 #pragma unroll
     for (int s = 1; s < kRankShares; ++s) below += counts[s][mine];
-    keys_out[below] = key;
-    tokens_out[below] = token;
+    sorted[below] = make_uint2(key, token);
   }
 }
 
-// More tokens: a least-significant-digit radix sort.  At most kParts CTAs have a contiguous part of the tokens each; a pass
-// counts the digits of each part, and then every part finds out where its tokens of each digit begin and puts them there, tile by
-// tile.
-constexpr int kParts = 2 * kSMs;
+// More tokens: a least-significant-digit radix sort.  Up to kParts CTAs have a contiguous part of the tokens each; a pass counts the
+// digits of each part, finds out where its tokens of each digit begin and puts them there, tile by tile.
+constexpr int kParts = 16 * kSMs;
+constexpr int kPartsUnscanned = 64;     // every CTA adds up the counts of so few parts by itself
 constexpr int kTileThreads = kZeroThreads;
 constexpr int kTileWarps = kTileThreads / 32;
 constexpr int kMaxDigit = 8;
@@ -211,6 +209,7 @@ constexpr int kMaxDigit = 8;
 struct SortPlan {
   int passes, digit;      // bits
   int items;              // tokens of a tile per thread: 4 or 16
+  int scanned;            // whether counts become places in a launch of their own
   int parts;
   long long part;         // tokens, whole tiles
 };
@@ -221,18 +220,19 @@ SortPlan sort_plan(long long tokens, long long n) {
   s.passes = (bits + kMaxDigit - 1) / kMaxDigit;
   s.digit = (bits + s.passes - 1) / s.passes;
   if (s.digit < 2) s.digit = 2;  // (four counts are read at a time)
-  // small tiles while they are enough for a part each: more CTAs that take less time
+  // small tiles while each is a part: more CTAs that take less time
   s.items = tokens <= (long long)kParts * kTileThreads * 4 ? 4 : 16;
   const long long tile = kTileThreads * s.items, tiles = (tokens + tile - 1) / tile;
   s.part = (tiles + kParts - 1) / kParts * tile;
   s.parts = (int)((tokens + s.part - 1) / s.part);
+  s.scanned = s.parts > kPartsUnscanned;
   return s;
 }
 
-// counts[part * digits + digit]
+// counts[part * digits + digit].  `pairs`: (key, token) as the pass before left them; the first pass reads the ids.
 template <int kTileItems>
 __global__ void __launch_bounds__(kTileThreads) sort_count_kernel(LookupGradParams p, ZeroPart zeros, SortPlan plan,
-                                                                  const unsigned* keys, int shift, unsigned* counts,
+                                                                  const uint2* pairs, int shift, unsigned* counts,
                                                                   unsigned* joins) {
   next_launch_may_start();
   if ((int)blockIdx.x >= zeros.first) {
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kTileThreads) sort_count_kernel(LookupGradPara
   const int digits = 1 << plan.digit;
   __shared__ unsigned bins[1 << kMaxDigit];
   for (int i = threadIdx.x; i < digits; i += kTileThreads) bins[i] = 0;
-  if (keys) wait_for_launch_before();
+  if (pairs) wait_for_launch_before();
   if (joins && blockIdx.x == 0 && threadIdx.x == 0) *joins = 0;
   __syncthreads();
   const long long begin = blockIdx.x * plan.part, end = min(begin + plan.part, p.tokens);
@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kTileThreads) sort_count_kernel(LookupGradPara
 #pragma unroll
     for (int i = 0; i < kTileItems; ++i) {
       const long long at = tile + i * kTileThreads + threadIdx.x;
-      key[i] = at >= end ? 0 : keys ? keys[at] : key_at(p, at);
+      key[i] = at >= end ? 0 : pairs ? pairs[at].x : key_at(p, at);
     }
 #pragma unroll
     for (int i = 0; i < kTileItems; ++i) {
@@ -265,6 +265,46 @@ __global__ void __launch_bounds__(kTileThreads) sort_count_kernel(LookupGradPara
   }
   __syncthreads();
   for (int i = threadIdx.x; i < digits; i += kTileThreads) counts[blockIdx.x * digits + i] = bins[i];
+}
+
+// Exclusive sum of one value per thread over a CTA of kTileThreads.
+__device__ __forceinline__ unsigned block_exclusive(unsigned x, unsigned* scratch /* kTileWarps */) {
+  const int lane = lane_id(), warp = threadIdx.x >> 5;
+  unsigned upto = x;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const unsigned y = __shfl_up_sync(FULL, upto, off);
+    if (lane >= off) upto += y;
+  }
+  if (lane == 31) scratch[warp] = upto;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kTileWarps; ++w) upto += w < warp ? scratch[w] : 0;
+  return upto - x;
+}
+
+// For each digit, one CTA: counts become the tokens of that digit in the parts before, and totals[digit] their number in all.
+constexpr int kScanEach = (kParts + kTileThreads - 1) / kTileThreads;
+__global__ void __launch_bounds__(kTileThreads) sort_scan_kernel(unsigned* counts, unsigned* totals, int digits, int parts) {
+  __shared__ unsigned scratch[kTileThreads / 32];
+  next_launch_may_start();
+  wait_for_launch_before();
+  const int digit = blockIdx.x;
+  unsigned c[kScanEach], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kScanEach; ++i) {
+    const int part = threadIdx.x * kScanEach + i;
+    c[i] = part < parts ? counts[part * digits + digit] : 0;
+    sum += c[i];
+  }
+  unsigned before = block_exclusive(sum, scratch);
+  if (threadIdx.x == kTileThreads - 1) totals[digit] = before + sum;
+#pragma unroll
+  for (int i = 0; i < kScanEach; ++i) {
+    const int part = threadIdx.x * kScanEach + i;
+    if (part < parts) counts[part * digits + digit] = before;
+    before += c[i];
+  }
 }
 
 // Rank of each of a warp's keys (lane l holds items l, 32 + l, ..) among the earlier keys of the warp with the same
@@ -287,11 +327,11 @@ __device__ __forceinline__ void warp_ranks(const unsigned (&key)[Items], int shi
   }
 }
 
+// Every tile is put in order in shared memory first, so that what goes to one digit's places is written side by side.
 template <int kTileItems>
 __global__ void __launch_bounds__(kTileThreads) sort_place_kernel(LookupGradParams p, ZeroPart zeros, SortPlan plan,
-                                                                  const unsigned* keys, const unsigned* tokens,
-                                                                  int shift, const unsigned* counts, unsigned* keys_out,
-                                                                  unsigned* tokens_out) {
+                                                                  const uint2* pairs, int shift, const unsigned* counts,
+                                                                  uint2* sorted) {
   next_launch_may_start();
   if ((int)blockIdx.x >= zeros.first) {
     write_zeros(zeros);
@@ -301,75 +341,96 @@ __global__ void __launch_bounds__(kTileThreads) sort_place_kernel(LookupGradPara
   constexpr int kDigits = 1 << kMaxDigit;
   static_assert(kDigits == kTileThreads, "a digit per thread");
   __shared__ unsigned short warp_counts[kTileWarps * kDigits];
-  __shared__ unsigned bases[kTileWarps * kDigits], starts[kDigits], before[kDigits], scratch[kTileWarps];
+  __shared__ unsigned starts[kDigits], before[kDigits], scratch[2][kTileWarps];
+  __shared__ uint2 tile_pairs[kTile];
   const int digits = 1 << plan.digit, warp = threadIdx.x >> 5, lane = lane_id(), parts = plan.parts;
-  // tokens of each digit in all parts, and in the ones before this: every warp takes some of the parts, a lane four digits
-  for (int i = threadIdx.x; i < digits; i += kTileThreads) starts[i] = before[i] = 0;
-  wait_for_launch_before();
-  __syncthreads();
-  for (int d = 4 * lane; d < digits; d += 128) {
-    unsigned all[4] = {0, 0, 0, 0}, earlier[4] = {0, 0, 0, 0};
-#pragma unroll 8
-    for (int i = warp; i < parts; i += kTileWarps) {
-      const uint4 c = *reinterpret_cast<const uint4*>(counts + i * digits + d);
-      const bool earlier_part = i < (int)blockIdx.x;
-      all[0] += c.x, all[1] += c.y, all[2] += c.z, all[3] += c.w;
-      earlier[0] += earlier_part ? c.x : 0, earlier[1] += earlier_part ? c.y : 0;
-      earlier[2] += earlier_part ? c.z : 0, earlier[3] += earlier_part ? c.w : 0;
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      atomicAdd(starts + d + k, all[k]);
-      atomicAdd(before + d + k, earlier[k]);
-    }
-  }
-  __syncthreads();
-  {
-    const unsigned x = (int)threadIdx.x < digits ? starts[threadIdx.x] : 0;
-    unsigned sum = x;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const unsigned y = __shfl_up_sync(FULL, sum, off);
-      if (lane >= off) sum += y;
-    }
-    if (lane == 31) scratch[warp] = sum;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) sum += scratch[w];
-    if ((int)threadIdx.x < digits) starts[threadIdx.x] = sum - x + before[threadIdx.x];
-  }
   const long long part_begin = blockIdx.x * plan.part, part_end = min(part_begin + plan.part, p.tokens);
-  for (long long tile = part_begin; tile < part_end; tile += kTile) {
-    for (int i = threadIdx.x; i < kTileWarps * digits / 2; i += kTileThreads) reinterpret_cast<unsigned*>(warp_counts)[i] = 0;
-    const long long begin = min(tile + warp * 32 * kTileItems, part_end);
-    const int valid = (int)min((long long)(32 * kTileItems), part_end - begin);
-    unsigned key[kTileItems], token[kTileItems], rank[kTileItems];
+  unsigned key[kTileItems], token[kTileItems], rank[kTileItems];
+  auto load = [&](long long tile) {
+    const long long begin = tile + warp * 32 * kTileItems + lane;
 #pragma unroll
     for (int i = 0; i < kTileItems; ++i) {
-      if (i * 32 + lane < valid) {
-        const long long at = begin + i * 32 + lane;
-        key[i] = keys ? keys[at] : key_at(p, at);
-        token[i] = tokens ? tokens[at] : (unsigned)at;
+      const long long at = begin + i * 32;
+      if (at < part_end) {
+        const uint2 pair = pairs ? pairs[at] : make_uint2(key_at(p, at), (unsigned)at);
+        key[i] = pair.x;
+        token[i] = pair.y;
       }
     }
+  };
+  // tokens of each digit in all parts, and in the ones before this
+  if (plan.scanned) {
+    wait_for_launch_before();
+    load(part_begin);
+    if ((int)threadIdx.x < digits) {
+      starts[threadIdx.x] = counts[parts * digits + threadIdx.x];
+      before[threadIdx.x] = counts[blockIdx.x * digits + threadIdx.x];
+    }
+  } else {
+    // every warp takes some of the parts, a lane four digits
+    for (int i = threadIdx.x; i < digits; i += kTileThreads) starts[i] = before[i] = 0;
+    wait_for_launch_before();
+    load(part_begin);
+    __syncthreads();
+    for (int d = 4 * lane; d < digits; d += 128) {
+      unsigned all[4] = {0, 0, 0, 0}, earlier[4] = {0, 0, 0, 0};
+#pragma unroll 8
+      for (int i = warp; i < parts; i += kTileWarps) {
+        const uint4 c = *reinterpret_cast<const uint4*>(counts + i * digits + d);
+        const bool earlier_part = i < (int)blockIdx.x;
+        all[0] += c.x, all[1] += c.y, all[2] += c.z, all[3] += c.w;
+        earlier[0] += earlier_part ? c.x : 0, earlier[1] += earlier_part ? c.y : 0;
+        earlier[2] += earlier_part ? c.z : 0, earlier[3] += earlier_part ? c.w : 0;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        atomicAdd(starts + d + k, all[k]);
+        atomicAdd(before + d + k, earlier[k]);
+      }
+    }
+  }
+  __syncthreads();
+  const bool mine = (int)threadIdx.x < digits;  // the thread's digit, and where its next token goes
+  unsigned next = block_exclusive(mine ? starts[threadIdx.x] : 0, scratch[0]) + (mine ? before[threadIdx.x] : 0);
+  for (long long tile = part_begin; tile < part_end; tile += kTile) {
+    if (tile > part_begin) load(tile);
+    for (int i = threadIdx.x; i < kTileWarps * digits / 2; i += kTileThreads) reinterpret_cast<unsigned*>(warp_counts)[i] = 0;
+    const int held = (int)min((long long)kTile, part_end - tile);
+    const int valid = max(0, min(32 * kTileItems, held - warp * 32 * kTileItems));
     __syncthreads();
     warp_ranks<kTileItems>(key, shift, digits - 1, valid, warp_counts + warp * digits, rank);
     __syncthreads();
-    if ((int)threadIdx.x < digits) {
-      unsigned base = starts[threadIdx.x];
+    // a digit's tokens in the warps before, and in the tile
+    unsigned total = 0;
+    if (mine) {
 #pragma unroll
       for (int w = 0; w < kTileWarps; ++w) {
-        bases[w * digits + threadIdx.x] = base;
-        base += warp_counts[w * digits + threadIdx.x];
+        const unsigned c = warp_counts[w * digits + threadIdx.x];
+        warp_counts[w * digits + threadIdx.x] = (unsigned short)total;
+        total += c;
       }
-      starts[threadIdx.x] = base;
+    }
+    const unsigned local = block_exclusive(total, scratch[1]);
+    if (mine) {
+      starts[threadIdx.x] = local;         // the digit's first place in the tile
+      before[threadIdx.x] = next - local;  // from a place in the tile to one in the result
+      next += total;
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kTileItems; ++i) {
       if (i * 32 + lane < valid) {
-        const unsigned at = bases[warp * digits + ((key[i] >> shift) & (digits - 1))] + rank[i];
-        keys_out[at] = key[i];
-        tokens_out[at] = token[i];
+        const unsigned digit = (key[i] >> shift) & (digits - 1);
+        tile_pairs[starts[digit] + warp_counts[warp * digits + digit] + rank[i]] = make_uint2(key[i], token[i]);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kTileItems; ++i) {
+      const int at = i * kTileThreads + threadIdx.x;
+      if (at < held) {
+        const uint2 pair = tile_pairs[at];
+        sorted[before[(pair.x >> shift) & (digits - 1)] + at] = pair;
       }
     }
     __syncthreads();
@@ -383,12 +444,12 @@ __global__ void __launch_bounds__(kTileThreads) sort_place_kernel(LookupGradPara
 // partial sum in fp32 (heads: of the row that the chunk before began; tails: of the row that goes on in the next one), and
 // join_kernel adds those up.
 constexpr int kSumThreads = 256;
-constexpr int kInFlight = 8;
+constexpr int kInFlight = 4;
 constexpr int kMostChunk = 64;
 constexpr int kSumLanes = 8;   // threads of a chunk at least
 
 struct SumPlan {
-  int chunk;         // tokens, a multiple of kInFlight
+  int chunk;         // tokens, a multiple of 2 * kInFlight
   long long chunks;
 };
 SumPlan sum_plan(long long tokens, long long d) {
@@ -396,7 +457,7 @@ SumPlan sum_plan(long long tokens, long long d) {
   // chunks of 64 tokens where that leaves every SM some 14 000 values to add side by side, shorter ones for fewer tokens (but
   // the shorter they are the more partial sums there are)
   s.chunk = kMostChunk;
-  const int least = tokens > 8192 ? 2 * kInFlight : kInFlight;
+  const int least = tokens > 8192 ? 16 : 8;
   while (s.chunk > least && tokens / s.chunk * d < (long long)kSMs * 14'000) s.chunk /= 2;
   s.chunks = (tokens + s.chunk - 1) / s.chunk;
   return s;
@@ -420,10 +481,10 @@ __device__ __forceinline__ void write_row(const LookupGradParams& p, unsigned ro
 // `lanes` threads have a chunk (of up to lanes * N dimensions); kInFlight rows of the gradient are on their way to each.  A
 // thread has N neighbouring values or, of rows that are no whole words (kApart), N values `lanes` apart.
 template <class G, class O, int N, bool kApart>
-__global__ void __launch_bounds__(kSumThreads, 3) sum_kernel(LookupGradParams p, SumPlan plan, const unsigned* keys,
-                                                          const unsigned* tokens, float* heads, float* tails,
-                                                          unsigned* joins, unsigned* join_list, int lanes) {
-  const int group = threadIdx.x / lanes, lane = threadIdx.x % lanes, groups = kSumThreads / lanes;
+__global__ void __launch_bounds__(kSumThreads, kApart || sizeof(G) * N > 8 ? 3 : 4) sum_kernel(LookupGradParams p, SumPlan plan, const uint2* sorted,
+                                                                                   float* heads, float* tails, unsigned* joins,
+                                                                                   unsigned* join_list, int lanes) {
+  const int group = threadIdx.x / lanes, lane = threadIdx.x % lanes, groups = blockDim.x / lanes;
   const long long chunk = (long long)blockIdx.x * groups + group;
   next_launch_may_start();
   wait_for_launch_before();
@@ -431,8 +492,9 @@ __global__ void __launch_bounds__(kSumThreads, 3) sum_kernel(LookupGradParams p,
   const unsigned none = (unsigned)p.n;
   const long long begin = chunk * plan.chunk, end = min(begin + plan.chunk, p.tokens);
   for (int i = lane; i < plan.chunk; i += lanes) {  // (the end of the last chunk as empty slots)
-    chunk_keys[group][i] = begin + i < end ? keys[begin + i] : none;
-    chunk_tokens[group][i] = begin + i < end ? tokens[begin + i] : 0;
+    const uint2 pair = begin + i < end ? sorted[begin + i] : make_uint2(none, 0);
+    chunk_keys[group][i] = pair.x;
+    chunk_tokens[group][i] = pair.y;
   }
   __syncthreads();
   if (chunk >= plan.chunks) return;
@@ -440,7 +502,7 @@ __global__ void __launch_bounds__(kSumThreads, 3) sum_kernel(LookupGradParams p,
   if (c >= p.d) return;
   const int held = kApart ? (int)min((long long)N, (p.d - c + lanes - 1) / lanes) : N;  // values
   const G* grad = static_cast<const G*>(p.grad) + c;
-  const unsigned before = begin > 0 ? keys[begin - 1] : none, after = end < p.tokens ? keys[end] : none;
+  const unsigned before = begin > 0 ? sorted[begin - 1].x : none, after = end < p.tokens ? sorted[end].x : none;
   unsigned row = chunk_keys[group][0];
   bool head = row == before;  // the row that the chunk begins with is another chunk's as well
   float sum[N];
@@ -467,29 +529,28 @@ __global__ void __launch_bounds__(kSumThreads, 3) sum_kernel(LookupGradParams p,
       write_row<O, N>(p, row, c, sum);
     }
   };
-  for (int t = 0; t < plan.chunk; t += kInFlight) {
-    unsigned key[kInFlight];
-#pragma unroll
-    for (int i = 0; i < kInFlight; i += 4) {
-      const uint4 k = *reinterpret_cast<const uint4*>(chunk_keys[group] + t + i);
-      key[i] = k.x, key[i + 1] = k.y, key[i + 2] = k.z, key[i + 3] = k.w;
-    }
-    // (whole words: a value of 16 bits that waits by itself takes a register)
-    using Word = typename WordOf<kApart ? sizeof(G) : sizeof(G) * N>::type;
-    constexpr int kWords = kApart ? N : 1;
-    Word word[kInFlight][kWords];
+  // (whole words: a value of 16 bits that waits by itself takes a register)
+  using Word = typename WordOf<kApart ? sizeof(G) : sizeof(G) * N>::type;
+  constexpr int kWords = kApart ? N : 1;
+  auto fetch = [&](int t, Word (&word)[kInFlight][kWords]) {
+    const uint4 k = *reinterpret_cast<const uint4*>(chunk_keys[group] + t), at = *reinterpret_cast<const uint4*>(chunk_tokens[group] + t);
+    const unsigned key[kInFlight] = {k.x, k.y, k.z, k.w}, token[kInFlight] = {at.x, at.y, at.z, at.w};
 #pragma unroll
     for (int i = 0; i < kInFlight; ++i) {
       if (key[i] == none) continue;
-      const G* from = grad + (long long)chunk_tokens[group][t + i] * p.grad_stride;
+      const G* from = grad + (long long)token[i] * p.grad_stride;
 #pragma unroll
       for (int j = 0; j < kWords; ++j)
         if (!kApart || j < held) word[i][j] = __ldcs(reinterpret_cast<const Word*>(from + (kApart ? j * lanes : 0)));
     }
+  };
+  auto add = [&](int t, const Word (&word)[kInFlight][kWords]) {
+    const uint4 k = *reinterpret_cast<const uint4*>(chunk_keys[group] + t);
+    const unsigned key[kInFlight] = {k.x, k.y, k.z, k.w};
 #pragma unroll
     for (int i = 0; i < kInFlight; ++i) {
       if (key[i] != row) {
-        if (key[i] == none) break;  // nothing but empty slots from here on, or the end
+        if (key[i] == none) return;  // nothing but empty slots from here on, or the end
         if (head)
           partial(heads);
         else
@@ -499,7 +560,6 @@ __global__ void __launch_bounds__(kSumThreads, 3) sum_kernel(LookupGradParams p,
 #pragma unroll
         for (int j = 0; j < N; ++j) sum[j] = 0.0f;
       }
-      if (row == none) return;  // a chunk of empty slots
       if constexpr (kApart) {
 #pragma unroll
         for (int j = 0; j < N; ++j) sum[j] += to_f32(*reinterpret_cast<const G*>(&word[i][j]));
@@ -509,6 +569,16 @@ __global__ void __launch_bounds__(kSumThreads, 3) sum_kernel(LookupGradParams p,
         for (int j = 0; j < N; ++j) sum[j] += to_f32(v.v[j]);
       }
     }
+  };
+  if (row == none) return;  // a chunk of empty slots
+  // two sets of words in turn: one on its way while the other one is added
+  Word even[kInFlight][kWords], odd[kInFlight][kWords];
+  fetch(0, even);
+  for (int t = 0; t < plan.chunk; t += 2 * kInFlight) {
+    fetch(t + kInFlight, odd);
+    add(t, even);
+    if (t + 2 * kInFlight < plan.chunk) fetch(t + 2 * kInFlight, even);
+    add(t + kInFlight, odd);
   }
   if (head) {
     partial(heads);
@@ -527,7 +597,7 @@ constexpr int kJoinDims = 128;
 constexpr long long kJoinAlone = 48;  // partial sums that a warp adds up by itself
 
 template <class O>
-__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(LookupGradParams p, SumPlan plan, const unsigned* keys,
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(LookupGradParams p, SumPlan plan, const uint2* sorted,
                                                                const float* heads, const float* tails,
                                                                const unsigned* joins, const unsigned* join_list) {
   __shared__ float sums[kJoinWarps][kJoinDims];
@@ -543,12 +613,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(LookupGradParams 
     unsigned row = 0;
     if (item < items) {
       chunk = join_list[item % count];  // (a CTA's warps take different rows: the longest ones are not all its own)
-      row = keys[(chunk + 1) * plan.chunk];
+      row = sorted[(chunk + 1) * plan.chunk].x;
       // the last chunk that begins with the row: 32 candidates at a time, the next ones first
       long long low = chunk + 1, step = 1;
       for (;;) {
         const long long at = low + (lane + 1) * step;
-        const unsigned same = __ballot_sync(FULL, at < plan.chunks && keys[min(at, plan.chunks - 1) * plan.chunk] == row);
+        const unsigned same = __ballot_sync(FULL, at < plan.chunks && sorted[min(at, plan.chunks - 1) * plan.chunk].x == row);
         const int reached = __popc(same);  // they are the first ones
         low += reached * step;
         if (reached == 32) {
@@ -622,8 +692,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(LookupGradParams 
 }
 
 struct GradSpace {
-  unsigned* keys[2];
-  unsigned* tokens[2];
+  uint2* pairs[2];  // (key, token)
   unsigned* counts;
   unsigned* joins;
   unsigned* join_list;
@@ -643,11 +712,8 @@ GradSpace grad_space(long long tokens, long long n, long long d, void* base) {
   const SumPlan sums = sum_plan(tokens, d);
   const SortPlan plan = sort_plan(tokens, n);
   const bool ranked = tokens <= kRankMost;
-  for (int i = 0; i < 2; ++i) {  // sum_kernel reads up to kInFlight - 1 words more
-    s.keys[i] = reinterpret_cast<unsigned*>(take(ranked && i ? 0 : tokens + kInFlight));
-    s.tokens[i] = reinterpret_cast<unsigned*>(take(ranked && i ? 0 : tokens + kInFlight));
-  }
-  s.counts = reinterpret_cast<unsigned*>(take(ranked ? 0 : (long long)plan.parts << plan.digit));
+  for (int i = 0; i < 2; ++i) s.pairs[i] = reinterpret_cast<uint2*>(take(ranked && i ? 0 : 2 * tokens));
+  s.counts = reinterpret_cast<unsigned*>(take(ranked ? 0 : (long long)(plan.parts + 1) << plan.digit));
   s.joins = reinterpret_cast<unsigned*>(take(1));
   s.join_list = reinterpret_cast<unsigned*>(take(sums.chunks));
   s.heads = reinterpret_cast<float*>(take(sums.chunks * d));
@@ -658,14 +724,16 @@ GradSpace grad_space(long long tokens, long long n, long long d, void* base) {
 
 template <class G, class O, int N, bool kApart>
 cudaError_t sum_t(const LookupGradParams& p, const SumPlan& plan, const GradSpace& s, int at, cudaStream_t stream) {
-  int lanes = next_pow2((p.d + N - 1) / N, kSumThreads);
+  // more than a warp: as many warps as it takes, in columns of equal width
+  const long long need = (p.d + N - 1) / N, columns = (need + kSumThreads - 1) / kSumThreads;
+  int lanes = need > 32 ? (int)((need + columns - 1) / columns + 31) / 32 * 32 : next_pow2(need, 32);
   if (lanes < kSumLanes) lanes = kSumLanes;
   const int groups = kSumThreads / lanes;
-  const long long blocks = (plan.chunks + groups - 1) / groups, columns = (p.d + (long long)lanes * N - 1) / ((long long)lanes * N);
+  const long long blocks = (plan.chunks + groups - 1) / groups;
   if (blocks > 0x7fffffffll || columns > 65535) return cudaErrorInvalidValue;
   const dim3 grid((unsigned)blocks, (unsigned)columns);
-  return launch_after(p.tokens > kRankMost, sum_kernel<G, O, N, kApart>, grid, kSumThreads, stream, p, plan, s.keys[at],
-                      s.tokens[at], s.heads, s.tails, s.joins, s.join_list, lanes);
+  return launch_after(p.tokens > kRankMost, sum_kernel<G, O, N, kApart>, grid, lanes * groups, stream, p, plan, s.pairs[at],
+                      s.heads, s.tails, s.joins, s.join_list, lanes);
 }
 
 template <class G, class O>
@@ -690,14 +758,13 @@ cudaError_t grad_t(const LookupGradParams& p, cudaStream_t stream) {
   int at = 0;
   if (p.tokens <= kRankMost) {
     const ZeroPart z = zeros((int)((p.tokens + kRankTokens - 1) / kRankTokens), 0, 1);
-    sort_rank_kernel<<<(unsigned)(z.first + zero_blocks(z)), kRankThreads, 0, stream>>>(p, z, s.keys[0], s.tokens[0], s.joins);
+    sort_rank_kernel<<<(unsigned)(z.first + zero_blocks(z)), kRankThreads, 0, stream>>>(p, z, s.pairs[0], s.joins);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   } else {
     const SortPlan sort = sort_plan(p.tokens, p.n);
     for (int pass = 0; pass < sort.passes; ++pass) {
-      const unsigned* keys = pass ? s.keys[at] : nullptr;
-      const unsigned* tokens = pass ? s.tokens[at] : nullptr;
+      const uint2* pairs = pass ? s.pairs[at] : nullptr;
       const int to = pass ? 1 - at : 0, shift = pass * sort.digit;
       const ZeroPart first = zeros(sort.parts, 2 * pass, 2 * sort.passes), second = zeros(sort.parts, 2 * pass + 1, 2 * sort.passes);
       auto* count = sort.items == 4 ? sort_count_kernel<4> : sort_count_kernel<16>;
@@ -705,10 +772,16 @@ cudaError_t grad_t(const LookupGradParams& p, cudaStream_t stream) {
       unsigned* joins = pass ? nullptr : s.joins;
       const dim3 grid((unsigned)(first.first + zero_blocks(first)));
       // (the first one starts when what came before on the stream is complete)
-      e = launch_after(pass > 0, count, grid, kTileThreads, stream, p, first, sort, keys, shift, s.counts, joins);
+      e = launch_after(pass > 0, count, grid, kTileThreads, stream, p, first, sort, pairs, shift, s.counts, joins);
       if (e != cudaSuccess) return e;
+      if (sort.scanned) {
+        unsigned* totals = s.counts + ((size_t)sort.parts << sort.digit);
+        e = launch_after(true, sort_scan_kernel, dim3(1u << sort.digit), kTileThreads, stream, s.counts, totals, 1 << sort.digit,
+                         sort.parts);
+        if (e != cudaSuccess) return e;
+      }
       e = launch_after(true, place, dim3((unsigned)(second.first + zero_blocks(second))), kTileThreads, stream, p, second,
-                       sort, keys, tokens, shift, s.counts, s.keys[to], s.tokens[to]);
+                       sort, pairs, shift, s.counts, s.pairs[to]);
       if (e != cudaSuccess) return e;
       at = to;
     }
@@ -725,7 +798,7 @@ cudaError_t grad_t(const LookupGradParams& p, cudaStream_t stream) {
   if (e != cudaSuccess || plan.chunks < 2) return e;
   const long long items = plan.chunks * ((p.d + kJoinDims - 1) / kJoinDims), wanted = (items + kJoinWarps - 1) / kJoinWarps;
   return launch_after(p.tokens > kRankMost, join_kernel<O>, dim3((unsigned)(wanted < 6 * kSMs ? wanted : 6 * kSMs)),
-                      kJoinWarps * 32, stream, p, plan, s.keys[at], s.heads, s.tails, s.joins, s.join_list);
+                      kJoinWarps * 32, stream, p, plan, s.pairs[at], s.heads, s.tails, s.joins, s.join_list);
 }
 
 }  // namespace
