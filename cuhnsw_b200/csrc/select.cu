@@ -62,8 +62,8 @@ struct Pool {
 
   __device__ void push(const Key& k) { keys[atomicAdd(count, 1)] = k; }
 
-  // All threads.  Up to a warp's worth are ranked by one warp; more go through a bitonic network over the smallest power of two
-  // that holds them.
+  // All threads.  Up to a warp's worth are ranked by one warp, up to a CTA's against each other; more go through a bitonic
+  // network over the smallest power of two that holds them.
   __device__ void sort() {
     __syncthreads();
     const int held = *count;
@@ -80,7 +80,21 @@ struct Pool {
       __syncthreads();
       return;
     }
-    int size = 64;
+    if (held <= kThreads) {
+      Key mine;
+      clear(mine);
+      int rank = 0;
+      if ((int)threadIdx.x < held) {
+        mine = keys[threadIdx.x];
+#pragma unroll 4
+        for (int i = 0; i < held; ++i) rank += above(keys[i], mine);
+      }
+      __syncthreads();
+      if ((int)threadIdx.x < held) keys[rank] = mine;
+      __syncthreads();
+      return;
+    }
+    int size = 2 * kThreads;
     while (size < held) size <<= 1;
     for (int i = held + threadIdx.x; i < size; i += kThreads) clear(keys[i]);
     for (int span = 2; span <= size; span <<= 1) {
@@ -115,10 +129,10 @@ struct Pool {
 
 // ---- one piece of one row of scores ---------------------------------------------------------------------------------
 
-// Every thread holds kEach scores.  The CTA's `keep` best: a bound that at least `keep` of them reach (groups of threads
-// are at least that many, and the smallest of the groups' largest scores is reached once in each), everything from there on
-// into a pool, the pool in order.  Also the piece's largest score and its sum of exponentials.  Bound: HBM bytes, and the
-// instructions for every score: its part in the maximum, in the sum, and one comparison.
+// Every thread holds kEach scores.  The CTA's `keep` best: of the largest scores of some four times as many groups of threads
+// the `keep`-th is a bound that as many scores reach; the scores of the few threads whose largest one reaches it are looked at again,
+// and what is not below goes into a pool, the pool in order.  Also the piece's largest score and its sum of
+// exponentials.  Bound: HBM bytes; a score costs its part in the maximum and in the sum.
 constexpr int kPoolScores = 2048;
 constexpr int kWarps = kThreads / 32;
 
@@ -128,61 +142,67 @@ __device__ __forceinline__ float exp2_of(float x) {
   return y;
 }
 
-template <class T, int N, int kEach>
-__global__ void __launch_bounds__(kThreads) piece_kernel(SelectParams p, int pieces, ScoreKey* best, float2* norms) {
+template <class T, int kEach>
+__global__ void __launch_bounds__(kThreads) piece_kernel(SelectParams p, int pieces, int piece, ScoreKey* best,
+                                                         float2* norms) {
+  constexpr int N = 16 / sizeof(T);
   __shared__ ScoreKey pool_keys[kPoolScores];
-  __shared__ int pool_count;
-  __shared__ float firsts[kThreads];
+  __shared__ int pool_count, hot_count;
+  __shared__ unsigned least_ord;
+  __shared__ unsigned char hot[kThreads];  // threads whose largest score reaches the bound
+  __shared__ __align__(16) float firsts[kThreads];
   __shared__ float warp_max[kWarps], warp_sum[kWarps];
   const int warp = threadIdx.x >> 5, lane = lane_id();
   const long long row = blockIdx.y + (long long)blockIdx.z * 65535;
   if (row >= p.sequences * p.beams) return;
   const long long seq = row / p.beams, beam = row % p.beams;
-  const T* scores = static_cast<const T*>(p.scores) + seq * p.seq_stride + beam * p.beam_stride;
-  const int vocabulary = (int)p.vocabulary;
-  const unsigned begin = blockIdx.x * (unsigned)(kThreads * kEach);  // (below 2^31, and so is the vocabulary)
-  auto place = [&](int i) { return begin + (unsigned)((i / N * kThreads + threadIdx.x) * N + i % N); };
-  if (threadIdx.x == 0) pool_count = 0;
+  // Pieces begin at 16-byte boundaries, wherever the row does: `skew` places before the row belong to none.
+  const T* of_row = static_cast<const T*>(p.scores) + seq * p.seq_stride + beam * p.beam_stride;
+  const int skew = (int)(reinterpret_cast<uintptr_t>(of_row) % 16 / sizeof(T));
+  const long long begin = (long long)blockIdx.x * piece - skew;  // of the row
+  const T* scores = of_row + begin;
+  const int low = begin < 0 ? (int)-begin : 0, held = (int)min((long long)piece, p.vocabulary - begin);
+  if (threadIdx.x == 0) pool_count = hot_count = 0;
   float x[kEach];
 #pragma unroll
   for (int i = 0; i < kEach; i += N) {
-    const unsigned at = place(i);
-    if (at + N <= (unsigned)vocabulary) {
-      const Vec<T, N> v = load_stream<T, N>(scores + at);
+    const int at = (i / N * kThreads + threadIdx.x) * N;
+    if (at >= low && at + N <= held) {
+      const Vec<T, N> v = load_vec<T, N>(scores + at);
 #pragma unroll
       for (int j = 0; j < N; ++j) x[i + j] = to_f32(v.v[j]);
     } else {
 #pragma unroll
-      for (int j = 0; j < N; ++j) x[i + j] = at + j < (unsigned)vocabulary ? to_f32(scores[at + j]) : -INFINITY;
+      for (int j = 0; j < N; ++j) x[i + j] = at + j >= low && at + j < held ? to_f32(scores[at + j]) : -INFINITY;
     }
   }
-  float top = x[0];
+  float top = -INFINITY;  // (a NaN is no candidate and does not count)
 #pragma unroll
-  for (int i = 1; i < kEach; ++i) top = fmaxf(top, x[i]);
-  // groups of `lanes` threads, at least `keep` of them; their largest scores
-  int lanes = kThreads;
-  while (lanes > 1 && kThreads / lanes < p.keep) lanes >>= 1;
+  for (int i = 0; i < kEach; ++i) top = fmaxf(top, x[i]);
+  // groups of `lanes` neighbouring threads, of those that have scores; their largest ones
+  const int busy = min(kThreads, (held + N - 1) / N);
+  int lanes = 32;
+  while (lanes > 1 && kThreads / lanes < 4 * p.keep) lanes >>= 1;
+  const int groups = max(0, (busy + lanes - 1) / lanes);
   float of_group = top, of_warp = top;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
     of_warp = fmaxf(of_warp, __shfl_xor_sync(FULL, of_warp, off));
     if (off < lanes) of_group = of_warp;
   }
-  firsts[threadIdx.x] = of_group;
+  if ((threadIdx.x & (lanes - 1)) == 0) firsts[threadIdx.x / lanes] = of_group;
   if (lane == 0) warp_max[warp] = of_warp;
+  if (threadIdx.x == 0) least_ord = 0xffffffffu;
   __syncthreads();
-  float most = -FLT_MAX, least = INFINITY;  // (of a row of -inf the exponentials are zeros)
-  if (lanes <= 32) {
-    for (int i = lane * lanes; i < kThreads; i += 32 * lanes) least = fminf(least, firsts[i]);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) least = fminf(least, __shfl_xor_sync(FULL, least, off));
-  } else {
-    for (int w = 0; w < kWarps; w += lanes / 32) {
-      float of_warps = warp_max[w];
-      for (int v = 1; v < lanes / 32; ++v) of_warps = fmaxf(of_warps, warp_max[w + v]);
-      least = fminf(least, of_warps);
-    }
+  // the smallest of those that fewer than `keep` others exceed
+  if ((int)threadIdx.x < groups) {
+    const float mine = firsts[threadIdx.x];
+    int larger = 0;
+#pragma unroll 8
+    for (int i = 0; i < groups; ++i) larger += firsts[i] > mine;
+    if (larger < p.keep) atomicMin(&least_ord, f2ord(mine));
   }
+  float most = -FLT_MAX;  // (of a row of -inf the exponentials are zeros)
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) most = fmaxf(most, warp_max[w]);
   if (p.log_softmax) {
@@ -193,29 +213,22 @@ __global__ void __launch_bounds__(kThreads) piece_kernel(SelectParams p, int pie
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(FULL, sum, off);
     if (lane == 0) warp_sum[warp] = sum;
   }
-  // -inf and NaN are no candidates: neither is at least the lowest number.  (A group without scores has no largest one.)
-  const float bound = fmaxf(least, -FLT_MAX);
-  int passing = 0;
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) passing += x[i] >= bound;
+  __syncthreads();
+  // -inf is no candidate: it is less than the lowest number.  (With fewer groups than results there is no bound.)
+  const float bound = groups < p.keep ? -FLT_MAX : fmaxf(ord2f(least_ord), -FLT_MAX);
+  if (top >= bound) hot[atomicAdd(&hot_count, 1)] = (unsigned char)threadIdx.x;
+  __syncthreads();
+  const int slots = hot_count * kEach;
   Pool<ScoreKey> pool{pool_keys, &pool_count, kPoolScores};
-  if (__syncthreads_or(passing > kPoolScores / kThreads) == 0) {
-    if (passing > 0) {
-#pragma unroll
-      for (int i = 0; i < kEach; ++i)
-        if (x[i] >= bound) pool.push(score_key(x[i], place(i)));
-    }
-  } else {
-    // so many that they may not fit: a score of each thread at a time
-    ScoreKey from = 0;
-#pragma unroll 1
-    for (int i = 0; i < kEach; ++i) {
-      pool.make_room(p.keep, from);
-      float xi = x[0];
-#pragma unroll
-      for (int j = 1; j < kEach; ++j) xi = j == i ? x[j] : xi;
-      const ScoreKey k = score_key(xi, place(i));
-      if (xi >= bound && k >= from) pool.push(k);
+  ScoreKey from = 0;
+  for (int slot = threadIdx.x; slot - (int)threadIdx.x < slots; slot += kThreads) {
+    if (slots > kPoolScores) pool.make_room(p.keep, from);
+    if (slot >= slots) continue;
+    const int i = slot % kEach, at = (i / N * kThreads + hot[slot / kEach]) * N + i % N;
+    const float xi = at >= low && at < held ? to_f32(scores[at]) : -INFINITY;
+    if (xi >= bound) {
+      const ScoreKey k = score_key(xi, (unsigned)(begin + at));
+      if (k >= from) pool.push(k);
     }
   }
   pool.sort();
@@ -226,8 +239,8 @@ __global__ void __launch_bounds__(kThreads) piece_kernel(SelectParams p, int pie
     norms[row * pieces + blockIdx.x] = make_float2(most, all);
   }
   ScoreKey* to = best + (row * pieces + blockIdx.x) * p.keep;
-  const int held = min(pool_count, p.keep);
-  for (int i = threadIdx.x; i < p.keep; i += kThreads) to[i] = i < held ? pool_keys[i] : 0;
+  const int kept = min(pool_count, p.keep);
+  for (int i = threadIdx.x; i < p.keep; i += kThreads) to[i] = i < kept ? pool_keys[i] : 0;
 }
 
 // ---- a sequence -----------------------------------------------------------------------------------------------------
@@ -242,6 +255,7 @@ __global__ void __launch_bounds__(kThreads) sequence_kernel(SelectParams p, int 
   TotalKey* pool_keys = reinterpret_cast<TotalKey*>(smem);
   double* offsets = reinterpret_cast<double*>(pool_keys + kPoolTotals);  // what a beam's scores are raised by
   __shared__ int pool_count;
+  __shared__ unsigned long long least_total;
   const int lane = lane_id(), warp = threadIdx.x >> 5;
   const long long seq = blockIdx.x;
   const int beams = (int)p.beams;
@@ -277,35 +291,48 @@ __global__ void __launch_bounds__(kThreads) sequence_kernel(SelectParams p, int 
   };
   Pool<TotalKey> pool{pool_keys, &pool_count, kPoolTotals};
   TotalKey least = {0, 0, 0};
-  if (lists >= p.keep && total > kThreads) {
-    // the best first total of each thread's lists, the `keep`-th of them all
-    TotalKey top = total_key(threadIdx.x, first);
-    for (long long list = threadIdx.x + kThreads; list < lists; list += kThreads) {
-      const TotalKey key = total_key(list, mine[list * p.keep]);
-      if (above(key, top)) top = key;
+  if (total > kThreads) {
+    // every thread one of the lists' first totals (the best of several lists', of more lists than threads), the `keep`-th of
+    // them all: as many candidates reach it
+    const long long heads = min((long long)kThreads, total);
+    unsigned long long* totals = reinterpret_cast<unsigned long long*>(pool_keys);
+    unsigned long long top = 0;
+    if (lists >= kThreads) {
+      for (long long list = threadIdx.x; list < lists; list += kThreads)
+        top = max(top, total_key(list, list < kThreads ? first : mine[list * p.keep]).total);
+    } else {
+      const unsigned list = threadIdx.x % (unsigned)lists, rank = threadIdx.x / (unsigned)lists;
+      if (rank < p.keep) top = total_key(list, rank == 0 ? first : mine[(long long)list * p.keep + rank]).total;
     }
-    pool_keys[threadIdx.x] = top;
+    totals[threadIdx.x] = top;
+    if (threadIdx.x == 0) least_total = ~0ull;
     __syncthreads();
-    const int held = (int)min((long long)kThreads, lists);
-    int rank = 0;
-    if (!none(top))
-      for (int i = 0; i < held; ++i) rank += above(pool_keys[i], top);
+    int larger = 0;
+#pragma unroll 8
+    for (int i = 0; i < kThreads; ++i) larger += totals[i] > top;
+    if (larger < p.keep) atomicMin(&least_total, top);
     __syncthreads();
-    if (!none(top) && rank == p.keep - 1) pool_keys[0] = top;
-    const bool there = __syncthreads_or(!none(top) && rank == p.keep - 1);
-    if (there) least = pool_keys[0];
+    // (places of the largest order: all of this total are above it)
+    if (heads >= p.keep) least = {least_total, 0xffffffffu, 0xffffffffu};
     __syncthreads();
   }
-  // list by list of the same rank: the best ones first
+  // All lists' totals of a rank after those of the one before, until none of a whole rank reaches the bound: the lists are in
+  // order.
+  const bool narrow = total < (1ll << 32);
+  auto candidate = [&](long long i) { return i < total ? mine[(narrow ? (unsigned)i % (unsigned)lists : i % lists) * p.keep +
+                                                              (narrow ? (unsigned)i / (unsigned)lists : i / lists)] : 0; };
+  ScoreKey next = candidate(threadIdx.x);
+  long long below = 0;
   for (long long begin = 0; begin < total; begin += kThreads) {
-    pool.make_room(p.keep, least);
+    if (begin > 0) pool.make_room(p.keep, least);
     const long long i = begin + threadIdx.x;
-    if (i < total) {
-      const unsigned long long list = total < (1ll << 32) ? (unsigned)i % (unsigned)lists : i % lists;
-      const unsigned long long rank = total < (1ll << 32) ? (unsigned)i / (unsigned)lists : i / lists;
-      const TotalKey key = total_key(list, mine[list * p.keep + rank]);
-      if (!none(key) && !above(least, key)) pool.push(key);
-    }
+    const ScoreKey k = next;
+    next = candidate(i + kThreads);
+    const TotalKey key = total_key(narrow ? (unsigned)i % (unsigned)lists : i % lists, k);
+    const bool reaches = !none(key) && !above(least, key);
+    if (reaches) pool.push(key);
+    below = __syncthreads_or(reaches) ? 0 : below + kThreads;
+    if (below >= lists) break;
   }
   pool.sort();
   const int found = min(pool_count, p.keep);
@@ -320,39 +347,32 @@ __global__ void __launch_bounds__(kThreads) sequence_kernel(SelectParams p, int 
 }
 
 struct SelectPlan {
-  int each;
+  int each;           // scores per thread at most
+  int piece;          // scores: whole words
   long long pieces;
 };
 SelectPlan select_plan(long long rows, long long vocabulary) {
   SelectPlan s;
-  // pieces of 8192 scores where that still gives every SM four of them
+  // pieces of up to 8192 scores where that still gives every SM four of them, all of about the same length
   s.each = 32;
   while (s.each > 8 && rows * ((vocabulary + kThreads * s.each - 1) / (kThreads * s.each)) < 4 * kSMs) s.each /= 2;
-  s.pieces = (vocabulary + kThreads * s.each - 1) / (kThreads * s.each);
+  const long long places = vocabulary + 7;  // and those before the row
+  s.pieces = (places + kThreads * s.each - 1) / (kThreads * s.each);
+  s.piece = (int)(((places + s.pieces - 1) / s.pieces + 7) / 8 * 8);
   return s;
 }
 
-template <class T, int N>
+template <class T>
 cudaError_t pieces_t(const SelectParams& p, const SelectPlan& plan, ScoreKey* best, float2* norms, cudaStream_t stream) {
   const long long rows = p.sequences * p.beams;
   const dim3 grid((unsigned)plan.pieces, (unsigned)(rows < 65535 ? rows : 65535), (unsigned)((rows + 65534) / 65535));
   if (plan.each == 32)
-    piece_kernel<T, N, 32><<<grid, kThreads, 0, stream>>>(p, (int)plan.pieces, best, norms);
+    piece_kernel<T, 32><<<grid, kThreads, 0, stream>>>(p, (int)plan.pieces, plan.piece, best, norms);
   else if (plan.each == 16)
-    piece_kernel<T, N, 16><<<grid, kThreads, 0, stream>>>(p, (int)plan.pieces, best, norms);
+    piece_kernel<T, 16><<<grid, kThreads, 0, stream>>>(p, (int)plan.pieces, plan.piece, best, norms);
   else
-    piece_kernel<T, N, 8><<<grid, kThreads, 0, stream>>>(p, (int)plan.pieces, best, norms);
+    piece_kernel<T, 8><<<grid, kThreads, 0, stream>>>(p, (int)plan.pieces, plan.piece, best, norms);
   return cudaGetLastError();
-}
-
-template <class T>
-cudaError_t pieces_words(const SelectParams& p, const SelectPlan& plan, ScoreKey* best, float2* norms,
-                         cudaStream_t stream) {
-  const int w = word_bytes(reinterpret_cast<uintptr_t>(p.scores) | (unsigned long long)(p.seq_stride * sizeof(T)) |
-                           (unsigned long long)(p.beam_stride * sizeof(T)));
-  if (w == 16) return pieces_t<T, 16 / sizeof(T)>(p, plan, best, norms, stream);
-  if (w >= 4) return pieces_t<T, 4 / sizeof(T)>(p, plan, best, norms, stream);
-  return pieces_t<T, 1>(p, plan, best, norms, stream);
 }
 
 // ---- states ---------------------------------------------------------------------------------------------------------
@@ -423,9 +443,9 @@ cudaError_t launch_select(const SelectParams& p, cudaStream_t stream) {
     return cudaErrorInvalidValue;
   ScoreKey* best = static_cast<ScoreKey*>(p.workspace);
   float2* norms = reinterpret_cast<float2*>(static_cast<char*>(p.workspace) + best_bytes(rows, plan.pieces, p.keep));
-  cudaError_t e = p.type == kF32   ? pieces_words<float>(p, plan, best, norms, stream)
-                  : p.type == kF16 ? pieces_words<__half>(p, plan, best, norms, stream)
-                                   : pieces_words<__nv_bfloat16>(p, plan, best, norms, stream);
+  cudaError_t e = p.type == kF32   ? pieces_t<float>(p, plan, best, norms, stream)
+                  : p.type == kF16 ? pieces_t<__half>(p, plan, best, norms, stream)
+                                   : pieces_t<__nv_bfloat16>(p, plan, best, norms, stream);
   if (e != cudaSuccess) return e;
   e = allow_smem<sequence_kernel>();
   if (e != cudaSuccess) return e;
