@@ -28,8 +28,7 @@ __device__ __forceinline__ unsigned key_place(ScoreKey k) { return ~(unsigned)k;
 // The same over a sequence: totals differ by less than fp32 resolves where two beams meet, so they are compared in 64 bits.
 struct TotalKey {
   unsigned long long total;  // order-preserving image of the double; 0: no candidate
-  unsigned place;
-  unsigned beam;
+  unsigned long long place;  // beam << 32 | place: the smaller one first
 };
 __device__ __forceinline__ unsigned long long d2ord(double x) {
   const long long u = __double_as_longlong(x + 0.0);
@@ -40,17 +39,15 @@ __device__ __forceinline__ double ord2d(unsigned long long o) {
 }
 __device__ __forceinline__ bool above(ScoreKey a, ScoreKey b) { return a > b; }
 __device__ __forceinline__ bool above(const TotalKey& a, const TotalKey& b) {
-  if (a.total != b.total) return a.total > b.total;
-  if (a.beam != b.beam) return a.beam < b.beam;
-  return a.place < b.place;
+  return a.total > b.total || (a.total == b.total && a.place < b.place);
 }
 __device__ __forceinline__ bool none(const TotalKey& k) { return k.total == 0; }
 __device__ __forceinline__ void clear(ScoreKey& k) { k = 0; }
-__device__ __forceinline__ void clear(TotalKey& k) { k = {0, 0, 0}; }
+__device__ __forceinline__ void clear(TotalKey& k) { k = {0, 0}; }
 
 __device__ __forceinline__ ScoreKey from_lane(ScoreKey k, int lane) { return shfl64(k, lane); }
 __device__ __forceinline__ TotalKey from_lane(const TotalKey& k, int lane) {
-  return {shfl64(k.total, lane), __shfl_sync(FULL, k.place, lane), __shfl_sync(FULL, k.beam, lane)};
+  return {shfl64(k.total, lane), shfl64(k.place, lane)};
 }
 
 // Candidates of a CTA in shared memory, in any order; `sort` puts them in descending order.
@@ -114,12 +111,13 @@ struct Pool {
     __syncthreads();
   }
 
-  // Makes room for kThreads more if there is none: the `keep` best stay, and `least` becomes the last of them.
-  __device__ void make_room(int keep, Key& least) {
+  // Makes room for kThreads more if there are over `most` (at most capacity - kThreads): the `keep` best stay, and `least`
+  // becomes the last of them.
+  __device__ void make_room(int keep, int most, Key& least) {
     __syncthreads();
     const int held = *count;
     __syncthreads();  // nobody pushes before all have read the same count
-    if (held + kThreads <= capacity) return;
+    if (held <= most) return;
     sort();
     if (threadIdx.x == 0) *count = min(*count, keep);
     __syncthreads();
@@ -129,11 +127,11 @@ struct Pool {
 
 // ---- one piece of one row of scores ---------------------------------------------------------------------------------
 
-// Every thread holds kEach scores.  The CTA's `keep` best: of the largest scores of some four times as many groups of threads
+// Every thread holds kEach scores.  The CTA's `keep` best: of the largest scores of twice as many groups of threads
 // the `keep`-th is a bound that as many scores reach; the scores of the few threads whose largest one reaches it are looked at again,
 // and what is not below goes into a pool, the pool in order.  Also the piece's largest score and its sum of
 // exponentials.  Bound: HBM bytes; a score costs its part in the maximum and in the sum.
-constexpr int kPoolScores = 2048;
+constexpr int kPoolScores = 4096;
 constexpr int kWarps = kThreads / 32;
 
 __device__ __forceinline__ float exp2_of(float x) {
@@ -182,7 +180,7 @@ __global__ void __launch_bounds__(kThreads) piece_kernel(SelectParams p, int pie
   // groups of `lanes` neighbouring threads, of those that have scores; their largest ones
   const int busy = min(kThreads, (held + N - 1) / N);
   int lanes = 32;
-  while (lanes > 1 && kThreads / lanes < 4 * p.keep) lanes >>= 1;
+  while (lanes > 1 && kThreads / lanes < 2 * p.keep) lanes >>= 1;
   const int groups = max(0, (busy + lanes - 1) / lanes);
   float of_group = top, of_warp = top;
 #pragma unroll
@@ -222,7 +220,7 @@ __global__ void __launch_bounds__(kThreads) piece_kernel(SelectParams p, int pie
   Pool<ScoreKey> pool{pool_keys, &pool_count, kPoolScores};
   ScoreKey from = 0;
   for (int slot = threadIdx.x; slot - (int)threadIdx.x < slots; slot += kThreads) {
-    if (slots > kPoolScores) pool.make_room(p.keep, from);
+    if (slots > kPoolScores) pool.make_room(p.keep, kPoolScores - kThreads, from);
     if (slot >= slots) continue;
     const int i = slot % kEach, at = (i / N * kThreads + hot[slot / kEach]) * N + i % N;
     const float xi = at >= low && at < held ? to_f32(scores[at]) : -INFINITY;
@@ -282,15 +280,15 @@ __global__ void __launch_bounds__(kThreads) sequence_kernel(SelectParams p, int 
   }
   __syncthreads();
   auto total_key = [&](long long list, ScoreKey k) {
-    TotalKey key = {0, 0, 0};
+    TotalKey key = {0, 0};
     if (k == 0) return key;
     const unsigned beam = (unsigned)list / (unsigned)pieces;
     const double value = offsets[beam] + (double)key_score(k);
-    if (value > -INFINITY) key = {d2ord(value), key_place(k), beam};
+    if (value > -INFINITY) key = {d2ord(value), (unsigned long long)beam << 32 | key_place(k)};
     return key;
   };
   Pool<TotalKey> pool{pool_keys, &pool_count, kPoolTotals};
-  TotalKey least = {0, 0, 0};
+  TotalKey least = {0, 0};
   if (total > kThreads) {
     // every thread one of the lists' first totals (the best of several lists', of more lists than threads), the `keep`-th of
     // them all: as many candidates reach it
@@ -313,7 +311,7 @@ __global__ void __launch_bounds__(kThreads) sequence_kernel(SelectParams p, int 
     if (larger < p.keep) atomicMin(&least_total, top);
     __syncthreads();
     // (places of the largest order: all of this total are above it)
-    if (heads >= p.keep) least = {least_total, 0xffffffffu, 0xffffffffu};
+    if (heads >= p.keep) least = {least_total, ~0ull};
     __syncthreads();
   }
   // All lists' totals of a rank after those of the one before, until none of a whole rank reaches the bound: the lists are in
@@ -324,7 +322,7 @@ __global__ void __launch_bounds__(kThreads) sequence_kernel(SelectParams p, int 
   ScoreKey next = candidate(threadIdx.x);
   long long below = 0;
   for (long long begin = 0; begin < total; begin += kThreads) {
-    if (begin > 0) pool.make_room(p.keep, least);
+    if (begin > 0) pool.make_room(p.keep, 2 * p.keep + 32, least);  // (the sooner the bound rises the less there is to sort)
     const long long i = begin + threadIdx.x;
     const ScoreKey k = next;
     next = candidate(i + kThreads);
@@ -340,8 +338,8 @@ __global__ void __launch_bounds__(kThreads) sequence_kernel(SelectParams p, int 
     const TotalKey k = pool_keys[i];
     const long long at = seq * p.keep + i;
     p.out_totals[at] = p.sign * (i < found ? (float)ord2d(k.total) : -INFINITY);
-    if (p.out_beams) p.out_beams[at] = i < found ? (int)k.beam : -1;
-    p.out_ids[at] = i < found ? (int)k.place : -1;
+    if (p.out_beams) p.out_beams[at] = i < found ? (int)(k.place >> 32) : -1;
+    p.out_ids[at] = i < found ? (int)(unsigned)k.place : -1;
   }
   if (p.out_found && threadIdx.x == 0) p.out_found[seq] = found;
 }
