@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from conftest import has_gpu
-from cuhnsw_b200 import cuhnsw_bind, table
+from cuhnsw_b200 import _table, cuhnsw_bind, table
 
 INVALID = -1
 # addresses that are aligned but belong to nobody: a refused call must not touch them
@@ -97,7 +97,6 @@ def test_workspaces_and_states_are_checked():
   assert lib().cuhnsw_reorder_device(state, 1, None, 2, 2, 2, None) == INVALID
   assert lib().cuhnsw_reorder_device(None, 1, A, 2, 2, 2, None) == INVALID
   assert lib().cuhnsw_reorder_device(state, -1, A, 2, 2, 2, None) == INVALID
-  assert ctypes.sizeof(state) == 8 * table._STATE_WORDS
 
 
 def test_torch_layer_refuses_tensors_of_the_host():
@@ -122,7 +121,7 @@ def test_torch_layer_refuses_tensors_of_the_host():
   (lambda: torch.zeros(2, 3, 6, 5)[:, :, ::2, ::2], None),
 ])
 def test_pieces_of_a_state(make, pieces):
-  got = table._pieces(make())
+  got = _table.pieces(make())
   assert got == pieces or pieces is not None and pieces[0] == 1 and got == (1, 0, pieces[2])
 
 
@@ -130,7 +129,7 @@ def test_pieces_cover_a_state():
   """Reading piece by piece gives the values in the order of the dense output."""
   base = torch.arange(2 * 3 * 4 * 9 * 5).view(2, 3, 4, 9, 5)
   for view in (base, base[:, :, :, 2:7], base[:, :, 1:3], base[:, :, :, :, 3:4], base.transpose(0, 1), base[:, :, :, 4]):
-    segments, between, each = table._pieces(view)
+    segments, between, each = _table.pieces(view)
     flat = base.view(-1)
     for s in range(view.shape[0]):
       for b in range(view.shape[1]):
