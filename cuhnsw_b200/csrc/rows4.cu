@@ -88,6 +88,8 @@ template <class T, int N, int kAt, bool kLong>
 __global__ void __launch_bounds__(kPackThreads) pack_kernel(const T* rows, long long row_stride, long long n, int d,
                                                             int group_shift, int groups, unsigned char* codes,
                                                             __nv_bfloat16* scales, int lanes) {
+  next_launch_may_start();
+  wait_for_launch_before();
   const int lane = threadIdx.x & (lanes - 1);
   const int blocks = (d + kBlock - 1) / kBlock, words = 4 * blocks, span = min(lanes, 1 << group_shift);
   const long long team = (long long)blockIdx.x * (kPackThreads / lanes) + threadIdx.x / lanes;
@@ -128,6 +130,8 @@ __global__ void __launch_bounds__(kPackThreads) pack_kernel(const T* rows, long 
 template <class T, int N>
 __global__ void __launch_bounds__(kPackThreads) pack_wide_kernel(const T* rows, long long row_stride, long long n, int d,
                                                                  int group, unsigned char* codes, __nv_bfloat16* scales) {
+  next_launch_may_start();
+  wait_for_launch_before();
   const int lane = lane_id();
   const long long row = (long long)blockIdx.x * (kPackThreads / 32) + (threadIdx.x >> 5);
   if (row >= n) return;
@@ -157,6 +161,8 @@ template <class T, int V>
 __global__ void __launch_bounds__(kPackThreads) unpack_kernel(const unsigned char* codes, const __nv_bfloat16* scales,
                                                               long long n, int d, int group, int group_shift, T* out,
                                                               int lanes, int each) {
+  next_launch_may_start();
+  wait_for_launch_before();
   const int lane = threadIdx.x & (lanes - 1);
   const long long first = ((long long)blockIdx.x * (kPackThreads / lanes) + threadIdx.x / lanes) * each;
   const int rows = (int)min((long long)each, n - first);
@@ -195,8 +201,8 @@ cudaError_t pack_n(const T* rows, long long row_stride, long long n, int d, long
   if (group / 8 > lanes && words > lanes) {
     const long long blocks = (n + kPackThreads / 32 - 1) / (kPackThreads / 32);
     if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
-    pack_wide_kernel<T, N><<<(unsigned)blocks, kPackThreads, 0, stream>>>(rows, row_stride, n, d, (int)group, c, s);
-    return cudaGetLastError();
+    return launch_early(pack_wide_kernel<T, N>, dim3((unsigned)blocks), kPackThreads, 0, stream, rows, row_stride, n, d,
+                        (int)group, c, s);
   }
   // a group that is longer than the row is as good as one of all its words
   const int group_words = group / 8 > lanes ? lanes : (int)(group / 8);
@@ -206,13 +212,8 @@ cudaError_t pack_n(const T* rows, long long row_stride, long long n, int d, long
   const bool longer = words > lanes, many = longer || n > (long long)4 * kSMs * teams;
   const long long per = longer || !many ? teams : 4 * teams, blocks = (n + per - 1) / per;
   if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
-  if (longer)
-    pack_kernel<T, N, 4, true><<<(unsigned)blocks, kPackThreads, 0, stream>>>(rows, row_stride, n, d, shift, groups, c, s, lanes);
-  else if (many)
-    pack_kernel<T, N, 4, false><<<(unsigned)blocks, kPackThreads, 0, stream>>>(rows, row_stride, n, d, shift, groups, c, s, lanes);
-  else
-    pack_kernel<T, N, 1, false><<<(unsigned)blocks, kPackThreads, 0, stream>>>(rows, row_stride, n, d, shift, groups, c, s, lanes);
-  return cudaGetLastError();
+  auto* kernel = longer ? pack_kernel<T, N, 4, true> : many ? pack_kernel<T, N, 4, false> : pack_kernel<T, N, 1, false>;
+  return launch_early(kernel, dim3((unsigned)blocks), kPackThreads, 0, stream, rows, row_stride, n, d, shift, groups, c, s, lanes);
 }
 
 template <class T>
@@ -236,9 +237,8 @@ cudaError_t unpack_v(const unsigned char* codes, const __nv_bfloat16* scales, lo
   if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
   int shift = 0;
   while ((1 << shift) < group) ++shift;
-  unpack_kernel<T, V><<<(unsigned)blocks, kPackThreads, 0, stream>>>(
-    codes, scales, n, d, group, (1 << shift) == group ? shift : -1, out, lanes, each);
-  return cudaGetLastError();
+  return launch_early(unpack_kernel<T, V>, dim3((unsigned)blocks), kPackThreads, 0, stream, codes, scales, n, d, group,
+                      (1 << shift) == group ? shift : -1, out, lanes, each);
 }
 
 template <class T>
@@ -465,6 +465,8 @@ __global__ void __launch_bounds__(32 * most_score_warps(kTiles), 1) scores_kerne
   using Pairs = typename Columns::Pairs;
   constexpr int kOutTiles = kTiles / Columns::kParts;
   extern __shared__ __align__(16) unsigned char smem[];
+  next_launch_may_start();
+  wait_for_launch_before();
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = lane_id(), g = lane >> 2, t = lane & 3;
   const int part = warp % l.split, set = warp / l.split, sets = warps / l.split;
   // the tiles of columns of the same rows run side by side: the second one finds the codes in the L2 cache
@@ -758,8 +760,8 @@ cudaError_t scores_t(const Scores4Params& p, int queries, cudaStream_t stream) {
   l.wide_scales = packed_groups(p.d, p.group) % per_four == 0 && reinterpret_cast<uintptr_t>(p.scales) % (2 * per_four) == 0;
   cudaError_t e = allow_smem<scores_kernel<Columns, kTiles, kGroup>>();
   if (e != cudaSuccess) return e;
-  scores_kernel<Columns, kTiles, kGroup><<<(unsigned)(step * l.column_tiles), 32 * warps, smem, stream>>>(p, l);
-  return cudaGetLastError();
+  return launch_early(scores_kernel<Columns, kTiles, kGroup>, dim3((unsigned)(step * l.column_tiles)), 32 * warps, smem, stream,
+                      p, l);
 }
 
 template <class Columns, int kTiles>

@@ -151,6 +151,8 @@ __global__ void __launch_bounds__(kThreads) piece_kernel(SelectParams p, int pie
   __shared__ __align__(16) float firsts[kThreads];
   __shared__ float warp_max[kWarps], warp_sum[kWarps];
   const int warp = threadIdx.x >> 5, lane = lane_id();
+  next_launch_may_start();
+  wait_for_launch_before();
   const long long row = blockIdx.y + (long long)blockIdx.z * 65535;
   if (row >= p.sequences * p.beams) return;
   const long long seq = row / p.beams, beam = row % p.beams;
@@ -259,7 +261,9 @@ __global__ void __launch_bounds__(kThreads) sequence_kernel(SelectParams p, int 
   const int beams = (int)p.beams;
   const long long lists = (long long)beams * pieces, total = lists * p.keep;
   const ScoreKey* mine = best + seq * total;
+  next_launch_may_start();
   if (threadIdx.x == 0) pool_count = 0;
+  wait_for_launch_before();
   const ScoreKey first = (long long)threadIdx.x < lists ? mine[threadIdx.x * p.keep] : 0;  // on its way meanwhile
   for (int b = warp; b < beams; b += kWarps) {
     double offset = p.totals ? (double)p.totals[seq * beams + b] : 0.0;
@@ -365,12 +369,10 @@ cudaError_t pieces_t(const SelectParams& p, const SelectPlan& plan, ScoreKey* be
   const long long rows = p.sequences * p.beams;
   const dim3 grid((unsigned)plan.pieces, (unsigned)(rows < 65535 ? rows : 65535), (unsigned)((rows + 65534) / 65535));
   if (plan.each == 32)
-    piece_kernel<T, 32><<<grid, kThreads, 0, stream>>>(p, (int)plan.pieces, plan.piece, best, norms);
-  else if (plan.each == 16)
-    piece_kernel<T, 16><<<grid, kThreads, 0, stream>>>(p, (int)plan.pieces, plan.piece, best, norms);
-  else
-    piece_kernel<T, 8><<<grid, kThreads, 0, stream>>>(p, (int)plan.pieces, plan.piece, best, norms);
-  return cudaGetLastError();
+    return launch_early(piece_kernel<T, 32>, grid, kThreads, 0, stream, p, (int)plan.pieces, plan.piece, best, norms);
+  if (plan.each == 16)
+    return launch_early(piece_kernel<T, 16>, grid, kThreads, 0, stream, p, (int)plan.pieces, plan.piece, best, norms);
+  return launch_early(piece_kernel<T, 8>, grid, kThreads, 0, stream, p, (int)plan.pieces, plan.piece, best, norms);
 }
 
 // ---- states ---------------------------------------------------------------------------------------------------------
@@ -401,6 +403,8 @@ __device__ __forceinline__ void copy_row(const ReorderState& s, const char* from
 
 // Grid: pieces of a row x rows x states
 __global__ void __launch_bounds__(kThreads) reorder_kernel(const __grid_constant__ ReorderParams p) {
+  next_launch_may_start();
+  wait_for_launch_before();
   const ReorderState& s = p.state[blockIdx.z];
   const long long rows = p.sequences * p.keep;
   for (long long row = blockIdx.y; row < rows; row += gridDim.y) {
@@ -447,8 +451,7 @@ cudaError_t launch_select(const SelectParams& p, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   e = allow_smem<sequence_kernel>();
   if (e != cudaSuccess) return e;
-  sequence_kernel<<<(unsigned)p.sequences, kThreads, smem, stream>>>(p, (int)plan.pieces, best, norms);
-  return cudaGetLastError();
+  return launch_early(sequence_kernel, dim3((unsigned)p.sequences), kThreads, smem, stream, p, (int)plan.pieces, best, norms);
 }
 
 cudaError_t launch_reorder(const ReorderState* states, int count, const int* beams_of, long long sequences,
@@ -472,9 +475,8 @@ cudaError_t launch_reorder(const ReorderState* states, int count, const int* bea
   p.beams = beams;
   p.keep = keep;
   const long long pieces = (most + 4 * kThreads - 1) / (4 * kThreads);
-  reorder_kernel<<<dim3((unsigned)(pieces < 4096 ? pieces : 4096), (unsigned)(rows < 65535 ? rows : 65535), (unsigned)count),
-                   kThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  const dim3 grid((unsigned)(pieces < 4096 ? pieces : 4096), (unsigned)(rows < 65535 ? rows : 65535), (unsigned)count);
+  return launch_early(reorder_kernel, grid, kThreads, 0, stream, p);
 }
 
 }  // namespace hnsw

@@ -23,6 +23,8 @@ constexpr int kLookupThreads = 256;
 template <class T, int N, int kRows, int kAt>
 __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(LookupParams p, int lanes) {
   const int group = threadIdx.x / lanes, lane = threadIdx.x % lanes, groups = kLookupThreads / lanes;
+  next_launch_may_start();
+  wait_for_launch_before();
   const long long first = ((long long)blockIdx.x * groups + group) * kRows;
   if (first >= p.tokens) return;
   const T* rows = static_cast<const T*>(p.rows);
@@ -78,10 +80,8 @@ cudaError_t lookup_t(const LookupParams& p, cudaStream_t stream) {
   const long long blocks = (p.tokens + per - 1) / per;
   if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
   if (many)
-    lookup_kernel<T, N, 4, kAt><<<(unsigned)blocks, kLookupThreads, 0, stream>>>(p, lanes);
-  else
-    lookup_kernel<T, N, 1, kAt><<<(unsigned)blocks, kLookupThreads, 0, stream>>>(p, lanes);
-  return cudaGetLastError();
+    return launch_early(lookup_kernel<T, N, 4, kAt>, dim3((unsigned)blocks), kLookupThreads, 0, stream, p, lanes);
+  return launch_early(lookup_kernel<T, N, 1, kAt>, dim3((unsigned)blocks), kLookupThreads, 0, stream, p, lanes);
 }
 
 template <class T>
@@ -141,6 +141,8 @@ constexpr int kRankTile = 2048;                                // keys in shared
 
 __global__ void __launch_bounds__(kRankThreads) sort_rank_kernel(LookupGradParams p, ZeroPart zeros, uint2* sorted,
                                                                  unsigned* joins) {
+  next_launch_may_start();
+  wait_for_launch_before();
   if ((int)blockIdx.x >= zeros.first) {
     write_zeros(zeros);
     return;
@@ -235,6 +237,7 @@ __global__ void __launch_bounds__(kTileThreads) sort_count_kernel(LookupGradPara
                                                                   const uint2* pairs, int shift, unsigned* counts,
                                                                   unsigned* joins) {
   next_launch_may_start();
+  wait_for_launch_before();
   if ((int)blockIdx.x >= zeros.first) {
     write_zeros(zeros);
     return;
@@ -243,7 +246,6 @@ __global__ void __launch_bounds__(kTileThreads) sort_count_kernel(LookupGradPara
   const int digits = 1 << plan.digit;
   __shared__ unsigned bins[1 << kMaxDigit];
   for (int i = threadIdx.x; i < digits; i += kTileThreads) bins[i] = 0;
-  if (pairs) wait_for_launch_before();
   if (joins && blockIdx.x == 0 && threadIdx.x == 0) *joins = 0;
   __syncthreads();
   const long long begin = blockIdx.x * plan.part, end = min(begin + plan.part, p.tokens);
@@ -334,6 +336,7 @@ __global__ void __launch_bounds__(kTileThreads) sort_place_kernel(LookupGradPara
                                                                   uint2* sorted) {
   next_launch_may_start();
   if ((int)blockIdx.x >= zeros.first) {
+    wait_for_launch_before();
     write_zeros(zeros);
     return;
   }
@@ -732,8 +735,8 @@ cudaError_t sum_t(const LookupGradParams& p, const SumPlan& plan, const GradSpac
   const long long blocks = (plan.chunks + groups - 1) / groups;
   if (blocks > 0x7fffffffll || columns > 65535) return cudaErrorInvalidValue;
   const dim3 grid((unsigned)blocks, (unsigned)columns);
-  return launch_after(p.tokens > kRankMost, sum_kernel<G, O, N, kApart>, grid, lanes * groups, stream, p, plan, s.pairs[at],
-                      s.heads, s.tails, s.joins, s.join_list, lanes);
+  return launch_early(sum_kernel<G, O, N, kApart>, grid, lanes * groups, 0, stream, p, plan, s.pairs[at], s.heads,
+                      s.tails, s.joins, s.join_list, lanes);
 }
 
 template <class G, class O>
@@ -758,8 +761,8 @@ cudaError_t grad_t(const LookupGradParams& p, cudaStream_t stream) {
   int at = 0;
   if (p.tokens <= kRankMost) {
     const ZeroPart z = zeros((int)((p.tokens + kRankTokens - 1) / kRankTokens), 0, 1);
-    sort_rank_kernel<<<(unsigned)(z.first + zero_blocks(z)), kRankThreads, 0, stream>>>(p, z, s.pairs[0], s.joins);
-    e = cudaGetLastError();
+    e = launch_early(sort_rank_kernel, dim3((unsigned)(z.first + zero_blocks(z))), kRankThreads, 0, stream, p, z, s.pairs[0],
+                     s.joins);
     if (e != cudaSuccess) return e;
   } else {
     const SortPlan sort = sort_plan(p.tokens, p.n);
@@ -771,17 +774,16 @@ cudaError_t grad_t(const LookupGradParams& p, cudaStream_t stream) {
       auto* place = sort.items == 4 ? sort_place_kernel<4> : sort_place_kernel<16>;
       unsigned* joins = pass ? nullptr : s.joins;
       const dim3 grid((unsigned)(first.first + zero_blocks(first)));
-      // (the first one starts when what came before on the stream is complete)
-      e = launch_after(pass > 0, count, grid, kTileThreads, stream, p, first, sort, pairs, shift, s.counts, joins);
+      e = launch_early(count, grid, kTileThreads, 0, stream, p, first, sort, pairs, shift, s.counts, joins);
       if (e != cudaSuccess) return e;
       if (sort.scanned) {
         unsigned* totals = s.counts + ((size_t)sort.parts << sort.digit);
-        e = launch_after(true, sort_scan_kernel, dim3(1u << sort.digit), kTileThreads, stream, s.counts, totals, 1 << sort.digit,
+        e = launch_early(sort_scan_kernel, dim3(1u << sort.digit), kTileThreads, 0, stream, s.counts, totals, 1 << sort.digit,
                          sort.parts);
         if (e != cudaSuccess) return e;
       }
-      e = launch_after(true, place, dim3((unsigned)(second.first + zero_blocks(second))), kTileThreads, stream, p, second,
-                       sort, pairs, shift, s.counts, s.pairs[to]);
+      e = launch_early(place, dim3((unsigned)(second.first + zero_blocks(second))), kTileThreads, 0, stream, p, second, sort,
+                       pairs, shift, s.counts, s.pairs[to]);
       if (e != cudaSuccess) return e;
       at = to;
     }
@@ -797,8 +799,8 @@ cudaError_t grad_t(const LookupGradParams& p, cudaStream_t stream) {
     e = sum_t<G, O, 4, true>(p, plan, s, at, stream);
   if (e != cudaSuccess || plan.chunks < 2) return e;
   const long long items = plan.chunks * ((p.d + kJoinDims - 1) / kJoinDims), wanted = (items + kJoinWarps - 1) / kJoinWarps;
-  return launch_after(p.tokens > kRankMost, join_kernel<O>, dim3((unsigned)(wanted < 6 * kSMs ? wanted : 6 * kSMs)),
-                      kJoinWarps * 32, stream, p, plan, s.pairs[at], s.heads, s.tails, s.joins, s.join_list);
+  return launch_early(join_kernel<O>, dim3((unsigned)(wanted < 6 * kSMs ? wanted : 6 * kSMs)), kJoinWarps * 32, 0, stream, p,
+                      plan, s.pairs[at], s.heads, s.tails, s.joins, s.join_list);
 }
 
 }  // namespace
