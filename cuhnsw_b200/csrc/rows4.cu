@@ -6,17 +6,11 @@
 // block j, the even ones in nibbles 0..3, the odd ones in nibbles 4..7.  So a lane's 16 bytes of a row are its part of four
 // steps of the matrix instruction over 32 dimensions each, a group of 32 or 64 dimensions ends between two steps, and
 // w & 0x000f000f is a pair of consecutive values in two halves of a register.
-#include "common.cuh"
-#include "table_common.cuh"
+#include "scores4.cuh"
 
 namespace hnsw {
 
 namespace {
-
-constexpr int kBlock = 32;             // dimensions of a block
-constexpr int kFour = 4 * kBlock;      // of four blocks
-
-__device__ __forceinline__ long long packed_groups_device(long long d, long long group) { return (d + group - 1) / group; }
 
 // Byte offset in a row of the word that holds dimensions 8 * index .. 8 * index + 7
 __device__ __forceinline__ int word_offset(int index, int blocks) {
@@ -286,88 +280,6 @@ __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_gro
 template <int Left>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(Left) : "memory"); }
 
-// (bits & mask) | magic in one instruction: that takes one constant, the other one has to be in a register already
-__device__ __forceinline__ unsigned and_or(unsigned bits, unsigned mask, unsigned magic) {
-  unsigned r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(bits), "r"(mask), "r"(magic));
-  return r;
-}
-__device__ __forceinline__ unsigned in_register(unsigned x) {
-  unsigned r;
-  asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(x));
-  return r;
-}
-// c += a * b; `first`: c = a * b
-#define MMA16816(types, c, a, b0, b1, first)                                                                         \
-  if (first)                                                                                                         \
-    asm("mma.sync.aligned.m16n8k16.row.col.f32." types ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};" \
-        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])                                                             \
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));                                  \
-  else                                                                                                               \
-    asm("mma.sync.aligned.m16n8k16.row.col.f32." types ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"  \
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                                                             \
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1))
-
-struct PairsF16 {
-  unsigned magic = in_register(0x64006400u);  // 1024, the last bit of whose mantissa is one
-  unsigned minus_low = in_register(0xe408e408u), sixteenth = in_register(0x2c002c00u), minus_high = in_register(0xd480d480u);
-  // two codes of nibbles `pair` and `pair` + 4 as code - 8
-  template <int Pair>
-  __device__ __forceinline__ unsigned values(unsigned w) const {
-    const unsigned u = Pair >= 2 ? w >> 8 : w;
-    unsigned r;
-    if (Pair % 2 == 0)  // 1024 + code - 1032
-      asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(and_or(u, 0x000f000fu, magic)), "r"(minus_low));
-    else  // (1024 + 16 * code) / 16 - 72
-      asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(and_or(u, 0x00f000f0u, magic)), "r"(sixteenth), "r"(minus_high));
-    return r;
-  }
-  static __device__ __forceinline__ void mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1, bool first) {
-    MMA16816("f16.f16", c, a, b0, b1, first);
-  }
-};
-struct PairsBF16 {
-  unsigned magic = in_register(0x43004300u);  // 128
-  unsigned minus = in_register(0xc308c308u), one = in_register(0x3f803f80u);
-  template <int Pair>
-  __device__ __forceinline__ unsigned values(unsigned w) const {
-    unsigned r;  // 128 + code - 136
-    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(and_or(w >> (4 * Pair), 0x000f000fu, magic)), "r"(one), "r"(minus));
-    return r;
-  }
-  static __device__ __forceinline__ void mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1, bool first) {
-    MMA16816("bf16.bf16", c, a, b0, b1, first);
-  }
-};
-
-// How the values of a query type become columns
-struct ColumnsF16 {
-  using In = __half;
-  using Pairs = PairsF16;
-  static constexpr int kParts = 1;
-  static __device__ __forceinline__ unsigned short part(__half x, int) { return __half_as_ushort(x); }
-};
-struct ColumnsBF16 {
-  using In = __nv_bfloat16;
-  using Pairs = PairsBF16;
-  static constexpr int kParts = 1;
-  static __device__ __forceinline__ unsigned short part(__nv_bfloat16 x, int) { return __bfloat16_as_ushort(x); }
-};
-struct ColumnsF32 {
-  using In = float;
-  using Pairs = PairsBF16;
-  static constexpr int kParts = 3;
-  // x = high + middle + low but for 2^-24 of it: each part is what the ones before leave, rounded to 8 bits
-  static __device__ __forceinline__ unsigned short part(float x, int which) {
-    const __nv_bfloat16 high = __float2bfloat16_rn(x);
-    if (which == 0) return __bfloat16_as_ushort(high);
-    // (an infinity or NaN is all in the first part: its remainder would be a NaN)
-    const float rest = isfinite(__bfloat162float(high)) ? x - __bfloat162float(high) : 0.0f;
-    const __nv_bfloat16 middle = __float2bfloat16_rn(rest);
-    return __bfloat16_as_ushort(which == 1 ? middle : __float2bfloat16_rn(rest - __bfloat162float(middle)));
-  }
-};
-
 struct ScoreLayout {
   int queries;       // of a tile of columns: at most 8 * kTiles / parts
   int pitch;         // values per column of a buffer of queries in shared memory
@@ -423,39 +335,6 @@ __device__ __forceinline__ void stage_queries(const Scores4Params& p, const Scor
       for (int i = threadIdx.x; i < eights; i += blockDim.x) eight(queries + q * p.query_stride, xs + q * l.pitch, i);
   }
 }
-
-__device__ __forceinline__ float bf16_low(unsigned pair) { return __uint_as_float(pair << 16); }
-__device__ __forceinline__ float bf16_high(unsigned pair) { return __uint_as_float(pair & 0xffff0000u); }
-
-// The scales of a row for four blocks: bfloat16, one to four of them.  `at`: the first one; left: how many there are from there on.
-template <int kGroup>
-struct FourScales {
-  unsigned low = 0, high = 0;
-  __device__ __forceinline__ void load(const unsigned short* at, int left, bool wide) {
-    if constexpr (kGroup == 4) {
-      low = *at;
-    } else if constexpr (kGroup == 2) {
-      low = wide ? *reinterpret_cast<const unsigned*>(at) : at[0] | (left > 1 ? (unsigned)at[1] << 16 : 0);
-    } else if (wide) {
-      const uint2 both = *reinterpret_cast<const uint2*>(at);
-      low = both.x;
-      high = both.y;
-    } else {
-      low = at[0] | (left > 1 ? (unsigned)at[1] << 16 : 0);
-      high = (left > 2 ? at[2] : 0) | (left > 3 ? (unsigned)at[3] << 16 : 0);
-    }
-  }
-  __device__ __forceinline__ FourScales of_lane(int lane) const {
-    FourScales r;
-    r.low = __shfl_sync(FULL, low, lane);
-    if (kGroup == 1) r.high = __shfl_sync(FULL, high, lane);
-    return r;
-  }
-  __device__ __forceinline__ float get(int j) const {
-    const unsigned pair = j < 2 ? low : high;
-    return j % 2 == 0 ? bf16_low(pair) : bf16_high(pair);
-  }
-};
 
 // kGroup: blocks of 32 dimensions per scale, 4 for four and more.  The parts of an fp32 query are the same column of three
 // operands, so that a lane holds all its sums.
@@ -810,6 +689,7 @@ cudaError_t launch_unpack4(const void* codes, const void* scales, long long n, l
 
 cudaError_t launch_scores4(const Scores4Params& p, cudaStream_t stream) {
   if (p.n <= 0 || p.nq <= 0) return cudaSuccess;
+  if (p.d <= kFour) return launch_scores4_narrow(p, stream);
   if (p.type == kF32) return scores_columns<ColumnsF32>(p, stream);
   if (p.type == kF16) return scores_columns<ColumnsF16>(p, stream);
   return scores_columns<ColumnsBF16>(p, stream);

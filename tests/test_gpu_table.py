@@ -310,6 +310,17 @@ def test_scores_of_many_rows_and_wide_rows():
     check_scores(packed, queries, None, packed.scores(queries))
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n, d, group", [(16_384, 256, 128), (16_500, 257, 32), (20_001, 300, 64), (16_385, 520, 256), (17_000, 1100, 384),
+                                         (40_007, 384, 32), (16_389, 2050, 64), (16_384, 4999, 128)])
+def test_scores_of_many_queries(dtype, n, d, group):
+  packed = random_packed(n + d, n, d, group)
+  for nq in (9, 16, 17, 32, 33, 50):
+    wide = normal(nq, nq, (d + 7) // 8 * 8, dtype=TYPES[dtype])  # rows at 16-byte boundaries
+    bias = normal(5, n) if nq % 2 else None
+    check_scores(packed, wide[:, :d], bias, packed.scores(wide[:, :d], bias))
+
+
 def test_scores_layouts_and_values():
   packed = random_packed(3, 77, 100, 32)
   wide = normal(4, 60, 300)
