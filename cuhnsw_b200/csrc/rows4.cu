@@ -256,16 +256,13 @@ cudaError_t unpack_t(const void* codes, const void* scales, long long n, long lo
 // code becomes a half or bfloat16 value exactly, and so do products and the sums of a group in fp32; the scale is applied to
 // a group's sum in fp32.  An fp32 query is three columns of bfloat16, 8 bits of it each, whose sums are added at the end.
 //
-// Bound: HBM bytes of the codes while the columns are few.  A warp has 32 rows and a share of their dimensions.  It copies its
-// codes asynchronously into a ring of its own in shared memory, two steps of 128 dimensions ahead and across the end of its rows, so
-// that nothing waits for a barrier to keep the copies going; every lane reads back what it copied itself.  A CTA's warps are
-// `split` shares x warps/split sets of 32 rows; all of them read the queries in shared memory.
+// Bound: HBM bytes of the codes while the columns are few, then instructions.  A warp has 32 rows and a share of their dimensions; the
+// codes of its next 128 dimensions, of its next rows behind the last ones, are on their way in registers while it multiplies
+// these.  A CTA's warps are `split` shares x warps/split sets of 32 rows; all of them read the queries in shared memory.
 constexpr int kRowTiles = 2;                  // operands of 16 rows per warp
 constexpr int kWarpRows = 16 * kRowTiles;
 constexpr int kRowsPerLane = 2 * kRowTiles;   // of the first operand: rows g, g + 8, g + 16, ..
 constexpr int kSumPitch = kWarpRows + 1;
-constexpr int kStages = 3;                    // of the ring
-constexpr int kStageBytes = kWarpRows * 64;
 // A CTA's warps where it has an SM for itself: with three and four tiles of columns sums need more registers than 16 warps leave.
 constexpr int most_score_warps(int tiles) { return tiles >= 3 ? 12 : 16; }
 
@@ -352,9 +349,8 @@ __global__ void __launch_bounds__(32 * most_score_warps(kTiles), 1) scores_kerne
   const long long q0 = (long long)(blockIdx.x % l.column_tiles) * l.queries;
   const int nq = (int)min((long long)l.queries, p.nq - q0);
   const int first_unit = blockIdx.x / l.column_tiles, step = gridDim.x / l.column_tiles;
-  // shared memory: the rings, the sums on their way out [warp][8 columns][row], the queries
-  const unsigned ring = (unsigned)__cvta_generic_to_shared(smem) + warp * (kStages * kStageBytes) + 16 * lane;
-  float* sums = reinterpret_cast<float*>(smem + warps * kStages * kStageBytes);
+  // shared memory: the sums on their way out [warp][8 columns][row], the queries
+  float* sums = reinterpret_cast<float*>(smem);
   unsigned short* xs = reinterpret_cast<unsigned short*>(sums + warps * 8 * kSumPitch);
   const int buffer = l.queries * Columns::kParts * l.pitch;  // of the second buffer of queries
   const int blocks = (int)((p.d + kBlock - 1) / kBlock), fours = (blocks + 3) / 4;
@@ -372,37 +368,37 @@ __global__ void __launch_bounds__(32 * most_score_warps(kTiles), 1) scores_kerne
   const int scale_at = (int)min((unsigned)(g + 8 * t), rows - 1) * groups;
   const Pairs pairs;
 
-  // The way through the rows: the fours of this warp's share of every chunk, unit after unit, two ahead of the sums.
+  // The way through the rows: the fours of this warp's share of every chunk, unit after unit, one ahead of the sums.
   const int share = (l.chunk_fours + l.split - 1) / l.split, first_four = part * share;
   int ahead_unit = first_four < min(l.chunk_fours, fours) ? first_unit : units;
   int ahead_four = first_four, ahead_left = min(share, fours - first_four);  // until the share of this chunk ends
-  unsigned ahead_slot = ring;
   const unsigned char* src = nullptr;
   const unsigned short* scale_src = nullptr;
-  FourScales<kGroup> scale, scale_1, scale_2;  // of the next four, of the one after it, ..
+  uint4 next_words[kRowsPerLane];
+  FourScales<kGroup> next_scale;
   auto start_unit = [&] {
     src = static_cast<const unsigned char*>(p.codes) + (long long)first_row(ahead_unit) * row_bytes + 64 * ahead_four;
     scale_src = static_cast<const unsigned short*>(p.scales) + (long long)first_row(ahead_unit) * groups + scale_at;
   };
   if (ahead_unit < units) start_unit();
-  auto copy = [&] {
+  auto load = [&] {
     if (ahead_unit < units) {
       if (4 * ahead_four + 4 <= blocks) {
 #pragma unroll
-        for (int i = 0; i < kRowsPerLane; ++i) copy_async<16>(ahead_slot + 512 * i, src + row_at[i]);
+        for (int i = 0; i < kRowsPerLane; ++i) next_words[i] = __ldcs(reinterpret_cast<const uint4*>(src + row_at[i]));
       } else {
         const int m = blocks - 4 * ahead_four;
         const unsigned char* from = src + 4 * t * m - 16 * t;
+#pragma unroll
         for (int i = 0; i < kRowsPerLane; ++i) {
-          if (m == 2) {
-            copy_async<8>(ahead_slot + 512 * i, from + row_at[i]);
-          } else {
-            for (int j = 0; j < m; ++j) copy_async<4>(ahead_slot + 512 * i + 4 * j, from + row_at[i] + 4 * j);
-          }
+          const unsigned* w = reinterpret_cast<const unsigned*>(from + row_at[i]);
+          next_words[i].x = w[0];
+          if (m > 1) next_words[i].y = w[1];
+          if (m > 2) next_words[i].z = w[2];
         }
       }
       const int at = kGroup < 4 ? ahead_four * (4 / kGroup) : group_fours == 1 ? ahead_four : ahead_four / group_fours;
-      scale_2.load(scale_src + at, groups - at, l.wide_scales);
+      next_scale.load(scale_src + at, groups - at, l.wide_scales);
       ++ahead_four;
       src += 64;
       if (--ahead_left == 0) {
@@ -416,14 +412,8 @@ __global__ void __launch_bounds__(32 * most_score_warps(kTiles), 1) scores_kerne
         ahead_left = min(share, fours - ahead_four);
       }
     }
-    ahead_slot = ahead_slot == ring + (kStages - 1) * kStageBytes ? ring : ahead_slot + kStageBytes;
-    copies_end();
   };
-  static_assert(kStages == 3, "scale, scale_1 and scale_2");
-  copy();
-  scale = scale_2;
-  copy();
-  scale_1 = scale_2;
+  load();
   stage_queries<Columns>(p, l, q0, nq, 0, min(l.chunk_fours, fours), false, xs);
 
   // lanes of columns that there are not read the last one's and throw the result away
@@ -431,15 +421,16 @@ __global__ void __launch_bounds__(32 * most_score_warps(kTiles), 1) scores_kerne
 #pragma unroll
   for (int i = 0; i < kTiles; ++i)
     column[i] = (Columns::kParts == 1 ? min(8 * i + g, nq - 1) : i * nq + min(g, nq - 1)) * l.pitch + 8 * t;
-  unsigned slot = ring;
   int current = 0;  // buffer of the queries
   __syncthreads();
 
   for (int unit = first_unit; unit < units; unit += step) {
-    // the row that this lane writes if its warp has rows for itself; its bias is on the way meanwhile
-    const unsigned mine_row = first_row(unit) + lane;
-    const bool writes = mine_row < rows && mine_row >= (unsigned)(unit * sets + set) * kWarpRows;
-    const float bias = p.bias && writes ? __ldg(p.bias + mine_row) : 0.0f;
+    float bias[kRowsPerLane];  // of a warp that has its rows for itself
+#pragma unroll
+    for (int i = 0; i < kRowsPerLane; ++i) {
+      const unsigned row = first_row(unit) + g + 8 * i;
+      bias[i] = p.bias && l.split == 1 && row < rows ? __ldg(p.bias + row) : 0.0f;
+    }
     float total[kRowTiles][kTiles][4];
 #pragma unroll
     for (int r = 0; r < kRowTiles; ++r)
@@ -453,25 +444,19 @@ __global__ void __launch_bounds__(32 * most_score_warps(kTiles), 1) scores_kerne
       if (l.chunks > 1 && (chunk + 1 < l.chunks || unit + step < units)) {
         const int next = chunk + 1 < l.chunks ? base + l.chunk_fours : 0;
         stage_queries<Columns>(p, l, q0, nq, next, min(l.chunk_fours, fours - next), true, xs + (current ^ 1) * buffer);
+        copies_end();
       }
       const unsigned short* values = xs + current * buffer + first_four * kFour;
 #pragma unroll 1
       for (int four = from; four < to; ++four, values += kFour) {
-        copy();
-        copies_wait<kStages - 1>();
         uint4 w[kRowsPerLane];
-#pragma unroll
-        for (int i = 0; i < kRowsPerLane; ++i)
-          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                       : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w)
-                       : "r"(slot + 512 * i)
-                       : "memory");
-        slot = slot == ring + (kStages - 1) * kStageBytes ? ring : slot + kStageBytes;
         FourScales<kGroup> use[kRowsPerLane];
 #pragma unroll
-        for (int i = 0; i < kRowsPerLane; ++i) use[i] = scale.of_lane((lane & ~3) + i);
-        scale = scale_1;
-        scale_1 = scale_2;
+        for (int i = 0; i < kRowsPerLane; ++i) {
+          w[i] = next_words[i];
+          use[i] = next_scale.of_lane((lane & ~3) + i);
+        }
+        load();
         float sum[kRowTiles][kTiles][4];
         auto block = [&](int j) {
           uint4 b[kTiles];
@@ -524,40 +509,45 @@ __global__ void __launch_bounds__(32 * most_score_warps(kTiles), 1) scores_kerne
         }
       }
       if (l.chunks > 1) {
-        // the next queries were copied with the first of this chunk's codes: three steps later they have arrived
-        if (to - from < kStages) copies_end(), copies_wait<0>();
+        copies_wait<0>();
         __syncthreads();
         current ^= 1;
       }
     }
-    // through shared memory, eight columns at a time: rows next to each other, the shares added up
-    float* mine = sums + warp * 8 * kSumPitch;
+    auto value = [&](int i, int r, int c) {
+      float y = total[r / 2][i * Columns::kParts][2 * (r % 2) + c];
+      if constexpr (Columns::kParts == 3)
+        y += total[r / 2][i * Columns::kParts + 1][2 * (r % 2) + c] + total[r / 2][i * Columns::kParts + 2][2 * (r % 2) + c];
+      return y;
+    };
+    if (l.split == 1) {
+      // eight rows of four queries at a time
+      const unsigned row0 = first_row(unit) + g;
 #pragma unroll
-    for (int i = 0; i < kOutTiles; ++i) {
-      const int some = min(8, nq - 8 * i);
-      if (some <= 0) break;
-#pragma unroll
-      for (int r = 0; r < kRowsPerLane; ++r) {
+      for (int i = 0; i < kOutTiles; ++i) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float y = total[r / 2][i * Columns::kParts][2 * (r % 2) + c];
-          if constexpr (Columns::kParts == 3)
-            y += total[r / 2][i * Columns::kParts + 1][2 * (r % 2) + c] +
-                 total[r / 2][i * Columns::kParts + 2][2 * (r % 2) + c];
-          mine[(2 * t + c) * kSumPitch + g + 8 * r] = y;
+          const int q = 8 * i + 2 * t + c;
+          if (q < nq) {
+            float* out = p.out + (q0 + q) * p.n + row0;
+#pragma unroll
+            for (int r = 0; r < kRowsPerLane; ++r)
+              if (row0 + 8 * r < rows) out[8 * r] = value(i, r, c) + bias[r];
+          }
         }
       }
-      float* out = p.out + (q0 + 8 * i) * p.n;
-      if (l.split == 1) {
-        __syncwarp();
-        if (writes) {
-          float* to_out = out + mine_row;
-          const float* from_sums = mine + lane;
-#pragma unroll 4
-          for (int q = 0; q < some; ++q, to_out += p.n, from_sums += kSumPitch) *to_out = *from_sums + bias;
-        }
-        __syncwarp();
-      } else {
+    } else {
+      // through shared memory, eight queries at a time: rows next to each other, the shares added up
+      float* mine = sums + warp * 8 * kSumPitch;
+#pragma unroll
+      for (int i = 0; i < kOutTiles; ++i) {
+        const int some = min(8, nq - 8 * i);
+        if (some <= 0) break;
+#pragma unroll
+        for (int r = 0; r < kRowsPerLane; ++r)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) mine[(2 * t + c) * kSumPitch + g + 8 * r] = value(i, r, c);
+        float* out = p.out + (q0 + 8 * i) * p.n;
         __syncthreads();
         // a warp takes a set's 32 rows of one column at a time
         for (int k = warp; k < some * sets; k += warps) {
@@ -589,7 +579,7 @@ cudaError_t scores_t(const Scores4Params& p, int queries, cudaStream_t stream) {
   auto space = [&](int warps, int in_chunk) {
     // eight lanes read 16 bytes of two columns and four parts: half a row of banks from column to column
     return (size_t)columns * (in_chunk * kFour + 32) * 2 * (in_chunk < fours ? 2 : 1) +
-           (size_t)warps * (kStages * kStageBytes + 8 * kSumPitch * 4);
+           (size_t)warps * 8 * kSumPitch * 4;
   };
   // two CTAs of eight warps per SM, or one of as many as the queries leave room for; queries that do not fit pass through
   // shared memory in chunks, for all warps of a CTA together
