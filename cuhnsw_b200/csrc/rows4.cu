@@ -391,10 +391,9 @@ __global__ void __launch_bounds__(32 * most_score_warps(kTiles), 1) scores_kerne
         const unsigned char* from = src + 4 * t * m - 16 * t;
 #pragma unroll
         for (int i = 0; i < kRowsPerLane; ++i) {
+          // (whatever the blocks behind the last one hold: their queries are zeros)
           const unsigned* w = reinterpret_cast<const unsigned*>(from + row_at[i]);
-          next_words[i].x = w[0];
-          if (m > 1) next_words[i].y = w[1];
-          if (m > 2) next_words[i].z = w[2];
+          next_words[i] = make_uint4(w[0], m > 1 ? w[1] : 0, m > 2 ? w[2] : 0, 0);
         }
       }
       const int at = kGroup < 4 ? ahead_four * (4 / kGroup) : group_fours == 1 ? ahead_four : ahead_four / group_fours;
@@ -491,21 +490,10 @@ __global__ void __launch_bounds__(32 * most_score_warps(kTiles), 1) scores_kerne
             }
           }
         };
-        if (4 * four + 4 <= blocks) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            block(j);
-            if ((j + 1) % kGroup == 0) add(j);
-          }
-        } else {
-          const int m = blocks - 4 * four;
-#pragma unroll
-          for (int j = 0; j < 3; ++j) {
-            if (j < m) {
-              block(j);
-              if ((j + 1) % kGroup == 0 || j == m - 1) add(j);
-            }
-          }
+        for (int j = 0; j < 4; ++j) {
+          block(j);
+          if ((j + 1) % kGroup == 0) add(j);
         }
       }
       if (l.chunks > 1) {
