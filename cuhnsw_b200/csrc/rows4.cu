@@ -256,15 +256,20 @@ cudaError_t unpack_t(const void* codes, const void* scales, long long n, long lo
 // code becomes a half or bfloat16 value exactly, and so do products and the sums of a group in fp32; the scale is applied to
 // a group's sum in fp32.  An fp32 query is three columns of bfloat16, 8 bits of it each, whose sums are added at the end.
 //
-// Bound: HBM bytes of the codes while the columns are few, then instructions.  A warp has 32 rows and a share of their dimensions; the
-// codes of its next 128 dimensions, of its next rows behind the last ones, are on their way in registers while it multiplies
-// these.  A CTA's warps are `split` shares x warps/split sets of 32 rows; all of them read the queries in shared memory.
-constexpr int kRowTiles = 2;                  // operands of 16 rows per warp
-constexpr int kWarpRows = 16 * kRowTiles;
-constexpr int kRowsPerLane = 2 * kRowTiles;   // of the first operand: rows g, g + 8, g + 16, ..
-constexpr int kSumPitch = kWarpRows + 1;
-// A CTA's warps where it has an SM for itself: with three and four tiles of columns sums need more registers than 16 warps leave.
-constexpr int most_score_warps(int tiles) { return tiles >= 3 ? 12 : 16; }
+// Bound: HBM bytes of the codes while the columns are few, then instructions.  A warp has 32 or 16 rows and a share of their
+// dimensions; the codes of its next 128 dimensions, of its next rows behind the last ones, are on their way in registers while
+// it multiplies these.  A CTA's warps are `split` shares x warps/split sets of rows; all of them read the queries in shared memory.
+constexpr int kMostScoreWarps = 16;  // of a CTA that has an SM for itself
+// A warp takes 32 rows where that leaves 16 warps the registers for its sums, of up to two tiles of columns, and 16 rows else.
+// (131 072 x 4096, 32 queries: 154 us with 16 rows and 16 warps, 156 with 16 and 20, 166 with 32 and 12; 16 queries and 8192
+// dimensions: 60 with 32 rows, 67 with 16.)
+template <int kTiles>
+struct ScoreShape {
+  static constexpr int kRowTiles = kTiles >= 3 ? 1 : 2;  // operands of 16 rows per warp
+  static constexpr int kWarpRows = 16 * kRowTiles;
+  static constexpr int kRowsPerLane = 2 * kRowTiles;     // of the first operand: rows g, g + 8, ..
+  static constexpr int kSumPitch = kWarpRows + 1;
+};
 
 template <int Bytes>
 __device__ __forceinline__ void copy_async(unsigned to, const void* from) {
@@ -282,7 +287,7 @@ struct ScoreLayout {
   int pitch;         // values per column of a buffer of queries in shared memory
   int chunk_fours;   // fours of blocks whose queries are in a buffer: all of them, or there are two buffers in turn
   int chunks;
-  int split;         // warps that share 32 rows, of every chunk
+  int split;         // warps that share the same rows, of every chunk
   int column_tiles;
   int wide_queries;  // 16-byte loads of queries
   int wide_scales;   // loads of all scales of four blocks at once
@@ -336,10 +341,12 @@ __device__ __forceinline__ void stage_queries(const Scores4Params& p, const Scor
 // kGroup: blocks of 32 dimensions per scale, 4 for four and more.  The parts of an fp32 query are the same column of three
 // operands, so that a lane holds all its sums.
 template <class Columns, int kTiles, int kGroup>
-__global__ void __launch_bounds__(32 * most_score_warps(kTiles), 1) scores_kernel(const __grid_constant__ Scores4Params p,
+__global__ void __launch_bounds__(32 * kMostScoreWarps, 1) scores_kernel(const __grid_constant__ Scores4Params p,
                                                                       const __grid_constant__ ScoreLayout l) {
   using Pairs = typename Columns::Pairs;
   constexpr int kOutTiles = kTiles / Columns::kParts;
+  constexpr int kRowTiles = ScoreShape<kTiles>::kRowTiles, kWarpRows = ScoreShape<kTiles>::kWarpRows;
+  constexpr int kRowsPerLane = ScoreShape<kTiles>::kRowsPerLane, kSumPitch = ScoreShape<kTiles>::kSumPitch;
   extern __shared__ __align__(16) unsigned char smem[];
   next_launch_may_start();
   wait_for_launch_before();
@@ -358,14 +365,14 @@ __global__ void __launch_bounds__(32 * most_score_warps(kTiles), 1) scores_kerne
   const int row_bytes = 16 * blocks;
   const unsigned rows = (unsigned)p.n;
   const int units = (int)((p.n + kWarpRows * sets - 1) / (kWarpRows * sets));
-  // a warp's last rows are the table's last 32: some of them are another warp's as well, which writes them
+  // a warp's last rows are the table's last ones: some of them are another warp's as well, which writes them
   const unsigned last_start = max(rows, (unsigned)kWarpRows) - kWarpRows;
   auto first_row = [&](int unit) { return min((unsigned)(unit * sets + set) * kWarpRows, last_start); };
   int row_at[kRowsPerLane];
 #pragma unroll
   for (int i = 0; i < kRowsPerLane; ++i) row_at[i] = (int)min((unsigned)(g + 8 * i), rows - 1) * row_bytes + 16 * t;
   // the lanes of a row load the scales of a row each: t those of row g + 8 * t
-  const int scale_at = (int)min((unsigned)(g + 8 * t), rows - 1) * groups;
+  const int scale_at = (int)min((unsigned)(g + 8 * (t % kRowsPerLane)), rows - 1) * groups;
   const Pairs pairs;
 
   // The way through the rows: the fours of this warp's share of every chunk, unit after unit, one ahead of the sums.
@@ -537,12 +544,12 @@ __global__ void __launch_bounds__(32 * most_score_warps(kTiles), 1) scores_kerne
           for (int c = 0; c < 2; ++c) mine[(2 * t + c) * kSumPitch + g + 8 * r] = value(i, r, c);
         float* out = p.out + (q0 + 8 * i) * p.n;
         __syncthreads();
-        // a warp takes a set's 32 rows of one column at a time
+        // a warp takes a set's rows of one column at a time
         for (int k = warp; k < some * sets; k += warps) {
           const int q = k / sets, s = k % sets;
           const unsigned nominal = (unsigned)(unit * sets + s) * kWarpRows;
           const unsigned row = min(nominal, last_start) + lane;
-          if (row < rows && row >= nominal) {
+          if (lane < kWarpRows && row < rows && row >= nominal) {
             const float* of_set = sums + (s * l.split * 8 + q) * kSumPitch + lane;
             float y = of_set[0];
             for (int other = 1; other < l.split; ++other) y += of_set[other * 8 * kSumPitch];
@@ -558,6 +565,7 @@ __global__ void __launch_bounds__(32 * most_score_warps(kTiles), 1) scores_kerne
 
 template <class Columns, int kTiles, int kGroup>
 cudaError_t scores_t(const Scores4Params& p, int queries, cudaStream_t stream) {
+  constexpr int kWarpRows = ScoreShape<kTiles>::kWarpRows, kSumPitch = ScoreShape<kTiles>::kSumPitch;
   constexpr int kMostSpace = 224 * 1024, kHalfSpace = 112 * 1024;  // shared memory of one CTA per SM, of each of two
   ScoreLayout l;
   l.queries = (int)(p.nq < queries ? p.nq : queries);
@@ -576,14 +584,14 @@ cudaError_t scores_t(const Scores4Params& p, int queries, cudaStream_t stream) {
   l.chunk_fours = fours;
   if (kTiles >= 3 || space(8, fours) > kHalfSpace) {
     per_sm = 1;
-    warps = most_score_warps(kTiles);
+    warps = kMostScoreWarps;
     while (warps > 8 && space(warps, fours) > kMostSpace) warps -= 4;
     if (space(warps, fours) > kMostSpace) {
-      warps = most_score_warps(kTiles);
+      warps = kMostScoreWarps;
       l.chunk_fours = 4;
     }
   }
-  // How many warps share 32 rows, and how many an SM's only CTA has: what takes the CTA with the most units the least time, in
+  // How many warps share the same rows, and how many an SM's only CTA has: what takes the CTA with the most units the least time, in
   // steps of four blocks of all its warps.  The end of a unit takes about two of them, four where sums of several warps are
   // added up; chunks of queries are as many bytes as the codes of `columns` rows, for fewer rows the more warps share them.
   const long long room = ((long long)kSMs * per_sm + l.column_tiles - 1) / l.column_tiles;
