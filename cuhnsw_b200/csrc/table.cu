@@ -596,17 +596,18 @@ __global__ void __launch_bounds__(kSumThreads, kApart || sizeof(G) * N > 8 ? 3 :
 // Rows that cross borders of chunks.  A warp takes one of them and kJoinDims dimensions; of a row with many partial sums the
 // CTA's warps add up a share each.
 constexpr int kJoinWarps = 8;
-constexpr int kJoinDims = 128;
+constexpr int kJoinBlocks = 48 / kJoinWarps * kSMs;
+constexpr int kJoinLoads = 32;       // in flight per lane
 constexpr long long kJoinAlone = 48;  // partial sums that a warp adds up by itself
 
-template <class O>
+template <class O, int kEach>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(LookupGradParams p, SumPlan plan, const uint2* sorted,
                                                                const float* heads, const float* tails,
                                                                const unsigned* joins, const unsigned* join_list) {
+  constexpr int kJoinDims = 32 * kEach;
   __shared__ float sums[kJoinWarps][kJoinDims];
   __shared__ long long first_of[kJoinWarps], parts_of[kJoinWarps];
   __shared__ unsigned row_of[kJoinWarps];
-  constexpr int kEach = kJoinDims / 32;
   const int warp = threadIdx.x >> 5, lane = lane_id();
   wait_for_launch_before();
   const long long count = *joins, items = count * ((p.d + kJoinDims - 1) / kJoinDims);
@@ -645,7 +646,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(LookupGradParams 
         ++from;
       }
       const float* head = heads + (from_chunk + from) * p.d + column * kJoinDims + lane;
-#pragma unroll 8
+#pragma unroll(kJoinLoads / kEach)
       for (long long k = from; k < to; ++k, head += p.d) {
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
@@ -798,9 +799,12 @@ cudaError_t grad_t(const LookupGradParams& p, cudaStream_t stream) {
   else
     e = sum_t<G, O, 4, true>(p, plan, s, at, stream);
   if (e != cudaSuccess || plan.chunks < 2) return e;
-  const long long items = plan.chunks * ((p.d + kJoinDims - 1) / kJoinDims), wanted = (items + kJoinWarps - 1) / kJoinWarps;
-  return launch_early(join_kernel<O>, dim3((unsigned)(wanted < 6 * kSMs ? wanted : 6 * kSMs)), kJoinWarps * 32, 0, stream, p,
-                      plan, s.pairs[at], s.heads, s.tails, s.joins, s.join_list);
+  auto join = [&](auto* kernel, int dims) {
+    const long long items = plan.chunks * ((p.d + dims - 1) / dims), wanted = (items + kJoinWarps - 1) / kJoinWarps;
+    return launch_early(kernel, dim3((unsigned)(wanted < kJoinBlocks ? wanted : kJoinBlocks)), kJoinWarps * 32, 0, stream, p,
+                        plan, s.pairs[at], s.heads, s.tails, s.joins, s.join_list);
+  };
+  return p.d <= 32 ? join(join_kernel<O, 1>, 32) : join(join_kernel<O, 4>, 128);
 }
 
 }  // namespace
