@@ -6,17 +6,18 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
-#include <ATen/ops/from_blob.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <limits>
 #include <sstream>
 #include <stdexcept>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/cuhnsw_b200.h"
@@ -53,9 +54,17 @@ int type_of(const at::Tensor& t) {
 
 bool is_tensor(PyObject* o) { return THPVariable_Check(o); }
 
-const at::Tensor& tensor(PyObject* o, const char* name) {
+// The tensor with its values in memory: a lazily conjugated or negated one (of torch.conj, torch.imag) as a copy.
+at::Tensor unpacked(PyObject* o) {
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_conj() && !t.is_neg()) return t;
+  c10::NoGradGuard no_grad;
+  return t.resolve_conj().resolve_neg();
+}
+
+at::Tensor tensor(PyObject* o, const char* name) {
   if (!is_tensor(o)) refuse(name, " must be a tensor");
-  return THPVariable_Unpack(o);
+  return unpacked(o);
 }
 
 int64_t integer(PyObject* o, const char* name) {
@@ -85,8 +94,8 @@ bool truth(PyObject* o) {
   return value != 0;
 }
 
-const at::Tensor& matrix(PyObject* o, const char* name) {
-  const at::Tensor& t = tensor(o, name);
+at::Tensor matrix(PyObject* o, const char* name) {
+  const at::Tensor t = tensor(o, name);
   if (!t.is_cuda()) refuse(name, " must be a CUDA tensor");
   if (type_of(t) < 0) refuse(name, " must be float32, float16 or bfloat16, not ", t.scalar_type());
   if (t.dim() != 2) refuse(name, " must have two dimensions, not ", t.dim());
@@ -107,11 +116,23 @@ at::Tensor dense(const at::Tensor& t) {
 
 at::Tensor ids_of(PyObject* o, const at::Device& device) {
   if (!is_tensor(o)) refuse("ids must be an int32 or int64 tensor");
-  const at::Tensor& ids = THPVariable_Unpack(o);
+  const at::Tensor ids = unpacked(o);
   if (ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong) refuse("ids must be an int32 or int64 tensor");
   if (ids.device() != device) refuse("ids are on ", ids.device(), ", the rows on ", device);
   if (ids.numel() > kMostIds) refuse(ids.numel(), " ids are too many");
   return dense(ids);
+}
+
+// Whether the memory from a tensor's first value to its last one meets another's.
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  auto range = [](const at::Tensor& t) {
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += t.size(i) > 0 ? (t.size(i) - 1) * t.stride(i) : 0;
+    return std::pair<uintptr_t, uintptr_t>(begin, t.numel() ? begin + (last + 1) * t.element_size() : begin);
+  };
+  const auto x = range(a), y = range(b);
+  return x.first < y.second && y.first < x.second;
 }
 
 at::Tensor make(at::IntArrayRef sizes, at::ScalarType type, const at::Device& device) {
@@ -148,6 +169,12 @@ PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t count, Py_ssize_t
     return kFunction(args);
   } catch (const std::bad_alloc&) {
     PyErr_NoMemory();
+  } catch (const c10::OutOfMemoryError& e) {
+    PyObject* torch = PyImport_ImportModule("torch");
+    PyObject* type = torch ? PyObject_GetAttrString(torch, "OutOfMemoryError") : nullptr;
+    if (type) PyErr_SetString(type, e.what_without_backtrace());
+    Py_XDECREF(type);
+    Py_XDECREF(torch);
   } catch (const c10::Error& e) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
   } catch (const std::exception& e) {
@@ -186,7 +213,7 @@ PyObject* lookup(PyObject* const* args) {  // rows, ids, scale
 }
 
 PyObject* lookup_grad(PyObject* const* args) {  // grad, ids, num_rows, scale, out or None, accumulate
-  const at::Tensor& given = tensor(args[0], "grad");
+  const at::Tensor given = tensor(args[0], "grad");
   if (!given.is_cuda() || type_of(given) < 0) refuse("grad must be a float32, float16 or bfloat16 CUDA tensor");
   const at::Device device = given.device();
   const at::Tensor ids = ids_of(args[1], device);
@@ -213,6 +240,9 @@ PyObject* lookup_grad(PyObject* const* args) {  // grad, ids, num_rows, scale, o
         out.size(0) != rows || out.size(1) != dims || !out.is_contiguous())
       refuse("out must be a dense [", rows, ", ", dims, "] tensor of ", grad.scalar_type(), " or float32 on ", device);
     if (out.requires_grad() && c10::GradMode::is_enabled()) refuse("out must not require a gradient");
+    if (out.is_neg()) refuse("out must not be a negated view");
+    if (overlap(out, grad) || overlap(out, ids)) refuse("out must not overlap grad or the ids");
+    out.unsafeGetTensorImpl()->bump_version();  // whoever keeps it for a backward pass learns that it has changed
   }
   if (out.numel() > 0) {
     const at::Tensor space = workspace(cuhnsw_lookup_grad_workspace(count, rows, dims), "cuhnsw_lookup_grad_workspace", device);
@@ -259,8 +289,8 @@ Packed packed_of(PyObject* const* args) {  // codes, scales, num_dims, group
   if (d < 1) refuse("num_dims must be at least 1");
   const int64_t width = 16 * ((d + 31) / 32), groups = (d + group - 1) / group;
   at::Tensor codes, scales;
-  if (is_tensor(args[0])) codes = THPVariable_Unpack(args[0]);
-  if (is_tensor(args[1])) scales = THPVariable_Unpack(args[1]);
+  if (is_tensor(args[0])) codes = unpacked(args[0]);
+  if (is_tensor(args[1])) scales = unpacked(args[1]);
   if (!codes.defined() || !codes.is_cuda() || codes.scalar_type() != at::kByte || codes.dim() != 2 ||
       codes.size(1) != width || !codes.is_contiguous() || reinterpret_cast<uintptr_t>(codes.const_data_ptr()) % 16 != 0)
     refuse("codes must be a dense, 16-byte aligned uint8 CUDA tensor [num_rows, ", width, "]");
@@ -288,32 +318,45 @@ PyObject* unpack(PyObject* const* args) {  // codes, scales, num_dims, group, dt
   return THPVariable_Wrap(out);
 }
 
-at::Tensor scores_of(const Packed& p, PyObject* queries_given, PyObject* bias_given) {
-  const at::Tensor& given = matrix(queries_given, "queries");
-  if (given.device() != p.device) refuse("queries are on ", given.device(), ", the rows on ", p.device);
-  if (given.size(1) != p.d) refuse("queries have ", given.size(1), " dimensions, the rows have ", p.d);
-  if (given.size(0) > 1 << 18) refuse(given.size(0), " queries are too many");
-  const at::Tensor queries = row_major(given);
+struct Asked {
+  at::Tensor queries, bias;  // no bias: undefined
+};
+
+Asked asked_of(const Packed& p, PyObject* queries_given, PyObject* bias_given) {
+  const at::Tensor queries = matrix(queries_given, "queries");
+  if (queries.device() != p.device) refuse("queries are on ", queries.device(), ", the rows on ", p.device);
+  if (queries.size(1) != p.d) refuse("queries have ", queries.size(1), " dimensions, the rows have ", p.d);
+  if (queries.size(0) > 1 << 18) refuse(queries.size(0), " queries are too many");
   at::Tensor bias;
   if (bias_given != Py_None) {
-    if (is_tensor(bias_given)) bias = THPVariable_Unpack(bias_given);
+    if (is_tensor(bias_given)) bias = unpacked(bias_given);
     if (!bias.defined() || bias.device() != p.device || bias.scalar_type() != at::kFloat || bias.dim() != 1 ||
         bias.size(0) != p.n)
       refuse("bias must be a float32 tensor [", p.n, "] beside the rows");
     bias = dense(bias);
   }
-  const at::Tensor out = make({queries.size(0), p.n}, at::kFloat, p.device);
+  return {row_major(queries), bias};
+}
+
+// Scores of `count` queries from the number `first` on.
+at::Tensor scores_of(const Packed& p, const Asked& asked, int64_t first, int64_t count) {
+  const at::Tensor out = make({count, p.n}, at::kFloat, p.device);
+  const at::Tensor& queries = asked.queries;
   run("cuhnsw_scores4_device", p.device, [&](void* stream) {
     return cuhnsw_scores4_device(p.codes.const_data_ptr(), p.scales.const_data_ptr(), p.n, p.d, p.group,
-                                 queries.const_data_ptr(), queries.stride(0), type_of(queries), queries.size(0),
-                                 bias.defined() ? bias.const_data_ptr<float>() : nullptr, out.mutable_data_ptr<float>(),
-                                 stream);
+                                 static_cast<const char*>(queries.const_data_ptr()) +
+                                   first * queries.stride(0) * (int64_t)queries.element_size(),
+                                 queries.stride(0), type_of(queries), count,
+                                 asked.bias.defined() ? asked.bias.const_data_ptr<float>() : nullptr,
+                                 out.mutable_data_ptr<float>(), stream);
   });
   return out;
 }
 
 PyObject* scores(PyObject* const* args) {  // codes, scales, num_dims, group, queries, bias or None
-  return THPVariable_Wrap(scores_of(packed_of(args), args[4], args[5]));
+  const Packed p = packed_of(args);
+  const Asked asked = asked_of(p, args[4], args[5]);
+  return THPVariable_Wrap(scores_of(p, asked, 0, asked.queries.size(0)));
 }
 
 // -- selection -----------------------------------------------------------------------------------------------------------
@@ -327,8 +370,10 @@ struct Selected {
   at::Tensor totals, beams, ids, found;
 };
 
+// `first`: of the sequences of `out`, the one that the first of these is
 void select(const at::Tensor& scores, int64_t seq_stride, int64_t beam_stride, int64_t sequences, int64_t beams,
-            int64_t vocabulary, const at::Tensor& totals, int64_t keep, bool log_softmax, bool negate, const Selected& out) {
+            int64_t vocabulary, const at::Tensor& totals, int64_t keep, bool log_softmax, bool negate, const Selected& out,
+            int64_t first) {
   const at::Device device = scores.device();
   const at::Tensor space =
     workspace(cuhnsw_select_workspace(sequences, beams, vocabulary, (int32_t)keep), "cuhnsw_select_workspace", device);
@@ -336,17 +381,21 @@ void select(const at::Tensor& scores, int64_t seq_stride, int64_t beam_stride, i
     return cuhnsw_select_device(
       scores.const_data_ptr(), seq_stride, beam_stride, type_of(scores),
       totals.defined() ? totals.const_data_ptr<float>() : nullptr, sequences, beams, vocabulary, (int32_t)keep, log_softmax,
-      negate, out.totals.mutable_data_ptr<float>(), out.beams.defined() ? out.beams.mutable_data_ptr<int32_t>() : nullptr,
-      out.ids.mutable_data_ptr<int32_t>(), out.found.defined() ? out.found.mutable_data_ptr<int32_t>() : nullptr,
-      space.mutable_data_ptr(), stream);
+      negate, out.totals.mutable_data_ptr<float>() + first * keep,
+      out.beams.defined() ? out.beams.mutable_data_ptr<int32_t>() + first * keep : nullptr,
+      out.ids.mutable_data_ptr<int32_t>() + first * keep,
+      out.found.defined() ? out.found.mutable_data_ptr<int32_t>() + first : nullptr, space.mutable_data_ptr(), stream);
   });
 }
+
+constexpr int64_t kSearchScores = 1ll << 30;  // scores of a search in memory at a time: 4 GB
+constexpr int64_t kSearchQueries = 32;        // but so many queries' at least
 
 PyObject* search(PyObject* const* args) {  // codes, scales, num_dims, group, queries, topk, bias or None
   const Packed p = packed_of(args);
   const int64_t topk = keep_of(integer(args[5], "topk"), "topk");
-  const at::Tensor all = scores_of(p, args[4], args[6]);
-  const int64_t count = all.size(0);
+  const Asked asked = asked_of(p, args[4], args[6]);
+  const int64_t count = asked.queries.size(0);
   const Selected out{make({count, topk}, at::kFloat, p.device), {}, make({count, topk}, at::kInt, p.device),
                      make({count}, at::kInt, p.device)};
   if (p.n == 0) {
@@ -354,13 +403,18 @@ PyObject* search(PyObject* const* args) {  // codes, scales, num_dims, group, qu
     out.ids.fill_(-1);
     out.found.zero_();
   } else {
-    select(all, p.n, p.n, count, 1, p.n, {}, topk, false, true, out);
+    const int64_t part = std::max(kSearchQueries, kSearchScores / p.n / kSearchQueries * kSearchQueries);
+    for (int64_t first = 0; first < count; first += part) {
+      const int64_t some = std::min(part, count - first);
+      const at::Tensor all = scores_of(p, asked, first, some);
+      select(all, p.n, p.n, some, 1, p.n, {}, topk, false, true, out, first);
+    }
   }
   return tuple_of({out.ids, out.totals, out.found});
 }
 
 PyObject* select_beams(PyObject* const* args) {  // scores, totals or None, keep or None, log_softmax
-  const at::Tensor& given = tensor(args[0], "scores");
+  const at::Tensor given = tensor(args[0], "scores");
   if (!given.is_cuda() || type_of(given) < 0) refuse("scores must be a float32, float16 or bfloat16 CUDA tensor");
   if (given.dim() != 3) refuse("scores must be [sequences, beams, vocabulary], not ", given.dim(), "-dimensional");
   const at::Device device = given.device();
@@ -370,7 +424,7 @@ PyObject* select_beams(PyObject* const* args) {  // scores, totals or None, keep
   if (beams > 16384) refuse(beams, " beams are too many");
   at::Tensor totals;
   if (args[1] != Py_None) {
-    if (is_tensor(args[1])) totals = THPVariable_Unpack(args[1]);
+    if (is_tensor(args[1])) totals = unpacked(args[1]);
     if (!totals.defined() || totals.device() != device || totals.scalar_type() != at::kFloat || totals.dim() != 2 ||
         totals.size(0) != sequences || totals.size(1) != beams)
       refuse("totals must be a float32 tensor [", sequences, ", ", beams, "] beside the scores");
@@ -384,7 +438,8 @@ PyObject* select_beams(PyObject* const* args) {  // scores, totals or None, keep
     out.beams.fill_(-1);
     out.ids.fill_(-1);
   } else {
-    select(scores, scores.stride(0), scores.stride(1), sequences, beams, vocabulary, totals, keep, log_softmax, false, out);
+    select(scores, scores.stride(0), scores.stride(1), sequences, beams, vocabulary, totals, keep, log_softmax, false, out,
+           0);
   }
   return tuple_of({out.totals, out.beams, out.ids});
 }
@@ -421,7 +476,7 @@ PyObject* reorder(PyObject* const* args) {  // states, beams
   const bool several = PyList_Check(args[0]) || PyTuple_Check(args[0]);
   if (!several && !is_tensor(args[0])) refuse("states must be a tensor or a list of tensors");
   at::Tensor beams;
-  if (is_tensor(args[1])) beams = THPVariable_Unpack(args[1]);
+  if (is_tensor(args[1])) beams = unpacked(args[1]);
   if (!beams.defined() || !beams.is_cuda() || beams.scalar_type() != at::kInt || beams.dim() != 2)
     refuse("beams must be an int32 CUDA tensor [sequences, keep]");
   beams = dense(beams);
@@ -435,9 +490,10 @@ PyObject* reorder(PyObject* const* args) {  // states, beams
   states.reserve(count);
   for (Py_ssize_t i = 0; i < count; ++i) {
     PyObject* o = several ? PySequence_Fast_GET_ITEM(args[0], i) : args[0];
-    if (!is_tensor(o) || THPVariable_Unpack(o).device() != device || THPVariable_Unpack(o).dim() < 2)
+    at::Tensor state;
+    if (is_tensor(o)) state = unpacked(o);
+    if (!state.defined() || state.device() != device || state.dim() < 2)
       refuse("a state must be a tensor [sequences, beams, ...] on ", device);
-    at::Tensor state = THPVariable_Unpack(o);
     const at::Tensor& first = i ? inputs[0] : state;
     if (state.size(0) != sequences || state.size(1) != first.size(1))
       refuse("states of shapes ", sizes_text(first.sizes()), " and ", sizes_text(state.sizes()), " for ", sequences,

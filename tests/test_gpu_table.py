@@ -3,6 +3,10 @@
 Tolerances: a rounding to a type is off by at most finfo(type).eps / 2 of the value; a sum of m products in fp32 by at most
 about m * 2^-24 times the sum of their magnitudes (2^-23 where the matrix instruction adds, which may cut instead of round)."""
 import math
+import subprocess
+import sys
+import threading
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -691,3 +695,129 @@ def test_refusals():
   refused("a state must be", lambda: table.reorder(scores[:, 0, 0], beams))
   refused("states of shapes", lambda: table.reorder([scores, scores[:, :2]], beams))
   refused("states of shapes", lambda: table.reorder(scores[:1], beams))
+
+
+def test_values_that_are_negated_lazily():
+  """torch.conj and .imag of it leave the sign to the next operator."""
+  pair = torch.complex(normal(1, 40, 64), normal(2, 40, 64))
+  rows = torch.conj(pair).imag
+  assert rows.is_neg()
+  plain = -pair.imag.contiguous()
+  ids = ids_of(3, 90, 40, "outside")
+  assert torch.equal(table.lookup(rows, ids), table.lookup(plain, ids))
+  assert torch.equal(table.lookup_grad(rows, ids[:40], 50), table.lookup_grad(plain, ids[:40], 50))
+  packed, want = table.pack_rows(rows, 32), table.pack_rows(plain, 32)
+  assert torch.equal(packed.codes, want.codes) and torch.equal(packed.scales, want.scales)
+  assert torch.equal(packed.scores(rows[:5]), packed.scores(plain[:5]))
+  got, want = table.select_beams(rows[None], rows[None, :, 0], 9), table.select_beams(plain[None], plain[None, :, 0], 9)
+  assert all(torch.equal(x, y) for x, y in zip(got, want))
+  states, beams = torch.conj(pair)[None], torch.tensor([[7, -1, 39]], dtype=torch.int32, device=DEV)
+  out = table.reorder(states, beams)[0]
+  assert torch.equal(out[0], pair[7].conj()) and torch.equal(out[2], pair[39].conj()) and (out[1] == 0).all()
+  with pytest.raises(RuntimeError, match="out must be a dense"):
+    table.lookup_grad(plain, ids[:40], 40, out=rows)
+  with pytest.raises(RuntimeError, match="negated"):
+    table.lookup_grad(plain, ids[:40], 40, out=torch._neg_view(torch.zeros((40, 64), device=DEV)))
+
+
+def test_an_output_that_others_use():
+  grad, ids = normal(1, 30, 16), ids_of(2, 30, 20, "uniform")
+  out, weight = torch.zeros((20, 16), device=DEV), torch.ones((20, 16), device=DEV, requires_grad=True)
+  product = (weight * out).sum()  # keeps `out` for its backward pass
+  table.lookup_grad(grad, ids, 20, out=out, accumulate=True)
+  with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+    product.backward()
+  both = torch.zeros((50, 16), device=DEV)
+  for part in (both[:20], both[10:30], both[29:49]):
+    with pytest.raises(RuntimeError, match="overlap"):
+      table.lookup_grad(both[:30], ids, 20, out=part)
+  assert (both == 0).all()
+  both[:30] = grad
+  assert torch.equal(table.lookup_grad(both[:30], ids, 20, out=both[30:]), table.lookup_grad(grad, ids, 20))
+  own = torch.arange(20, device=DEV).view(torch.float32).view(20, 2)
+  with pytest.raises(RuntimeError, match="overlap"):
+    table.lookup_grad(grad[:20, :2], own.view(torch.int64).view(20), 20, out=own)
+
+
+def test_results_that_memory_does_not_hold():
+  rows = torch.zeros((1, 1 << 24), device=DEV)
+  with pytest.raises(torch.OutOfMemoryError):
+    table.lookup(rows, torch.zeros(1 << 16, dtype=torch.int64, device=DEV))
+  assert (table.lookup(rows, torch.zeros(2, dtype=torch.int64, device=DEV)) == 0).all()
+
+
+def test_a_search_in_parts():
+  """More scores than are kept at a time.  All products and sums are whole numbers, exact in any order."""
+  n, d, count = 1_200_000, 32, 1000
+  codes = torch.randint(0, 256, (n, 16), generator=gen(1), device=DEV).to(torch.uint8)
+  packed = table.PackedRows(codes, torch.ones((n, 1), dtype=torch.bfloat16, device=DEV), d, 32)
+  queries = torch.randint(-3, 4, (count, d), generator=gen(2), device=DEV).float()
+  bias = torch.randint(-5, 6, (n,), generator=gen(3), device=DEV).float()
+  assert n * count > 1 << 30
+  nns, distances, found = packed.search(queries, 7, bias)
+  assert (found == 7).all()
+  values = packed.unpack()
+  for first in (0, 850, 990):  # (queries of two parts among them)
+    scores = queries[first:first + 10].double() @ values.double().T + bias.double()
+    order = (-scores).sort(dim=1, stable=True)
+    assert torch.equal(nns[first:first + 10].long(), order.indices[:, :7])
+    assert torch.equal(distances[first:first + 10].double(), order.values[:, :7])
+  whole = [packed.search(queries[i:i + 500], 7, bias) for i in (0, 500)]
+  assert torch.equal(nns, torch.cat([w[0] for w in whole])) and torch.equal(distances, torch.cat([w[1] for w in whole]))
+
+
+def test_threads_on_streams_of_their_own():
+  rows = normal(1, 4000, 96, dtype=torch.float16)
+  packed = table.pack_rows(rows, 32)
+  work = []
+  for i in range(4):
+    count = (9, 700, 9000, 30_000)[i]
+    work.append((ids_of(10 + i, count, 4000, "zipf"), normal(20 + i, count, 96), normal(30 + i, 1 + 3 * i, 96)))
+  def run(ids, grad, queries):
+    gradient = table.lookup_grad(grad, ids, 4000)
+    scores = packed.scores(queries)
+    return gradient, scores, *packed.search(queries, 5), *table.select_beams(scores[None], keep=8), table.lookup(rows, ids, 2.0)
+  want = [run(*w) for w in work]
+  torch.cuda.synchronize()
+  wrong, errors = [], []
+  def repeat(i):
+    try:
+      with torch.cuda.stream(torch.cuda.Stream()):
+        for _ in range(20):
+          got = run(*work[i])
+          if not all(torch.equal(x, y) for x, y in zip(got, want[i])):
+            wrong.append(i)
+    except Exception as e:  # (an exception in a thread would go unseen)
+      errors.append(e)
+  threads = [threading.Thread(target=repeat, args=(i,)) for i in range(4)]
+  for t in threads:
+    t.start()
+  for t in threads:
+    t.join()
+  assert not errors and not wrong
+
+
+def test_a_capture_without_a_call_before_it():
+  """The first calls of a process are captured ones."""
+  program = """
+import torch
+from cuhnsw_b200 import table
+rows, grad = torch.randn(1000, 256, device="cuda"), torch.randn(20000, 256, device="cuda")
+ids, queries = torch.randint(0, 1000, (20000,), device="cuda"), torch.randn(3, 256, device="cuda")
+torch.cuda.synchronize()
+def run():
+  scores = table.pack_rows(rows).scores(queries)
+  best = table.select_beams(scores[None], keep=5)
+  return table.lookup(rows, ids), table.lookup_grad(grad, ids, 1000), scores, *best, table.reorder(scores[None], best[1])
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+  outs = run()
+for t in outs: t.zero_()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(x, y) for x, y in zip(outs, run()))
+assert torch.equal(outs[0], rows[ids])
+"""
+  done = subprocess.run([sys.executable, "-c", program], cwd=Path(__file__).resolve().parent.parent, timeout=300,
+                        capture_output=True, text=True)
+  assert done.returncode == 0, done.stderr[-2000:]
