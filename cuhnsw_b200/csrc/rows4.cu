@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kPackThreads) unpack_kernel(const unsigned cha
 #pragma unroll 4
     for (int r = 0; r < rows; ++r) {
       const unsigned word = __ldg(reinterpret_cast<const unsigned*>(word_at));
-      const float scale = __bfloat162float(*scale_at);
+      const float scale = __bfloat162float(__ldg(scale_at));
       T v[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) {
