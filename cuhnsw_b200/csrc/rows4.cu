@@ -638,12 +638,17 @@ cudaError_t scores_group(const Scores4Params& p, int queries, cudaStream_t strea
 
 template <class Columns>
 cudaError_t scores_columns(const Scores4Params& p, cudaStream_t stream) {
-  // as many queries at a time as the operands have columns, in tiles of equal size.  (fp32 queries are taken apart on
-  // their way into shared memory, which is better done once: fewer at a time where that makes them fit.)
-  constexpr long long kSpace = 132 * 1024;
-  const long long fit = kSpace / (Columns::kParts * 2 * ((p.d + kFour - 1) / kFour * kFour + 32));
-  long long queries = Columns::kParts == 1 ? 32 : fit >= 4 && fit < 8 ? fit : 8;
-  const long long tiles = (p.nq + queries - 1) / queries;
+  // as many queries at a time as the operands have columns, in tiles of equal size
+  long long queries = Columns::kParts == 1 ? 32 : 8, tiles = (p.nq + queries - 1) / queries;
+  if constexpr (Columns::kParts == 3) {
+    // fp32 queries are taken apart on their way into shared memory, for each chunk again where they do not fit.  With few rows,
+    // smaller tiles that do fit are better: their rows find idle warps.  (8 queries of 5000 dimensions, 3000 rows: two tiles 18
+    // us, chunks 28; 9000 rows: 50 and 39.)
+    constexpr long long kSpace = 208 * 1024;
+    const long long fit = kSpace / (Columns::kParts * 2 * ((p.d + kFour - 1) / kFour * kFour + 32));
+    const long long smaller = fit > 0 ? (p.nq + fit - 1) / fit : 0, sets = (p.n + 15) / 16;
+    if (fit >= 4 && fit < 8 && smaller * sets <= 4 * kSMs) tiles = smaller;
+  }
   queries = (p.nq + tiles - 1) / tiles;
   if constexpr (Columns::kParts == 3) {
     return scores_group<Columns, 3>(p, (int)queries, stream);
