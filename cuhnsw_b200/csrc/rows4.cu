@@ -371,8 +371,10 @@ __global__ void __launch_bounds__(32 * kMostScoreWarps, 1) scores_kernel(const _
   int row_at[kRowsPerLane];
 #pragma unroll
   for (int i = 0; i < kRowsPerLane; ++i) row_at[i] = (int)min((unsigned)(g + 8 * i), rows - 1) * row_bytes + 16 * t;
-  // the lanes of a row load the scales of a row each: t those of row g + 8 * t
-  const int scale_at = (int)min((unsigned)(g + 8 * (t % kRowsPerLane)), rows - 1) * groups;
+  // The lanes of a row load the scales of a row each, t those of row g + 8 * t; of two rows and four scales, two each.
+  constexpr bool kHalves = kGroup == 1 && kRowsPerLane == 2;
+  const int half = kHalves ? 2 * (t >> 1) : 0;
+  const int scale_at = (int)min((unsigned)(g + 8 * (t % kRowsPerLane)), rows - 1) * groups + half;
   const Pairs pairs;
 
   // The way through the rows: the fours of this warp's share of every chunk, unit after unit, one ahead of the sums.
@@ -382,7 +384,7 @@ __global__ void __launch_bounds__(32 * kMostScoreWarps, 1) scores_kernel(const _
   const unsigned char* src = nullptr;
   const unsigned short* scale_src = nullptr;
   uint4 next_words[kRowsPerLane];
-  FourScales<kGroup> next_scale;
+  FourScales<kHalves ? 2 : kGroup> next_scale;
   auto start_unit = [&] {
     src = static_cast<const unsigned char*>(p.codes) + (long long)first_row(ahead_unit) * row_bytes + 64 * ahead_four;
     scale_src = static_cast<const unsigned short*>(p.scales) + (long long)first_row(ahead_unit) * groups + scale_at;
@@ -404,7 +406,7 @@ __global__ void __launch_bounds__(32 * kMostScoreWarps, 1) scores_kernel(const _
         }
       }
       const int at = kGroup < 4 ? ahead_four * (4 / kGroup) : group_fours == 1 ? ahead_four : ahead_four / group_fours;
-      next_scale.load(scale_src + at, groups - at, l.wide_scales);
+      next_scale.load(scale_src + at, groups - at - half, l.wide_scales);
       ++ahead_four;
       src += 64;
       if (--ahead_left == 0) {
@@ -460,7 +462,12 @@ __global__ void __launch_bounds__(32 * kMostScoreWarps, 1) scores_kernel(const _
 #pragma unroll
         for (int i = 0; i < kRowsPerLane; ++i) {
           w[i] = next_words[i];
-          use[i] = next_scale.of_lane((lane & ~3) + i);
+          if constexpr (kHalves) {
+            use[i].low = next_scale.of_lane((lane & ~3) + i).low;
+            use[i].high = next_scale.of_lane((lane & ~3) + i + 2).low;
+          } else {
+            use[i] = next_scale.of_lane((lane & ~3) + i);
+          }
         }
         load();
         float sum[kRowTiles][kTiles][4];

@@ -103,7 +103,7 @@ struct FourScales {
     if constexpr (kGroup == 4) {
       low = *at;
     } else if constexpr (kGroup == 2) {
-      low = wide ? *reinterpret_cast<const unsigned*>(at) : at[0] | (left > 1 ? (unsigned)at[1] << 16 : 0);
+      low = wide ? *reinterpret_cast<const unsigned*>(at) : (left > 0 ? at[0] : 0) | (left > 1 ? (unsigned)at[1] << 16 : 0);
     } else if (wide) {
       const uint2 both = *reinterpret_cast<const uint2*>(at);
       low = both.x;
