@@ -22,19 +22,17 @@ __device__ __forceinline__ int word_offset(int index, int blocks) {
 
 constexpr int kPackThreads = 256;
 
+// (d is a multiple of N)
 template <class T, int N>
 __device__ __forceinline__ void load_eight(const T* row, int dim, int d, T (&v)[8]) {
-  if (dim + 8 <= d) {
 #pragma unroll
-    for (int i = 0; i < 8; i += N) {
-      T w[N];
-      load_many<T, N>(row + dim + i, w);
+  for (int i = 0; i < 8; i += N) {
+    T w[N];
 #pragma unroll
-      for (int j = 0; j < N; ++j) v[i + j] = w[j];
-    }
-  } else {
+    for (int j = 0; j < N; ++j) w[j] = from_f32<T>(0.0f);
+    if (dim + i < d) load_many<T, N>(row + dim + i, w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = dim + i < d ? row[dim + i] : from_f32<T>(0.0f);
+    for (int j = 0; j < N; ++j) v[i + j] = w[j];
   }
 }
 
@@ -47,15 +45,21 @@ __device__ __forceinline__ float largest(const T (&v)[8], float most) {
 
 __device__ __forceinline__ __nv_bfloat16 scale_of(float most) { return __float2bfloat16_rn(__fmul_rn(most, 1.0f / 7.0f)); }
 
+__device__ __forceinline__ constexpr int nibble_shift(int i) { return 4 * ((i >> 1) + 4 * (i & 1)); }
+
+__device__ __forceinline__ bool ordinary(float step) { return step > 1e-30f && step < 1e30f; }  // so is its reciprocal
+
+// The codes of eight values.  step: an ordinary scale.
 template <class T>
 __device__ __forceinline__ unsigned codes_of(const T (&v)[8], float step) {
-  constexpr int kNibble[8] = {0, 4, 1, 5, 2, 6, 3, 7};
-  // Added to a small number, this leaves its nearest whole number (the even one of two) in the last bits.
+  // Added to a small number, this leaves its nearest whole number (the even one of two) in the last bits; what else it leaves is
+  // taken away for all eight at once.
   constexpr float kWhole = 12582912.0f;
-  constexpr unsigned kWholeBits = 0x4b400000u;
-  const bool plain = step > 1e-30f && step < 1e30f;
-  const float inverse = plain ? __frcp_rn(step) : 0.0f;
+  constexpr unsigned kLess = 0x4b400000u - 8;
   unsigned word = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) word -= kLess << nibble_shift(i);
+  const float inverse = __frcp_rn(step);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float x = to_f32(v[i]);
@@ -64,14 +68,18 @@ __device__ __forceinline__ unsigned codes_of(const T (&v)[8], float step) {
     // System/6000 processor, 1990).  Its magnitude is below 7.1, as the scale is the largest value's.
     const float near = x * inverse;
     const float quotient = __fmaf_rn(__fmaf_rn(-near, step, x), inverse, near);
-    word += (__float_as_uint(quotient + kWhole) - kWholeBits + 8) << (4 * kNibble[i]);
+    word += __float_as_uint(quotient + kWhole) << nibble_shift(i);
   }
-  if (!plain) {  // no scale, or one whose reciprocal is no ordinary number
-    word = 0;
-    for (int i = 0; i < 8; ++i) {
-      const float q = step > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(to_f32(v[i]), step)), -8.0f), 7.0f) : 0.0f;
-      word |= (unsigned)((int)q + 8) << (4 * ((i >> 1) + 4 * (i & 1)));
-    }
+  return word;
+}
+
+// The same with no scale, or with one whose reciprocal is no ordinary number.
+template <class T>
+__device__ __forceinline__ unsigned codes_of_any(const T (&v)[8], float step) {
+  unsigned word = 0;
+  for (int i = 0; i < 8; ++i) {
+    const float q = step > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(to_f32(v[i]), step)), -8.0f), 7.0f) : 0.0f;
+    word |= (unsigned)((int)q + 8) << nibble_shift(i);
   }
   return word;
 }
@@ -103,17 +111,38 @@ __global__ void __launch_bounds__(kPackThreads) pack_kernel(const T* rows, long 
         for (int i = 0; i < 8; ++i) v[k][i] = from_f32<T>(0.0f);
       }
     }
+    float most[kAt];
+#pragma unroll
+    for (int k = 0; k < kAt; ++k) most[k] = largest(v[k], 0.0f);
+    for (int off = 1; off < span; off <<= 1) {
+#pragma unroll
+      for (int k = 0; k < kAt; ++k) most[k] = fmaxf(most[k], __shfl_xor_sync(FULL, most[k], off));
+    }
+    unsigned word[kAt];
+    bool live[kAt], other = false;
+#pragma unroll
+    for (int k = 0; k < kAt; ++k) {
+      if (kLong && first - lane + k * lanes >= words) {  // (behind the row for the whole warp)
+        live[k] = false;
+        continue;
+      }
+      most[k] = __bfloat162float(scale_of(most[k]));
+      word[k] = codes_of(v[k], most[k]);
+      live[k] = row + (kLong ? 0 : k) < n && (kLong ? first + k * lanes : first) < words;
+      other = other || (live[k] && !ordinary(most[k]));
+    }
+    if (other) {
+#pragma unroll
+      for (int k = 0; k < kAt; ++k)
+        if (live[k] && !ordinary(most[k])) word[k] = codes_of_any(v[k], most[k]);
+    }
 #pragma unroll
     for (int k = 0; k < kAt; ++k) {
       const int w = kLong ? first + k * lanes : first;
-      float most = largest(v[k], 0.0f);
-      for (int off = 1; off < span; off <<= 1) most = fmaxf(most, __shfl_xor_sync(FULL, most, off));
-      const __nv_bfloat16 scale = scale_of(most);
-      if (row + (kLong ? 0 : k) < n && w < words) {
-        const unsigned word = codes_of(v[k], __bfloat162float(scale));
-        *reinterpret_cast<unsigned*>(dst + (kLong ? 0 : k * (16ll * blocks)) + word_offset(w, blocks)) = word;
+      if (live[k]) {
+        *reinterpret_cast<unsigned*>(dst + (kLong ? 0 : k * (16ll * blocks)) + word_offset(w, blocks)) = word[k];
         const int g = w >> group_shift;
-        if (g << group_shift == w && g < groups) to_scales[(kLong ? 0 : k * groups) + g] = scale;
+        if (g << group_shift == w && g < groups) to_scales[(kLong ? 0 : k * groups) + g] = __float2bfloat16_rn(most[k]);
       }
     }
     if (!kLong) break;
@@ -143,7 +172,8 @@ __global__ void __launch_bounds__(kPackThreads) pack_wide_kernel(const T* rows, 
     const __nv_bfloat16 scale = scale_of(most);
     for (int w = first + lane; w < until; w += 32) {
       load_eight<T, N>(src, 8 * w, d, v);
-      const unsigned word = codes_of(v, __bfloat162float(scale));
+      const float step = __bfloat162float(scale);
+      const unsigned word = ordinary(step) ? codes_of(v, step) : codes_of_any(v, step);
       *reinterpret_cast<unsigned*>(codes + row * (16ll * blocks) + word_offset(w, blocks)) = word;
     }
     if (lane == 0) scales[row * groups + g] = scale;
@@ -165,7 +195,7 @@ __global__ void __launch_bounds__(kPackThreads) unpack_kernel(const unsigned cha
     const unsigned char* word_at = codes + first * row_bytes + word_offset(dim >> 3, blocks);
     const __nv_bfloat16* scale_at = scales + first * groups + (group_shift >= 0 ? dim >> group_shift : dim / group);
     T* to = out + first * d + dim;
-#pragma unroll 4
+#pragma unroll 8
     for (int r = 0; r < rows; ++r) {
       const unsigned word = __ldg(reinterpret_cast<const unsigned*>(word_at));
       const float scale = __bfloat162float(__ldg(scale_at));
@@ -213,7 +243,8 @@ cudaError_t pack_n(const T* rows, long long row_stride, long long n, int d, long
 template <class T>
 cudaError_t pack_t(const T* rows, long long row_stride, long long n, long long d, long long group, void* codes,
                    void* scales, cudaStream_t stream) {
-  const int w = word_bytes(reinterpret_cast<uintptr_t>(rows) | (unsigned long long)(row_stride * sizeof(T)));
+  const int w = word_bytes(reinterpret_cast<uintptr_t>(rows) | (unsigned long long)(row_stride * sizeof(T)) |
+                           (unsigned long long)(d * sizeof(T)));
   if (w == 16) return pack_n<T, 16 / sizeof(T)>(rows, row_stride, n, (int)d, group, codes, scales, stream);
   if (w == 8) return pack_n<T, 8 / sizeof(T)>(rows, row_stride, n, (int)d, group, codes, scales, stream);
   if (w == 4) return pack_n<T, 4 / sizeof(T)>(rows, row_stride, n, (int)d, group, codes, scales, stream);
