@@ -248,7 +248,8 @@ __global__ void __launch_bounds__(kThreads) piece_kernel(SelectParams p, int pie
 constexpr int kPoolTotals = 2048;
 
 // One CTA per sequence.  The lists of the pieces are in order: of their first totals the `keep`-th is a bound that as many
-// candidates reach, and from there on there are few.
+// candidates reach, and from there on there are few.  Bound: latency, a chain of some ten steps.  (8 sequences of 4 beams over
+// 32 000 ids, 64 lists: 25 us for a whole step of a beam search, 42 if up to 256 candidates are put in order without a bound.)
 __global__ void __launch_bounds__(kThreads) sequence_kernel(SelectParams p, int pieces, const ScoreKey* best,
                                                             const float2* norms) {
   extern __shared__ __align__(16) unsigned char smem[];
@@ -293,7 +294,7 @@ __global__ void __launch_bounds__(kThreads) sequence_kernel(SelectParams p, int 
   };
   Pool<TotalKey> pool{pool_keys, &pool_count, kPoolTotals};
   TotalKey least = {0, 0};
-  if (total > kThreads) {
+  if (total > 32) {
     // every thread one of the lists' first totals (the best of several lists', of more lists than threads), the `keep`-th of
     // them all: as many candidates reach it
     const long long heads = min((long long)kThreads, total);

@@ -132,8 +132,9 @@ __device__ __forceinline__ unsigned key_at(const LookupGradParams& p, long long 
 }
 
 // Up to kRankMost tokens: every token's place is the number of smaller keys and of equal ones before it, counted against all
-// tokens: no pass depends on another one.  8192 tokens take 14 us, 2048 seven, 511 three.
-constexpr int kRankMost = 8192;
+// tokens: no pass depends on another one.  (The whole gradient, 64 floats a row: 4096 tokens 24 us, by digits 29; 6000 tokens 29
+// and 30; 8192 tokens 40 and 32.)
+constexpr int kRankMost = 6144;
 constexpr int kRankThreads = kZeroThreads;
 constexpr int kRankTokens = 64;                                // of a CTA
 constexpr int kRankShares = kRankThreads / kRankTokens;        // threads that share a token
@@ -797,6 +798,10 @@ cudaError_t grad_t(const LookupGradParams& p, cudaStream_t stream) {
     e = sum_t<G, O, 16 / sizeof(G), false>(p, plan, s, at, stream);
   else if (w >= 8 && to >= 8)
     e = sum_t<G, O, 8 / sizeof(G), false>(p, plan, s, at, stream);
+  else if (w >= 4 && to >= 4 && (sizeof(G) == 2 || p.d <= kSumThreads))
+    // (whole words of one float, of rows that a CTA has threads for: 60 000 tokens of 17 floats 42 us, 55 with floats apart;
+    // 20 000 of 953: 79 and 75)
+    e = sum_t<G, O, 4 / sizeof(G), false>(p, plan, s, at, stream);
   else
     e = sum_t<G, O, 4, true>(p, plan, s, at, stream);
   if (e != cudaSuccess || plan.chunks < 2) return e;
