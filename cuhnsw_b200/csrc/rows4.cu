@@ -85,7 +85,8 @@ __device__ __forceinline__ unsigned codes_of_any(const T (&v)[8], float step) {
 }
 
 // `lanes` lanes (a power of two, at most a warp) take as many words of eight dimensions of a row at a time, whole groups; kAt times
-// in a row before they look at the first: of kAt rows that are no longer than that, or of one row.  Bound: HBM bytes.
+// in a row before they look at the first: of kAt rows that are no longer than that, or of one row.  Bound: instructions (some
+// 20 per value; 50 000 rows of 2048 bfloat16 in 80 us, 3.2 TB/s, issue slots 0.8 in use).
 template <class T, int N, int kAt, bool kLong>
 __global__ void __launch_bounds__(kPackThreads) pack_kernel(const T* rows, long long row_stride, long long n, int d,
                                                             int group_shift, int groups, unsigned char* codes,
@@ -181,6 +182,7 @@ __global__ void __launch_bounds__(kPackThreads) pack_wide_kernel(const T* rows, 
 }
 
 // `lanes` threads share `each` rows, V neighbouring values of each (V divides 8): where they are in a row is worked out once.
+// Bound: HBM bytes (50 000 rows of 2048 to fp32 in 84 us, 5.5 TB/s; with 4 rows on their way instead of 8 96 us, with 16 101).
 template <class T, int V>
 __global__ void __launch_bounds__(kPackThreads) unpack_kernel(const unsigned char* codes, const __nv_bfloat16* scales,
                                                               long long n, int d, int group, int group_shift, T* out,
@@ -233,6 +235,8 @@ cudaError_t pack_n(const T* rows, long long row_stride, long long n, int d, long
   int shift = 0;
   while ((1 << shift) < group_words) ++shift;
   const int teams = kPackThreads / lanes, groups = (int)((d + group - 1) / group);
+  // four rows or four words of a row at a time, unless that leaves SMs without work (1 183 514 rows of 50 floats 60 us, one at a
+  // time 73; 20 000 of 64 are 4.4 and 4.0)
   const bool longer = words > lanes, many = longer || n > (long long)4 * kSMs * teams;
   const long long per = longer || !many ? teams : 4 * teams, blocks = (n + per - 1) / per;
   if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
@@ -255,7 +259,7 @@ template <class T, int V>
 cudaError_t unpack_v(const unsigned char* codes, const __nv_bfloat16* scales, long long n, int d, int group, T* out,
                      cudaStream_t stream) {
   const int lanes = next_pow2((d + V - 1) / V, kPackThreads);
-  // 16 rows, fewer while there are not four CTAs per SM
+  // 16 rows, fewer while there are not four CTAs per SM (1 183 514 rows of 50 dimensions 63 us, one at a time 246)
   int each = 16;
   while (each > 1 && n / ((long long)(kPackThreads / lanes) * each) < 4 * kSMs) each /= 2;
   const long long per = (long long)(kPackThreads / lanes) * each, blocks = (n + per - 1) / per;
@@ -718,7 +722,7 @@ cudaError_t launch_unpack4(const void* codes, const void* scales, long long n, l
 
 cudaError_t launch_scores4(const Scores4Params& p, cudaStream_t stream) {
   if (p.n <= 0 || p.nq <= 0) return cudaSuccess;
-  if (p.d <= kFour) return launch_scores4_narrow(p, stream);
+  if (p.d <= kFour) return launch_scores4_narrow(p, stream);  // (both sides measured there)
   if (p.type == kF32) return scores_columns<ColumnsF32>(p, stream);
   if (p.type == kF16) return scores_columns<ColumnsF16>(p, stream);
   return scores_columns<ColumnsBF16>(p, stream);

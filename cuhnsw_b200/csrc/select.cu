@@ -130,7 +130,8 @@ struct Pool {
 // Every thread holds kEach scores.  The CTA's `keep` best: of the largest scores of twice as many groups of threads
 // the `keep`-th is a bound that as many scores reach; the scores of the few threads whose largest one reaches it are looked at again,
 // and what is not below goes into a pool, the pool in order.  Also the piece's largest score and its sum of
-// exponentials.  Bound: HBM bytes; a score costs its part in the maximum and in the sum.
+// exponentials.  Bound: instructions and HBM bytes; a score costs its part in the maximum and in the sum (256 x 131 072 floats in
+// 40 us, 3.4 TB/s, issue slots 0.58 in use).
 constexpr int kPoolScores = 4096;
 constexpr int kWarps = kThreads / 32;
 
@@ -356,7 +357,8 @@ struct SelectPlan {
 };
 SelectPlan select_plan(long long rows, long long vocabulary) {
   SelectPlan s;
-  // pieces of up to 8192 scores where that still gives every SM four of them, all of about the same length
+  // Pieces of up to 8192 scores where that still gives every SM four of them, all of about the same length.  (A step of a beam
+  // search, 32 x 8 beams of 131 072 ids: 89 us, with pieces of 2048 127; 1 x 4 of 32 000: 27 us with 2048, 33 with 8192.)
   s.each = 32;
   while (s.each > 8 && rows * ((vocabulary + kThreads * s.each - 1) / (kThreads * s.each)) < 4 * kSMs) s.each /= 2;
   const long long places = vocabulary + 7;  // and those before the row
@@ -402,7 +404,7 @@ __device__ __forceinline__ void copy_row(const ReorderState& s, const char* from
   }
 }
 
-// Grid: pieces of a row x rows x states
+// Grid: pieces of a row x rows x states.  Bound: HBM bytes (a cache of 269 MB there and back in 42 us, from the L2 cache in part).
 __global__ void __launch_bounds__(kThreads) reorder_kernel(const __grid_constant__ ReorderParams p) {
   next_launch_may_start();
   wait_for_launch_before();

@@ -19,7 +19,8 @@ __device__ __forceinline__ long long id_at(const void* ids, int ids64, long long
 
 constexpr int kLookupThreads = 256;
 
-// `lanes` threads take kRows tokens at once and kAt words of each, so that so many loads of each are in flight.  Bound: HBM bytes.
+// `lanes` threads take kRows tokens at once and kAt words of each, so that so many loads of each are in flight.  Bound: HBM bytes
+// (100 000 rows of 50 floats out of 1 183 514 in 10 us, 4.1 TB/s of sectors of 32 bytes), of few tokens the launch (3 us).
 template <class T, int N, int kRows, int kAt>
 __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(LookupParams p, int lanes) {
   const int group = threadIdx.x / lanes, lane = threadIdx.x % lanes, groups = kLookupThreads / lanes;
@@ -74,7 +75,8 @@ cudaError_t lookup_t(const LookupParams& p, cudaStream_t stream) {
   constexpr int kAt = N * sizeof(T) >= 8 ? 1 : 4;
   const int lanes = next_pow2((p.d + kAt * N - 1) / (kAt * N), kLookupThreads);
   const int groups = kLookupThreads / lanes;
-  // four rows at a time, unless there are too few tokens to give every SM work
+  // Four rows at a time, unless there are too few tokens to give every SM work.  (50 000 rows of 1024 bfloat16 30 us, one at a
+  // time 48; 8 of 2048 3.4 us, one at a time 2.9.)
   const bool many = p.tokens > (long long)4 * groups * kSMs;
   const long long per = (many ? 4 : 1) * groups;
   const long long blocks = (p.tokens + per - 1) / per;
@@ -204,14 +206,17 @@ __global__ void __launch_bounds__(kRankThreads) sort_rank_kernel(LookupGradParam
 // More tokens: a least-significant-digit radix sort.  Up to kParts CTAs have a contiguous part of the tokens each; a pass counts the
 // digits of each part, finds out where its tokens of each digit begin and puts them there, tile by tile.
 constexpr int kParts = 16 * kSMs;
-constexpr int kPartsUnscanned = 64;     // every CTA adds up the counts of so few parts by itself
+// Every CTA adds up the counts of so few parts by itself.  (The whole gradient, 16 000 tokens: 31 us, with a launch for it 39;
+// 250 000: 78, with it 61.)
+constexpr int kPartsUnscanned = 64;
 constexpr int kTileThreads = kZeroThreads;
 constexpr int kTileWarps = kTileThreads / 32;
+constexpr int kTileItems = 4;           // tokens of a tile per thread (16: 4 000 000 tokens 338 us, with 4 294; 250 000: 81 and 61)
+constexpr int kTile = kTileThreads * kTileItems;
 constexpr int kMaxDigit = 8;
 
 struct SortPlan {
   int passes, digit;      // bits
-  int items;              // tokens of a tile per thread: 4 or 16
   int scanned;            // whether counts become places in a launch of their own
   int parts;
   long long part;         // tokens, whole tiles
@@ -223,17 +228,14 @@ SortPlan sort_plan(long long tokens, long long n) {
   s.passes = (bits + kMaxDigit - 1) / kMaxDigit;
   s.digit = (bits + s.passes - 1) / s.passes;
   if (s.digit < 2) s.digit = 2;  // (four counts are read at a time)
-  // small tiles while each is a part: more CTAs that take less time
-  s.items = tokens <= (long long)kParts * kTileThreads * 4 ? 4 : 16;
-  const long long tile = kTileThreads * s.items, tiles = (tokens + tile - 1) / tile;
-  s.part = (tiles + kParts - 1) / kParts * tile;
+  const long long tiles = (tokens + kTile - 1) / kTile;
+  s.part = (tiles + kParts - 1) / kParts * kTile;
   s.parts = (int)((tokens + s.part - 1) / s.part);
   s.scanned = s.parts > kPartsUnscanned;
   return s;
 }
 
 // counts[part * digits + digit].  `pairs`: (key, token) as the pass before left them; the first pass reads the ids.
-template <int kTileItems>
 __global__ void __launch_bounds__(kTileThreads) sort_count_kernel(LookupGradParams p, ZeroPart zeros, SortPlan plan,
                                                                   const uint2* pairs, int shift, unsigned* counts,
                                                                   unsigned* joins) {
@@ -243,7 +245,6 @@ __global__ void __launch_bounds__(kTileThreads) sort_count_kernel(LookupGradPara
     write_zeros(zeros);
     return;
   }
-  constexpr int kTile = kTileThreads * kTileItems;
   const int digits = 1 << plan.digit;
   __shared__ unsigned bins[1 << kMaxDigit];
   for (int i = threadIdx.x; i < digits; i += kTileThreads) bins[i] = 0;
@@ -312,12 +313,11 @@ __global__ void __launch_bounds__(kTileThreads) sort_scan_kernel(unsigned* count
 
 // Rank of each of a warp's keys (lane l holds items l, 32 + l, ..) among the earlier keys of the warp with the same
 // digit; counts[digit] ends as the warp's number of keys with that digit.
-template <int Items>
-__device__ __forceinline__ void warp_ranks(const unsigned (&key)[Items], int shift, unsigned mask, int valid,
-                                           unsigned short* counts, unsigned (&rank)[Items]) {
+__device__ __forceinline__ void warp_ranks(const unsigned (&key)[kTileItems], int shift, unsigned mask, int valid,
+                                           unsigned short* counts, unsigned (&rank)[kTileItems]) {
   const unsigned earlier = (1u << lane_id()) - 1;
 #pragma unroll
-  for (int i = 0; i < Items; ++i) {
+  for (int i = 0; i < kTileItems; ++i) {
     if (i * 32 >= valid) break;
     const bool live = i * 32 + lane_id() < valid;
     const unsigned digit = (key[i] >> shift) & mask;
@@ -331,7 +331,6 @@ __device__ __forceinline__ void warp_ranks(const unsigned (&key)[Items], int shi
 }
 
 // Every tile is put in order in shared memory first, so that what goes to one digit's places is written side by side.
-template <int kTileItems>
 __global__ void __launch_bounds__(kTileThreads) sort_place_kernel(LookupGradParams p, ZeroPart zeros, SortPlan plan,
                                                                   const uint2* pairs, int shift, const unsigned* counts,
                                                                   uint2* sorted) {
@@ -341,7 +340,6 @@ __global__ void __launch_bounds__(kTileThreads) sort_place_kernel(LookupGradPara
     write_zeros(zeros);
     return;
   }
-  constexpr int kTile = kTileThreads * kTileItems;
   constexpr int kDigits = 1 << kMaxDigit;
   static_assert(kDigits == kTileThreads, "a digit per thread");
   __shared__ unsigned short warp_counts[kTileWarps * kDigits];
@@ -402,7 +400,7 @@ __global__ void __launch_bounds__(kTileThreads) sort_place_kernel(LookupGradPara
     const int held = (int)min((long long)kTile, part_end - tile);
     const int valid = max(0, min(32 * kTileItems, held - warp * 32 * kTileItems));
     __syncthreads();
-    warp_ranks<kTileItems>(key, shift, digits - 1, valid, warp_counts + warp * digits, rank);
+    warp_ranks(key, shift, digits - 1, valid, warp_counts + warp * digits, rank);
     __syncthreads();
     // a digit's tokens in the warps before, and in the tile
     unsigned total = 0;
@@ -484,11 +482,12 @@ __device__ __forceinline__ void write_row(const LookupGradParams& p, unsigned ro
 }
 
 // `lanes` threads have a chunk (of up to lanes * N dimensions); kInFlight rows of the gradient are on their way to each.  A
-// thread has N neighbouring values or, of rows that are no whole words (kApart), N values `lanes` apart.
+// thread has N neighbouring values or, of rows that are no whole words (kApart), N values `lanes` apart.  Bound: HBM latency of
+// rows anywhere (1 000 003 of 50 floats in 100 us, 3.8 TB/s; eight rows on their way instead of four: the same).
 template <class G, class O, int N, bool kApart>
-__global__ void __launch_bounds__(kSumThreads, kApart || sizeof(G) * N > 8 ? 3 : 4) sum_kernel(LookupGradParams p, SumPlan plan, const uint2* sorted,
-                                                                                   float* heads, float* tails, unsigned* joins,
-                                                                                   unsigned* join_list, int lanes) {
+__global__ void __launch_bounds__(kSumThreads, kApart || sizeof(G) * N > 8 ? 3 : 4)
+  sum_kernel(LookupGradParams p, SumPlan plan, const uint2* sorted, float* heads, float* tails, unsigned* joins,
+             unsigned* join_list, int lanes) {
   const int group = threadIdx.x / lanes, lane = threadIdx.x % lanes, groups = blockDim.x / lanes;
   const long long chunk = (long long)blockIdx.x * groups + group;
   next_launch_may_start();
@@ -595,8 +594,9 @@ __global__ void __launch_bounds__(kSumThreads, kApart || sizeof(G) * N > 8 ? 3 :
   }
 }
 
-// Rows that cross borders of chunks.  A warp takes one of them and kJoinDims dimensions; of a row with many partial sums the
-// CTA's warps add up a share each.
+// Rows that cross borders of chunks.  A warp takes one of them and 32 * kEach dimensions; of a row with many partial sums the
+// CTA's warps add up a share each.  Bound: latency, some eight dependent loads (8 to 18 us).  Of up to 32 dimensions 32 partial
+// sums are on their way at a time: 300 000 tokens of 17 dimensions, half of them of a few rows, 68 us with kEach 1, 81 with 4.
 constexpr int kJoinWarps = 8;
 constexpr int kJoinBlocks = 48 / kJoinWarps * kSMs;
 constexpr int kJoinLoads = 32;       // in flight per lane
@@ -773,11 +773,9 @@ cudaError_t grad_t(const LookupGradParams& p, cudaStream_t stream) {
       const uint2* pairs = pass ? s.pairs[at] : nullptr;
       const int to = pass ? 1 - at : 0, shift = pass * sort.digit;
       const ZeroPart first = zeros(sort.parts, 2 * pass, 2 * sort.passes), second = zeros(sort.parts, 2 * pass + 1, 2 * sort.passes);
-      auto* count = sort.items == 4 ? sort_count_kernel<4> : sort_count_kernel<16>;
-      auto* place = sort.items == 4 ? sort_place_kernel<4> : sort_place_kernel<16>;
       unsigned* joins = pass ? nullptr : s.joins;
       const dim3 grid((unsigned)(first.first + zero_blocks(first)));
-      e = launch_early(count, grid, kTileThreads, 0, stream, p, first, sort, pairs, shift, s.counts, joins);
+      e = launch_early(sort_count_kernel, grid, kTileThreads, 0, stream, p, first, sort, pairs, shift, s.counts, joins);
       if (e != cudaSuccess) return e;
       if (sort.scanned) {
         unsigned* totals = s.counts + ((size_t)sort.parts << sort.digit);
@@ -785,7 +783,7 @@ cudaError_t grad_t(const LookupGradParams& p, cudaStream_t stream) {
                          sort.parts);
         if (e != cudaSuccess) return e;
       }
-      e = launch_early(place, dim3((unsigned)(second.first + zero_blocks(second))), kTileThreads, 0, stream, p, second, sort,
+      e = launch_early(sort_place_kernel, dim3((unsigned)(second.first + zero_blocks(second))), kTileThreads, 0, stream, p, second, sort,
                        pairs, shift, s.counts, s.pairs[to]);
       if (e != cudaSuccess) return e;
       at = to;

@@ -1,7 +1,7 @@
 // The operators over a table of embeddings for torch tensors: checks of the arguments, results and workspaces from torch's
 // allocator, torch's current stream, and one call of the C ABI (include/cuhnsw_b200.h).  Functions of the module
 // cuhnsw_b200._table, which cuhnsw_b200/table.py documents and calls with positional arguments.  (Compiled, because the same
-// steps in Python take longer than the kernels of a single token: 50 us for a step of a beam search, of which 12 are left.)
+// steps in Python take longer than the kernels of a single token: 50 us for a step of a beam search, of which 15 are left.)
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
