@@ -50,7 +50,8 @@ def lookup(rows, ids, scale=1.0):
 
   rows: float32, float16 or bfloat16 ``[num_rows, num_dims]``, rows any distance apart; ids: int32 or int64 of any shape.  An id
   outside ``0 .. num_rows-1`` gives zeros and gets no gradient: the -1 of an empty result slot of a search, or the padding of a
-  batch.  Differentiable in ``rows`` (once): see ``lookup_grad``."""
+  batch.  Differentiable in ``rows`` (once): see ``lookup_grad``.  The backward pass may be captured into a CUDA graph
+  as torch's own may: not while an eager graph of the same leaf lives, which torch answers with an error."""
   if isinstance(rows, torch.Tensor) and rows.requires_grad and torch.is_grad_enabled():
     return _Lookup.apply(rows, ids, scale)
   return _table.lookup(rows, ids, scale)
@@ -61,7 +62,8 @@ def lookup_grad(grad, ids, num_rows, scale=1.0, out=None, accumulate=False):
 
   grad: ``ids.shape + (num_dims,)``; the sums are taken in fp32 over the ids sorted by row, in a fixed order, and rounded
   once: the same call gives the same bits.  out: a dense ``[num_rows, num_dims]`` tensor of grad's type or of float32 (default: a
-  new one of grad's type); with ``accumulate`` the gradient is added to what it holds, and rows without ids keep their bits."""
+  new one of grad's type) that overlaps neither grad nor ids; with ``accumulate`` the gradient is added to what it holds, and
+  rows without ids keep their bits."""
   return _table.lookup_grad(grad, ids, num_rows, scale, out, accumulate)
 
 
@@ -110,7 +112,7 @@ class PackedRows:
     """``CuHNSW.search_knn``'s triple from an exhaustive search of the dot metric over these rows: (nns int32 ``[Q, topk]``,
     distances float32 ``[Q, topk]``, found_cnt int32 ``[Q]``), rows ascending by (distance, id), empty slots -1 / +inf; CUDA
     tensors.  A distance is minus the score (``scores``; with ``bias`` = -|row|^2 / 2 the order is that of the l2
-    metric).  topk up to 256."""
+    metric).  topk up to 256.  The scores of as many queries as fill 4 GB, at least 32, are held at a time."""
     return _table.search(self.codes, self.scales, self.num_dims, self.group, queries, topk, bias)
 
 
