@@ -141,6 +141,26 @@ def test_grad_against_64_bits(dtype, out_type, count, n, d, kind):
     assert torch.equal(table.lookup_grad(grad, ids, n, 1.5), out)
 
 
+@pytest.mark.parametrize("dtype, out_type", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("bf16", "f32"), ("f16", "f32")])
+@pytest.mark.parametrize("count, n, d, kind", [
+  (1, 1, 1, "one"), (32, 40, 5, "zipf"), (31, 3, 512, "any"), (32, 1, 511, "one"), (33, 200_000, 13, "any"), (256, 60_000, 24, "zipf"),
+  (257, 20_000, 120, "zipf"), (512, 5000, 500, "one"), (512, 5001, 512, "zipf"), (511, 300_000, 9, "empty"), (512, 100_000, 50, "ascending"),
+  (512, 1_000_003, 16, "any"), (500, 1500, 1021, "any"), (513, 5000, 500, "zipf")])
+def test_grad_of_few_tokens(dtype, out_type, count, n, d, kind):
+  grad = normal(count, count, d + 3, dtype=TYPES[dtype])[:, :d]
+  ids = ids_of(count + 2, count, n, kind, torch.int32 if count % 2 else torch.int64)
+  if ids.dtype == torch.int64 and count > 8:
+    ids[3], ids[5] = -2 ** 63, 2 ** 63 - 1
+  space = torch.full((n * d + 2,), 7.0, dtype=TYPES[out_type], device=DEV)
+  out = space[1:-1].view(n, d)  # at an odd place, between values that stay
+  table.lookup_grad(grad, ids, n, -2.5, out=out)
+  assert space[0] == 7 and space[-1] == 7
+  check_grad(grad, ids, n, -2.5, out)
+  even = table.lookup_grad(grad.contiguous(), ids, n, -2.5, out=torch.full_like(out, math.nan))
+  check_grad(grad, ids, n, -2.5, even)
+  assert torch.equal(table.lookup_grad(grad.contiguous(), ids, n, -2.5, out=torch.full_like(out, math.nan)), even)
+
+
 def test_grad_takes_any_layout():
   wide = normal(3, 500, 100)
   ids = ids_of(4, 500, 60, "any")
