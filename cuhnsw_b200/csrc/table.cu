@@ -203,8 +203,8 @@ __global__ void __launch_bounds__(kRankThreads) sort_rank_kernel(LookupGradParam
   }
 }
 
-// More tokens: a least-significant-digit radix sort.  Up to kParts CTAs have a contiguous part of the tokens each; a pass counts the
-// digits of each part, finds out where its tokens of each digit begin and puts them there, tile by tile.
+// More tokens: a least-significant-digit radix sort.  Up to kParts CTAs have a contiguous part of the tokens each; a pass counts
+// the digits of each part, finds out where its tokens of each digit begin and puts them there, tile by tile.
 constexpr int kParts = 16 * kSMs;
 // Every CTA adds up the counts of so few parts by itself.  (The whole gradient, 16 000 tokens: 31 us, with a launch for it 39;
 // 250 000: 78, with it 61.)
@@ -492,7 +492,8 @@ __global__ void __launch_bounds__(kSumThreads, kApart || sizeof(G) * N > 8 ? 3 :
   const long long chunk = (long long)blockIdx.x * groups + group;
   next_launch_may_start();
   wait_for_launch_before();
-  __shared__ __align__(16) unsigned chunk_keys[kSumThreads / kSumLanes][kMostChunk], chunk_tokens[kSumThreads / kSumLanes][kMostChunk];
+  __shared__ __align__(16) unsigned chunk_keys[kSumThreads / kSumLanes][kMostChunk];
+  __shared__ __align__(16) unsigned chunk_tokens[kSumThreads / kSumLanes][kMostChunk];
   const unsigned none = (unsigned)p.n;
   const long long begin = chunk * plan.chunk, end = min(begin + plan.chunk, p.tokens);
   for (int i = lane; i < plan.chunk; i += lanes) {  // (the end of the last chunk as empty slots)
@@ -537,7 +538,8 @@ __global__ void __launch_bounds__(kSumThreads, kApart || sizeof(G) * N > 8 ? 3 :
   using Word = typename WordOf<kApart ? sizeof(G) : sizeof(G) * N>::type;
   constexpr int kWords = kApart ? N : 1;
   auto fetch = [&](int t, Word (&word)[kInFlight][kWords]) {
-    const uint4 k = *reinterpret_cast<const uint4*>(chunk_keys[group] + t), at = *reinterpret_cast<const uint4*>(chunk_tokens[group] + t);
+    const uint4 k = *reinterpret_cast<const uint4*>(chunk_keys[group] + t);
+    const uint4 at = *reinterpret_cast<const uint4*>(chunk_tokens[group] + t);
     const unsigned key[kInFlight] = {k.x, k.y, k.z, k.w}, token[kInFlight] = {at.x, at.y, at.z, at.w};
 #pragma unroll
     for (int i = 0; i < kInFlight; ++i) {
@@ -809,7 +811,8 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(LookupGradParams p, in
     const int s = long_rows[i], row = sorted_row[s];
     int length = 0;
     for (int base = s; base < count; base += kFewThreads)
-      length += __syncthreads_count(base + (int)threadIdx.x < count && sorted_row[min(base + (int)threadIdx.x, count - 1)] == row);
+      length += __syncthreads_count(base + (int)threadIdx.x < count &&
+                                    sorted_row[min(base + (int)threadIdx.x, count - 1)] == row);
     const int share = (length + groups - 1) / groups, from = min(length, group * share), to = min(length, from + share);
     for (int base = 0; base < d; base += lanes * N) {
       const int c = base + lane * N;
@@ -924,7 +927,8 @@ cudaError_t grad_t(const LookupGradParams& p, cudaStream_t stream) {
     for (int pass = 0; pass < sort.passes; ++pass) {
       const uint2* pairs = pass ? s.pairs[at] : nullptr;
       const int to = pass ? 1 - at : 0, shift = pass * sort.digit;
-      const ZeroPart first = zeros(sort.parts, 2 * pass, 2 * sort.passes), second = zeros(sort.parts, 2 * pass + 1, 2 * sort.passes);
+      const ZeroPart first = zeros(sort.parts, 2 * pass, 2 * sort.passes);
+      const ZeroPart second = zeros(sort.parts, 2 * pass + 1, 2 * sort.passes);
       unsigned* joins = pass ? nullptr : s.joins;
       const dim3 grid((unsigned)(first.first + zero_blocks(first)));
       e = launch_early(sort_count_kernel, grid, kTileThreads, 0, stream, p, first, sort, pairs, shift, s.counts, joins);
@@ -935,8 +939,8 @@ cudaError_t grad_t(const LookupGradParams& p, cudaStream_t stream) {
                          sort.parts);
         if (e != cudaSuccess) return e;
       }
-      e = launch_early(sort_place_kernel, dim3((unsigned)(second.first + zero_blocks(second))), kTileThreads, 0, stream, p, second, sort,
-                       pairs, shift, s.counts, s.pairs[to]);
+      e = launch_early(sort_place_kernel, dim3((unsigned)(second.first + zero_blocks(second))), kTileThreads, 0, stream, p, second,
+                       sort, pairs, shift, s.counts, s.pairs[to]);
       if (e != cudaSuccess) return e;
       at = to;
     }

@@ -60,7 +60,7 @@ def lookup(rows, ids, scale=1.0):
 def lookup_grad(grad, ids, num_rows, scale=1.0, out=None, accumulate=False):
   """The gradient of ``lookup``'s rows: ``out[r] = scale * sum of grad[t] over all t with ids[t] == r``, for every row.
 
-  grad: ``ids.shape + (num_dims,)``; the sums are taken in fp32 over the ids sorted by row, in a fixed order, and rounded
+  grad: ``ids.shape + (num_dims,)``; the sums are taken in fp32 in a fixed order, and rounded
   once: the same call gives the same bits.  out: a dense ``[num_rows, num_dims]`` tensor of grad's type or of float32 (default: a
   new one of grad's type) that overlaps neither grad nor ids; with ``accumulate`` the gradient is added to what it holds, and
   rows without ids keep their bits."""

@@ -201,7 +201,7 @@ int cuhnsw_lookup_device(const void* d_rows, int64_t row_stride, int64_t num_row
 /* The gradient of that lookup: d_out[r] = scale * sum of d_grad[t] over all t with d_ids[t] = r, for every row of the
  * table; with `accumulate` it is added to what d_out holds, and rows without ids keep their bits.  d_grad: num_ids rows of num_dims
  * values of `type`, grad_stride values apart; d_out: num_rows x num_dims, dense, of out_type (`type` or CUHNSW_F32).
- * The ids are sorted and the sums taken in fp32 in a fixed order: the result does not change from call to call. */
+ * The sums are taken in fp32 in a fixed order: the result does not change from call to call.  d_out must not overlap the inputs. */
 int64_t cuhnsw_lookup_grad_workspace(int64_t num_ids, int64_t num_rows, int64_t num_dims);
 int cuhnsw_lookup_grad_device(const void* d_grad, int64_t grad_stride, int32_t type, const void* d_ids, int32_t ids64,
                               int64_t num_ids, int64_t num_rows, int64_t num_dims, float scale, void* d_out,
