@@ -8,6 +8,8 @@
 // w & 0x000f000f is a pair of consecutive values in two halves of a register.
 #include "scores4.cuh"
 
+#include <type_traits>
+
 namespace hnsw {
 
 namespace {
@@ -84,32 +86,98 @@ __device__ __forceinline__ unsigned codes_of_any(const T (&v)[8], float step) {
   return word;
 }
 
-// `lanes` lanes (a power of two, at most a warp) take as many words of eight dimensions of a row at a time, whole groups; kAt times
-// in a row before they look at the first: of kAt rows that are no longer than that, or of one row.  Bound: instructions (some
-// 20 per value; 50 000 rows of 2048 bfloat16 in 80 us, 3.2 TB/s, issue slots 0.8 in use).
-template <class T, int N, int kAt, bool kLong>
-__global__ void __launch_bounds__(kPackThreads) pack_kernel(const T* rows, long long row_stride, long long n, int d,
-                                                            int group_shift, int groups, unsigned char* codes,
-                                                            __nv_bfloat16* scales, int lanes) {
+// `lanes` lanes (a power of two, at most a warp) take the words of eight dimensions of kAt rows at once.  Bound: instructions, some
+// 20 per value (1 183 514 rows of 50 floats in 60 us, 4.9 TB/s).
+template <class T, int N, int kAt>
+__global__ void __launch_bounds__(kPackThreads, 4) pack_kernel(const T* rows, long long row_stride, long long n, int d,
+                                                               int group_shift, int groups, unsigned char* codes,
+                                                               __nv_bfloat16* scales, int lanes) {
   next_launch_may_start();
   wait_for_launch_before();
   const int lane = threadIdx.x & (lanes - 1);
   const int blocks = (d + kBlock - 1) / kBlock, words = 4 * blocks, span = min(lanes, 1 << group_shift);
-  const long long team = (long long)blockIdx.x * (kPackThreads / lanes) + threadIdx.x / lanes;
-  const long long row = kLong ? team : team * kAt;
+  const long long row = ((long long)blockIdx.x * (kPackThreads / lanes) + threadIdx.x / lanes) * kAt;
   const T* src = rows + row * row_stride;
   unsigned char* dst = codes + row * (16ll * blocks);
   __nv_bfloat16* to_scales = scales + row * groups;
-  for (int first = lane; first - lane < words; first += kAt * lanes) {
+  T v[kAt][8];
+#pragma unroll
+  for (int k = 0; k < kAt; ++k) {
+    if (row + k < n && 8 * lane < d) {
+      load_eight<T, N>(src + k * row_stride, 8 * lane, d, v[k]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[k][i] = from_f32<T>(0.0f);
+    }
+  }
+  float most[kAt];
+#pragma unroll
+  for (int k = 0; k < kAt; ++k) most[k] = largest(v[k], 0.0f);
+  for (int off = 1; off < span; off <<= 1) {
+#pragma unroll
+    for (int k = 0; k < kAt; ++k) most[k] = fmaxf(most[k], __shfl_xor_sync(FULL, most[k], off));
+  }
+  unsigned word[kAt];
+  bool live[kAt], other = false;
+#pragma unroll
+  for (int k = 0; k < kAt; ++k) {
+    most[k] = __bfloat162float(scale_of(most[k]));
+    word[k] = codes_of(v[k], most[k]);
+    live[k] = row + k < n && lane < words;
+    other = other || (live[k] && !ordinary(most[k]));
+  }
+  if (other) {
+#pragma unroll
+    for (int k = 0; k < kAt; ++k)
+      if (live[k] && !ordinary(most[k])) word[k] = codes_of_any(v[k], most[k]);
+  }
+  const int g = lane >> group_shift;
+#pragma unroll
+  for (int k = 0; k < kAt; ++k) {
+    if (live[k]) {
+      *reinterpret_cast<unsigned*>(dst + k * (16ll * blocks) + word_offset(lane, blocks)) = word[k];
+      if (g << group_shift == lane && g < groups) to_scales[k * groups + g] = __float2bfloat16_rn(most[k]);
+    }
+  }
+}
+
+// Rows of more than 32 words: a warp has a row, and 4 x 32 words of it at a time, whole ones without a question (50 000 rows of 2048
+// bfloat16 in 66 us, 3.9 TB/s; with a question at each word 80).  Bound: instructions.
+template <class T, int N>
+__global__ void __launch_bounds__(kPackThreads) pack_long_kernel(const T* rows, long long row_stride, long long n, int d,
+                                                                 int group_shift, int groups, unsigned char* codes,
+                                                                 __nv_bfloat16* scales) {
+  constexpr int kAt = 4;
+  next_launch_may_start();
+  wait_for_launch_before();
+  const int lane = lane_id();
+  const long long row = (long long)blockIdx.x * (kPackThreads / 32) + (threadIdx.x >> 5);
+  if (row >= n) return;
+  const int blocks = (d + kBlock - 1) / kBlock, words = 4 * blocks, span = 1 << group_shift;
+  const T* src = rows + row * row_stride + 8 * lane;
+  unsigned char* dst = codes + row * (16ll * blocks);
+  __nv_bfloat16* to_scales = scales + row * groups;
+  // where a lane's word is among 32 of whole fours, and whether it is the first of its group
+  const int at_lane = 64 * (lane >> 4) + 16 * (lane & 3) + 4 * ((lane >> 2) & 3);
+  const bool leads = (lane & (span - 1)) == 0;
+  auto pass = [&](int begin, auto all_whole) {
+    constexpr bool kWhole = decltype(all_whole)::value;
     T v[kAt][8];
+    bool whole[kAt];  // 32 whole words, of whole fours
 #pragma unroll
     for (int k = 0; k < kAt; ++k) {
-      const int w = kLong ? first + k * lanes : first;
-      if (row + (kLong ? 0 : k) < n && 8 * w < d) {
-        load_eight<T, N>(src + (kLong ? 0 : k * row_stride), 8 * w, d, v[k]);
-      } else {
+      const int first = begin + 32 * k;
+      whole[k] = kWhole || 8 * (first + 32) <= d;
+      if (whole[k]) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[k][i] = from_f32<T>(0.0f);
+        for (int i = 0; i < 8; i += N) {
+          T part[N];
+          load_many<T, N>(src + 8 * first + i, part);
+#pragma unroll
+          for (int j = 0; j < N; ++j) v[k][i + j] = part[j];
+        }
+      } else {
+        load_eight<T, N>(src + 8 * first, 0, d - 8 * (first + lane), v[k]);
       }
     }
     float most[kAt];
@@ -120,34 +188,34 @@ __global__ void __launch_bounds__(kPackThreads) pack_kernel(const T* rows, long 
       for (int k = 0; k < kAt; ++k) most[k] = fmaxf(most[k], __shfl_xor_sync(FULL, most[k], off));
     }
     unsigned word[kAt];
-    bool live[kAt], other = false;
+    bool other = false;
 #pragma unroll
     for (int k = 0; k < kAt; ++k) {
-      if (kLong && first - lane + k * lanes >= words) {  // (behind the row for the whole warp)
-        live[k] = false;
-        continue;
-      }
+      if (!kWhole && begin + 32 * k >= words) continue;  // (behind the row, for the whole warp)
       most[k] = __bfloat162float(scale_of(most[k]));
       word[k] = codes_of(v[k], most[k]);
-      live[k] = row + (kLong ? 0 : k) < n && (kLong ? first + k * lanes : first) < words;
-      other = other || (live[k] && !ordinary(most[k]));
+      other = other || ((kWhole || begin + 32 * k + lane < words) && !ordinary(most[k]));
     }
     if (other) {
 #pragma unroll
       for (int k = 0; k < kAt; ++k)
-        if (live[k] && !ordinary(most[k])) word[k] = codes_of_any(v[k], most[k]);
+        if (!ordinary(most[k])) word[k] = codes_of_any(v[k], most[k]);
     }
 #pragma unroll
     for (int k = 0; k < kAt; ++k) {
-      const int w = kLong ? first + k * lanes : first;
-      if (live[k]) {
-        *reinterpret_cast<unsigned*>(dst + (kLong ? 0 : k * (16ll * blocks)) + word_offset(w, blocks)) = word[k];
-        const int g = w >> group_shift;
-        if (g << group_shift == w && g < groups) to_scales[(kLong ? 0 : k * groups) + g] = __float2bfloat16_rn(most[k]);
+      const int w = begin + 32 * k + lane;
+      if (whole[k]) {
+        *reinterpret_cast<unsigned*>(dst + at_lane + 4 * (begin + 32 * k)) = word[k];
+        if (leads) to_scales[w >> group_shift] = __float2bfloat16_rn(most[k]);
+      } else if (w < words) {
+        *reinterpret_cast<unsigned*>(dst + word_offset(w, blocks)) = word[k];
+        if (leads && w >> group_shift < groups) to_scales[w >> group_shift] = __float2bfloat16_rn(most[k]);
       }
     }
-    if (!kLong) break;
-  }
+  };
+  int begin = 0;
+  for (; 8 * (begin + 32 * kAt) <= d; begin += 32 * kAt) pass(begin, std::true_type());
+  if (begin < words) pass(begin, std::false_type());
 }
 
 // Groups that are more than a warp's words: a warp per row, every group read twice.
@@ -235,12 +303,15 @@ cudaError_t pack_n(const T* rows, long long row_stride, long long n, int d, long
   int shift = 0;
   while ((1 << shift) < group_words) ++shift;
   const int teams = kPackThreads / lanes, groups = (int)((d + group - 1) / group);
-  // four rows or four words of a row at a time, unless that leaves SMs without work (1 183 514 rows of 50 floats 60 us, one at a
+  // four rows at a time, unless that leaves SMs without work (1 183 514 rows of 50 floats 60 us, one at a
   // time 73; 20 000 of 64 are 4.4 and 4.0)
   const bool longer = words > lanes, many = longer || n > (long long)4 * kSMs * teams;
   const long long per = longer || !many ? teams : 4 * teams, blocks = (n + per - 1) / per;
   if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
-  auto* kernel = longer ? pack_kernel<T, N, 4, true> : many ? pack_kernel<T, N, 4, false> : pack_kernel<T, N, 1, false>;
+  if (longer)  // (blocks of a warp per row)
+    return launch_early(pack_long_kernel<T, N>, dim3((unsigned)blocks), kPackThreads, 0, stream, rows, row_stride, n, d, shift,
+                        groups, c, s);
+  auto* kernel = many ? pack_kernel<T, N, 4> : pack_kernel<T, N, 1>;
   return launch_early(kernel, dim3((unsigned)blocks), kPackThreads, 0, stream, rows, row_stride, n, d, shift, groups, c, s, lanes);
 }
 
