@@ -377,16 +377,11 @@ struct ScoreShape {
   static constexpr int kSumPitch = kWarpRows + 1;
 };
 
-template <int Bytes>
-__device__ __forceinline__ void copy_async(unsigned to, const void* from) {
-  if constexpr (Bytes == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(Bytes) : "memory");
+__device__ __forceinline__ void copy_async(unsigned to, const void* from) {  // 16 bytes
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int Left>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(Left) : "memory"); }
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
 struct ScoreLayout {
   int queries;       // of a tile of columns: at most 8 * kTiles / parts
@@ -412,7 +407,7 @@ __device__ __forceinline__ void stage_queries(const Scores4Params& p, const Scor
     const bool whole = l.wide_queries && 8 * i + 8 <= left;
     if constexpr (Columns::kParts == 1) {
       if (later && whole) {
-        copy_async<16>((unsigned)__cvta_generic_to_shared(to + 8 * i), src + 8 * i);
+        copy_async((unsigned)__cvta_generic_to_shared(to + 8 * i), src + 8 * i);
         return;
       }
     }
@@ -617,7 +612,7 @@ __global__ void __launch_bounds__(32 * kMostScoreWarps, 1) scores_kernel(const _
         }
       }
       if (l.chunks > 1) {
-        copies_wait<0>();
+        copies_wait();
         __syncthreads();
         current ^= 1;
       }
@@ -673,7 +668,7 @@ __global__ void __launch_bounds__(32 * kMostScoreWarps, 1) scores_kernel(const _
       }
     }
   }
-  copies_wait<0>();
+  copies_wait();
 }
 
 template <class Columns, int kTiles, int kGroup>

@@ -41,13 +41,6 @@ struct WordOf<4> { using type = unsigned; };
 template <>
 struct WordOf<2> { using type = unsigned short; };
 
-// read once: the row is of no use to the next CTA of this SM
-template <class T, int N>
-__device__ __forceinline__ Vec<T, N> load_stream(const T* p) {
-  using W = typename WordOf<sizeof(T) * N>::type;
-  const W w = __ldcs(reinterpret_cast<const W*>(p));
-  return *reinterpret_cast<const Vec<T, N>*>(&w);
-}
 template <class T, int N>
 __device__ __forceinline__ Vec<T, N> load_vec(const T* p) {
   using W = typename WordOf<sizeof(T) * N>::type;
