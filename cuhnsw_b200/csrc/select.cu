@@ -135,6 +135,27 @@ struct Pool {
 constexpr int kPoolScores = 4096;
 constexpr int kWarps = kThreads / 32;
 
+// Words of 16 bytes moved down by W words of 4 bytes and, if `half`, 2 bytes more: what each leaves the lane above gives, and lane 31
+// the first word of the next 32 (`edges`: of 32 threads' words each).
+template <int W, int Words, int Bytes>
+__device__ __forceinline__ void move_words(uint4 (&word)[Words], bool half, const uint4* edges) {
+  constexpr int kTaken = W + (Bytes == 2 ? 1 : 0);  // words of 4 bytes that come from above
+#pragma unroll
+  for (int i = 0; i < Words; ++i) {
+    const uint4 edge = lane_id() == 31 ? edges[i * kWarps] : make_uint4(0, 0, 0, 0);
+    const unsigned last[4] = {edge.x, edge.y, edge.z, edge.w};
+    unsigned w[8] = {word[i].x, word[i].y, word[i].z, word[i].w};
+#pragma unroll
+    for (int k = 0; k < kTaken; ++k) {
+      const unsigned above = __shfl_down_sync(FULL, w[k], 1);
+      w[4 + k] = lane_id() == 31 ? last[k] : above;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = Bytes == 2 && half ? __funnelshift_r(w[k + W], w[k + W + 1], 16) : w[k + W];
+    word[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 __device__ __forceinline__ float exp2_of(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -142,7 +163,7 @@ __device__ __forceinline__ float exp2_of(float x) {
 }
 
 template <class T, int kEach>
-__global__ void __launch_bounds__(kThreads) piece_kernel(SelectParams p, int pieces, int piece, ScoreKey* best,
+__global__ void __launch_bounds__(kThreads, 4) piece_kernel(SelectParams p, int pieces, int piece, ScoreKey* best,
                                                          float2* norms) {
   constexpr int N = 16 / sizeof(T);
   __shared__ ScoreKey pool_keys[kPoolScores];
@@ -157,24 +178,66 @@ __global__ void __launch_bounds__(kThreads) piece_kernel(SelectParams p, int pie
   const long long row = blockIdx.y + (long long)blockIdx.z * 65535;
   if (row >= p.sequences * p.beams) return;
   const long long seq = row / p.beams, beam = row % p.beams;
-  // Pieces begin at 16-byte boundaries, wherever the row does: `skew` places before the row belong to none.
-  const T* of_row = static_cast<const T*>(p.scores) + seq * p.seq_stride + beam * p.beam_stride;
-  const int skew = (int)(reinterpret_cast<uintptr_t>(of_row) % 16 / sizeof(T));
-  const long long begin = (long long)blockIdx.x * piece - skew;  // of the row
-  const T* scores = of_row + begin;
-  const int low = begin < 0 ? (int)-begin : 0, held = (int)min((long long)piece, p.vocabulary - begin);
+  // Which scores a thread holds depends on their places in the row alone, not on where in memory the row begins: equal rows have
+  // equal sums to the last bit, and equal totals are ties.
+  constexpr int kWords = kEach / N;
+  const long long begin = (long long)blockIdx.x * piece;  // of the row
+  const T* scores = static_cast<const T*>(p.scores) + seq * p.seq_stride + beam * p.beam_stride + begin;
+  const int skew = (int)(reinterpret_cast<uintptr_t>(scores) % 16 / sizeof(T));  // (a piece is whole words)
+  const int held = (int)min((long long)piece, p.vocabulary - begin);
   if (threadIdx.x == 0) pool_count = hot_count = 0;
   float x[kEach];
+  if (skew == 0) {
 #pragma unroll
-  for (int i = 0; i < kEach; i += N) {
-    const int at = (i / N * kThreads + threadIdx.x) * N;
-    if (at >= low && at + N <= held) {
-      const Vec<T, N> v = load_vec<T, N>(scores + at);
+    for (int i = 0; i < kEach; i += N) {
+      const int at = (i / N * kThreads + threadIdx.x) * N;
+      if (at + N <= held) {
+        const Vec<T, N> v = load_vec<T, N>(scores + at);
 #pragma unroll
-      for (int j = 0; j < N; ++j) x[i + j] = to_f32(v.v[j]);
-    } else {
+        for (int j = 0; j < N; ++j) x[i + j] = to_f32(v.v[j]);
+      } else {
 #pragma unroll
-      for (int j = 0; j < N; ++j) x[i + j] = at + j >= low && at + j < held ? to_f32(scores[at + j]) : -INFINITY;
+        for (int j = 0; j < N; ++j) x[i + j] = at + j < held ? to_f32(scores[at + j]) : -INFINITY;
+      }
+    }
+  } else {
+    // Aligned words from `skew` places earlier on, then put in their places.  (Selection from 256 x 131 071 floats, caches cold: 58 us,
+    // with both words of each loaded 73; 256 x 131 072: 52.)
+    __shared__ uint4 edges[kWords * kWarps + 1];
+    const int least = begin > 0 ? -skew : 0, last = (int)min((long long)held + N, p.vocabulary - begin);  // of the row
+    auto load = [&](int at) {
+      Vec<T, N> v;
+      if (at >= least && at + N <= last) {
+        v = load_vec<T, N>(scores + at);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v.v[j] = at + j >= least && at + j < last ? scores[at + j] : from_f32<T>(0.0f);
+      }
+      return *reinterpret_cast<const uint4*>(&v);
+    };
+    uint4 word[kWords];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) word[i] = load((int)(i * kThreads + threadIdx.x) * N - skew);
+    if (threadIdx.x == 0) edges[kWords * kWarps] = load(kEach * kThreads - skew);
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) edges[i * kWarps + warp] = word[i];
+    }
+    __syncthreads();
+    const int bytes = skew * (int)sizeof(T);
+    const bool half = bytes & 2;
+    switch (bytes / 4) {
+      case 0: move_words<0, kWords, sizeof(T)>(word, half, edges + warp + 1); break;
+      case 1: move_words<1, kWords, sizeof(T)>(word, half, edges + warp + 1); break;
+      case 2: move_words<2, kWords, sizeof(T)>(word, half, edges + warp + 1); break;
+      default: move_words<3, kWords, sizeof(T)>(word, half, edges + warp + 1); break;
+    }
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      const Vec<T, N> v = *reinterpret_cast<const Vec<T, N>*>(&word[i]);
+      const int at = (int)(i * kThreads + threadIdx.x) * N;
+#pragma unroll
+      for (int j = 0; j < N; ++j) x[i * N + j] = at + j < held ? to_f32(v.v[j]) : -INFINITY;
     }
   }
   float top = -INFINITY;  // (a NaN is no candidate and does not count)
@@ -226,7 +289,7 @@ __global__ void __launch_bounds__(kThreads) piece_kernel(SelectParams p, int pie
     if (slots > kPoolScores) pool.make_room(p.keep, kPoolScores - kThreads, from);
     if (slot >= slots) continue;
     const int i = slot % kEach, at = (i / N * kThreads + hot[slot / kEach]) * N + i % N;
-    const float xi = at >= low && at < held ? to_f32(scores[at]) : -INFINITY;
+    const float xi = at < held ? to_f32(scores[at]) : -INFINITY;
     if (xi >= bound) {
       const ScoreKey k = score_key(xi, (unsigned)(begin + at));
       if (k >= from) pool.push(k);
@@ -361,9 +424,8 @@ SelectPlan select_plan(long long rows, long long vocabulary) {
   // search, 32 x 8 beams of 131 072 ids: 89 us, with pieces of 2048 127; 1 x 4 of 32 000: 27 us with 2048, 33 with 8192.)
   s.each = 32;
   while (s.each > 8 && rows * ((vocabulary + kThreads * s.each - 1) / (kThreads * s.each)) < 4 * kSMs) s.each /= 2;
-  const long long places = vocabulary + 7;  // and those before the row
-  s.pieces = (places + kThreads * s.each - 1) / (kThreads * s.each);
-  s.piece = (int)(((places + s.pieces - 1) / s.pieces + 7) / 8 * 8);
+  s.pieces = (vocabulary + kThreads * s.each - 1) / (kThreads * s.each);
+  s.piece = (int)(((vocabulary + s.pieces - 1) / s.pieces + 7) / 8 * 8);
   return s;
 }
 
