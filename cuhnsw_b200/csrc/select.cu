@@ -311,10 +311,23 @@ __global__ void __launch_bounds__(kThreads, 4) piece_kernel(SelectParams p, int 
 
 constexpr int kPoolTotals = 2048;
 
+__device__ __forceinline__ float score_at(const SelectParams& p, long long at) {
+  if (p.type == kF32) return static_cast<const float*>(p.scores)[at];
+  if (p.type == kF16) return to_f32(static_cast<const __half*>(p.scores)[at]);
+  return to_f32(static_cast<const __nv_bfloat16*>(p.scores)[at]);
+}
+
+// Whether different scores, raised by `offset`, may round to the same `total`.  They are no further apart than the doubles beside the
+// total, 2^-52 of it, and no closer than 2^-24 of the larger one: that is at most 2^-28 of the total.  (The rest is room for the
+// roundings of the difference.  Infinities and 0 beside an offset count as such.)
+__device__ __forceinline__ bool merged(double offset, double total) {
+  return offset != 0.0 && !(fabs(total - offset) * 0x1p27 > fabs(total));
+}
+
 // One CTA per sequence.  The lists of the pieces are in order: of their first totals the `keep`-th is a bound that as many
 // candidates reach, and from there on there are few.  Bound: latency, a chain of some ten steps.  (8 sequences of 4 beams over
 // 32 000 ids, 64 lists: 25 us for a whole step of a beam search, 42 if up to 256 candidates are put in order without a bound.)
-__global__ void __launch_bounds__(kThreads) sequence_kernel(SelectParams p, int pieces, const ScoreKey* best,
+__global__ void __launch_bounds__(kThreads) sequence_kernel(SelectParams p, int pieces, int piece, const ScoreKey* best,
                                                             const float2* norms) {
   extern __shared__ __align__(16) unsigned char smem[];
   TotalKey* pool_keys = reinterpret_cast<TotalKey*>(smem);
@@ -403,6 +416,48 @@ __global__ void __launch_bounds__(kThreads) sequence_kernel(SelectParams p, int 
   }
   pool.sort();
   const int found = min(pool_count, p.keep);
+  // A list has its piece's best scores.  What it lacks can only matter in totals equal to the last result's, of a beam whose
+  // offset gives different scores the same total: then the results of that total are looked for again, in the order of the places.
+  // (Found fewer than `keep`: the lists lack nothing.)
+  const bool one = (int)threadIdx.x < found;
+  const TotalKey own = one ? pool_keys[threadIdx.x] : TotalKey{0, 0};
+  const unsigned long long border = pool_keys[max(found - 1, 0)].total;
+  if (__syncthreads_or(one && found == p.keep && own.total == border && merged(offsets[own.place >> 32], ord2d(border)))) {
+    __shared__ unsigned masks[2][kWarps];
+    int taken = __syncthreads_count(one && own.total > border);  // of the results
+    for (long long base = 0; base < lists && taken < found; base += kThreads) {
+      // pieces that have such a total: their lists begin at or above it and do not end above it
+      const long long mine_list = base + threadIdx.x;
+      const bool has = mine_list < lists && total_key(mine_list, mine[mine_list * p.keep]).total >= border &&
+                       total_key(mine_list, mine[mine_list * p.keep + p.keep - 1]).total <= border;
+      const unsigned having = __ballot_sync(FULL, has);
+      if (lane == 0) masks[0][warp] = having;
+      __syncthreads();
+      for (int w = 0; w < kWarps; ++w) {
+        for (unsigned left = masks[0][w]; left && taken < found; left &= left - 1) {
+          const unsigned list = (unsigned)base + 32 * w + __ffs(left) - 1, beam = list / (unsigned)pieces;
+          const long long begin = (long long)(list % (unsigned)pieces) * piece, end = min(begin + piece, p.vocabulary);
+          const long long row = seq * p.seq_stride + beam * p.beam_stride;
+          for (long long at = begin; at < end && taken < found; at += kThreads) {
+            const long long v = at + threadIdx.x;
+            const float score = v < end ? score_at(p, row + v) : -INFINITY;
+            const bool same = score > -INFINITY && d2ord(offsets[beam] + (double)score) == border;
+            const unsigned all = __ballot_sync(FULL, same);
+            if (lane == 0) masks[1][warp] = all;
+            __syncthreads();
+            int before = taken + __popc(all & ((1u << lane) - 1));
+            for (int other = 0; other < kWarps; ++other) {
+              before += other < warp ? __popc(masks[1][other]) : 0;
+              taken += __popc(masks[1][other]);
+            }
+            if (same && before < found) pool_keys[before] = {border, (unsigned long long)beam << 32 | (unsigned)v};
+            __syncthreads();
+          }
+        }
+      }
+      __syncthreads();
+    }
+  }
   for (int i = threadIdx.x; i < p.keep; i += kThreads) {
     const TotalKey k = pool_keys[i];
     const long long at = seq * p.keep + i;
@@ -516,7 +571,8 @@ cudaError_t launch_select(const SelectParams& p, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   e = allow_smem<sequence_kernel>();
   if (e != cudaSuccess) return e;
-  return launch_early(sequence_kernel, dim3((unsigned)p.sequences), kThreads, smem, stream, p, (int)plan.pieces, best, norms);
+  return launch_early(sequence_kernel, dim3((unsigned)p.sequences), kThreads, smem, stream, p, (int)plan.pieces, plan.piece, best,
+                      norms);
 }
 
 cudaError_t launch_reorder(const ReorderState* states, int count, const int* beams_of, long long sequences,

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from cuhnsw_b200 import table
-from test_gpu_table import DEV, TYPES, gen, normal, plain_select
+from test_gpu_table import DEV, TYPES, check_select, gen, normal, plain_select
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +34,45 @@ def test_equal_beams_are_ties_wherever_their_rows_begin(dtype, v):
       assert torch.equal(totals, first) and torch.equal(totals[0], totals[1])
   exact = row.double() - torch.logsumexp(row.double(), 0)
   assert (first[0, 0].double() - exact.max()).abs() <= 2 ** -20 + 2 ** -24 * exact.max().abs()
+
+
+@pytest.mark.parametrize("offset", [-1e30, 1e30, float(torch.finfo(torch.float32).min), math.inf, -1e9])
+@pytest.mark.parametrize("b, v", [(1, 5), (1, 100), (3, 700), (1, 9000), (2, 40_003), (300, 40)])
+def test_totals_that_do_not_tell_scores_apart(offset, b, v):
+  """Where a beam's total is so large that a score changes nothing, its continuations are ties: the smaller ids come first."""
+  place = torch.arange(v, device=DEV)
+  for i, dtype in enumerate(TYPES.values()):
+    for row in (place / 8, -place / 8, normal(v + i, v), (place % 7 == 3) * 1.0, normal(v, v) * 1e-20):
+      scores = row.to(dtype).expand(2, b, v).clone()
+      scores[:, :, v // 2] = -math.inf
+      scores[1].masked_fill_(torch.rand((b, v), generator=gen(i), device=DEV) < 0.3, math.nan)
+      totals = torch.full((2, b), offset, device=DEV)
+      totals[1, b // 2] = -2e30  # one beam before or after the others
+      for keep in (1, 4, 37, 256):
+        # (every term is a double without rounding but for the total itself, which is the same rounding on both sides)
+        check_select(scores, totals, keep, False)
+
+
+def test_totals_that_tell_some_scores_apart():
+  """Beams of all kinds side by side, and scores close enough to 0 to vanish beside an ordinary total."""
+  g = gen(3)
+  tiny = 10.0 ** (-30 * torch.rand((3, 5, 3000), generator=g, device=DEV))
+  scores = torch.where(torch.rand(tiny.shape, generator=g, device=DEV) < 0.5, tiny, -tiny)
+  scores[0, 0, ::3] = 0.0
+  scores[0, 1, ::2] = -0.0
+  for totals in ([-20.0, -20.5, -20.0, -19.75, -20.0], [-20.0] * 5, [0.0, -0.0, 0.0, 0.0, 0.0], [-1e-9] * 5, [3.0, 1e30, -1e30, 1e30, -math.inf],
+                 [-1e8, -1e9, -1e8, -1e8, -1e9]):
+    for keep in (1, 5, 60, 256):
+      for dtype in TYPES.values():
+        at = torch.tensor(totals, device=DEV).expand(3, 5).contiguous()
+        check_select(scores.to(dtype), at, keep, False)
+        check_select(scores[:, :, :70].to(dtype), at, keep, False)  # (fewer continuations than results of some beams)
+  # steps that a total of 1e9 merges by the dozen, at every place of a long row
+  scores = (torch.randint(0, 1000, (1, 3, 50_000), generator=g, device=DEV) * 1e-9).float()
+  for totals in ([1e9, 1e9, 1e9], [1e6, 1e6 + 1, 1e6 + 1], [-30.0, -30.0, -30.0]):
+    for keep in (1, 7, 100, 256):
+      check_select(scores, torch.tensor([totals], device=DEV), keep, False)
+  # with the scores normalised too: the total is the beam's alone
+  scores = normal(5, 2, 3, 6000, dtype=torch.float16)
+  for keep in (1, 9, 256):
+    check_select(scores, torch.tensor([[1e30, 1e30, 1e25], [-1e30, -1e30, -1e30]], device=DEV), keep, True)
