@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(kNarrowThreads) narrow_kernel(const __grid_con
     float bias[kRowsPerLane];
 #pragma unroll
     for (int i = 0; i < kRowsPerLane; ++i)
-      bias[i] = p.bias && (whole || (unsigned)(g + 8 * i) < rows) ? __ldg(p.bias + row0 + g + 8 * i) : 0.0f;
+      bias[i] = p.bias && (whole || (unsigned)(g + 8 * i) < rows) ? p.bias[row0 + g + 8 * i] : 0.0f;
     float total[kRowTiles][kTiles][4];
 #pragma unroll
     for (int s = 0; s < kScales; ++s) {

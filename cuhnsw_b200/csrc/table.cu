@@ -12,7 +12,7 @@ namespace hnsw {
 namespace {
 
 __device__ __forceinline__ long long id_at(const void* ids, int ids64, long long t) {
-  return ids64 ? __ldg(static_cast<const long long*>(ids) + t) : (long long)__ldg(static_cast<const int*>(ids) + t);
+  return ids64 ? static_cast<const long long*>(ids)[t] : (long long)static_cast<const int*>(ids)[t];
 }
 
 // ---- lookup ---------------------------------------------------------------------------------------------------------

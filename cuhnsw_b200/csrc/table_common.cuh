@@ -106,7 +106,8 @@ cudaError_t allow_smem() {
 
 // A launch that may be set up while the one before it on the stream still runs: its kernel calls wait_for_launch_before() ahead of
 // everything that it reads or writes in common with what came before, and next_launch_may_start() as soon as the one after it may be
-// set up.  Saves one to two microseconds a launch.
+// set up.  Saves one to two microseconds a launch.  Such a kernel is alive while its inputs may still be written, so it reads them by
+// ordinary loads: read-only ones (__ldg, ld.global.nc) are for what does not change as long as a kernel lives.
 __device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void next_launch_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -1,6 +1,8 @@
 """The operators over a table of embeddings without a GPU: what the C ABI and the torch layer refuse, and the host's part of
 the beams' states."""
 import ctypes
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -141,3 +143,13 @@ def test_pieces_cover_a_state():
 @pytest.mark.skipif(has_gpu(), reason="checks the failure mode of a machine without a GPU")
 def test_fails_loudly_without_a_gpu():
   assert lookup() == -5 and pack() == -5 and select() == -5
+
+
+def test_kernels_that_start_early_read_by_ordinary_loads():
+  """Read-only loads are for data that nobody writes while the kernel lives, and these live before the launch ahead of them ends."""
+  csrc = Path(__file__).resolve().parent.parent / "cuhnsw_b200" / "csrc"
+  launchers = [f for f in csrc.glob("*.cu") if "launch_early(" in f.read_text()]
+  assert len(launchers) >= 4
+  for f in launchers + list(csrc.glob("table_common.cuh")) + list(csrc.glob("scores4.cuh")):
+    code = re.sub(r"//[^\n]*", "", f.read_text())
+    assert not re.search(r"__ldg\b|ld\.global(\.\w+)*\.nc|__restrict__|tex1Dfetch", code), f.name
