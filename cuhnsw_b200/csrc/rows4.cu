@@ -38,10 +38,18 @@ __device__ __forceinline__ void load_eight(const T* row, int dim, int d, T (&v)[
   }
 }
 
+// The larger one; NaN if one of them is.
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// (A NaN becomes its group's scale, and so NaN all that the group's codes stand for: they have no room for one.)
 template <class T>
 __device__ __forceinline__ float largest(const T (&v)[8], float most) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(to_f32(v[i])));
+  for (int i = 0; i < 8; ++i) most = max_or_nan(most, fabsf(to_f32(v[i])));
   return most;
 }
 
@@ -75,13 +83,15 @@ __device__ __forceinline__ unsigned codes_of(const T (&v)[8], float step) {
   return word;
 }
 
-// The same with no scale, or with one whose reciprocal is no ordinary number.
+// The same with no scale, or with one whose reciprocal is no ordinary number.  (Beside an infinite scale infinities keep their sign, 7
+// or -8 times the scale, and 0 times it is a NaN: what was finite is lost.)
 template <class T>
 __device__ __forceinline__ unsigned codes_of_any(const T (&v)[8], float step) {
   unsigned word = 0;
   for (int i = 0; i < 8; ++i) {
-    const float q = step > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(to_f32(v[i]), step)), -8.0f), 7.0f) : 0.0f;
-    word |= (unsigned)((int)q + 8) << nibble_shift(i);
+    const float x = to_f32(v[i]);
+    const float q = !(step > 0.0f) ? 0.0f : isinf(x) ? x : rintf(__fdiv_rn(x, step));
+    word |= (unsigned)((int)fminf(fmaxf(q, -8.0f), 7.0f) + 8) << nibble_shift(i);
   }
   return word;
 }
@@ -115,7 +125,7 @@ __global__ void __launch_bounds__(kPackThreads, 4) pack_kernel(const T* rows, lo
   for (int k = 0; k < kAt; ++k) most[k] = largest(v[k], 0.0f);
   for (int off = 1; off < span; off <<= 1) {
 #pragma unroll
-    for (int k = 0; k < kAt; ++k) most[k] = fmaxf(most[k], __shfl_xor_sync(FULL, most[k], off));
+    for (int k = 0; k < kAt; ++k) most[k] = max_or_nan(most[k], __shfl_xor_sync(FULL, most[k], off));
   }
   unsigned word[kAt];
   bool live[kAt], other = false;
@@ -185,7 +195,7 @@ __global__ void __launch_bounds__(kPackThreads) pack_long_kernel(const T* rows, 
     for (int k = 0; k < kAt; ++k) most[k] = largest(v[k], 0.0f);
     for (int off = 1; off < span; off <<= 1) {
 #pragma unroll
-      for (int k = 0; k < kAt; ++k) most[k] = fmaxf(most[k], __shfl_xor_sync(FULL, most[k], off));
+      for (int k = 0; k < kAt; ++k) most[k] = max_or_nan(most[k], __shfl_xor_sync(FULL, most[k], off));
     }
     unsigned word[kAt];
     bool other = false;
@@ -237,7 +247,7 @@ __global__ void __launch_bounds__(kPackThreads) pack_wide_kernel(const T* rows, 
       load_eight<T, N>(src, 8 * w, d, v);
       most = largest(v, most);
     }
-    for (int off = 1; off < 32; off <<= 1) most = fmaxf(most, __shfl_xor_sync(FULL, most, off));
+    for (int off = 1; off < 32; off <<= 1) most = max_or_nan(most, __shfl_xor_sync(FULL, most, off));
     const __nv_bfloat16 scale = scale_of(most);
     for (int w = first + lane; w < until; w += 32) {
       load_eight<T, N>(src, 8 * w, d, v);

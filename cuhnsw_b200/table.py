@@ -71,8 +71,9 @@ def lookup_grad(grad, ids, num_rows, scale=1.0, out=None, accumulate=False):
 
 
 def pack_rows(rows, group=64):
-  """``PackedRows`` of a float32, float16 or bfloat16 ``[num_rows, num_dims]`` tensor of finite values: a code of 4 bits per
-  value and a bfloat16 scale per ``group`` consecutive dimensions (32, 64 or a multiple of 128)."""
+  """``PackedRows`` of a float32, float16 or bfloat16 ``[num_rows, num_dims]`` tensor: a code of 4 bits per value and a
+  bfloat16 scale per ``group`` consecutive dimensions (32, 64 or a multiple of 128).  A group with a NaN becomes NaN altogether; in one
+  with an infinity the infinities stay and the rest becomes NaN."""
   codes, scales = _table.pack(rows, group)
   return PackedRows(codes, scales, rows.shape[1], group)
 

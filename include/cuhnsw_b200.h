@@ -210,7 +210,8 @@ int cuhnsw_lookup_grad_device(const void* d_grad, int64_t grad_stride, int32_t t
 /* Rows in 4 bits.  A value is (code - 8) * scale, with a code of 0..15 per value and a bfloat16 scale per `group` consecutive
  * dimensions (32, 64 or a multiple of 128; the last group of a row may be shorter):
  *   scale = bfloat16(largest magnitude of the group * fp32(1 / 7)),  code = round_half_even(value / scale) within -8..7, plus 8
- * (8 where the scale is 0).  Values have to be finite.
+ * (8 where the scale is 0).  A group with a value that is not finite is lost, and no other group: with a NaN its scale is NaN, and
+ * so are all its values; with an infinity its scale is infinite, infinities keep their sign and its finite values become NaN.
  * d_scales: num_rows x ceil(num_dims / group).  d_codes: num_rows x 16 * ceil(num_dims / 32) bytes, 16-byte aligned.  A
  * row's bytes are little-endian 32-bit words of eight codes; blocks of 32 dimensions lie in fours, the last of a row as many
  * as are left (m of them): word t*m + j of a four (t = 0..3) holds dimensions 8t..8t+7 of its block j, the even ones

@@ -76,3 +76,33 @@ def test_totals_that_tell_some_scores_apart():
   scores = normal(5, 2, 3, 6000, dtype=torch.float16)
   for keep in (1, 9, 256):
     check_select(scores, torch.tensor([[1e30, 1e30, 1e25], [-1e30, -1e30, -1e30]], device=DEV), keep, True)
+
+
+# -- 4 bits ----------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n, d, group", [(9, 32, 32), (20_000, 50, 32), (300, 200, 64), (8000, 256, 256), (40, 300, 512), (60, 700, 128),
+                                         (50, 2048, 128), (33, 1500, 512)])
+def test_what_is_not_finite_costs_its_group_alone(dtype, n, d, group):
+  rows = normal(d, n, d, dtype=TYPES[dtype])
+  groups = -(-d // group)
+  bad = torch.zeros((n, groups * group), dtype=torch.bool, device=DEV)
+  bad[:, :d] = torch.rand((n, d), generator=gen(1), device=DEV) < 1 / (4 * min(d, group))
+  bad[0, 0] = bad[n - 1, d - 1] = True
+  values = torch.tensor([math.nan, math.inf, -math.inf], device=DEV)[torch.randint(0, 3, (n, groups * group), generator=gen(2), device=DEV)]
+  values[0, 0] = math.nan
+  spoilt = torch.where(bad[:, :d], values[:, :d].to(rows.dtype), rows)
+  clean = torch.where(bad[:, :d], 0.0, rows)
+  got, want = table.pack_rows(spoilt, group), table.pack_rows(clean, group)
+  lost = bad.view(n, groups, group).any(2)
+  nan = (bad & values.isnan()).view(n, groups, group).any(2)
+  assert torch.equal(got.scales[~lost], want.scales[~lost])
+  assert got.scales[nan].isnan().all() and (got.scales[lost & ~nan] == math.inf).all()
+  out = got.unpack()
+  of = lambda mask: mask.repeat_interleave(group, 1)[:, :d]
+  expected = torch.where(of(nan), math.nan, torch.where(of(lost), torch.where(bad[:, :d], values[:, :d], math.nan), want.unpack()))
+  assert torch.equal(out.isnan(), expected.isnan()) and torch.equal(out.nan_to_num(1e30), expected.nan_to_num(1e30))
+  # no product of another row is touched
+  scores, fine = got.scores(rows[:3]), want.scores(rows[:3])
+  assert torch.equal(scores[:, ~lost.any(1)], fine[:, ~lost.any(1)]) and not scores[:, lost.any(1)].isfinite().any()
