@@ -10,10 +10,13 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
 #include <limits>
+#include <memory>
 #include <sstream>
 #include <stdexcept>
 #include <string>
@@ -66,6 +69,35 @@ at::Tensor tensor(PyObject* o, const char* name) {
   if (!is_tensor(o)) refuse(name, " must be a tensor");
   return unpacked(o);
 }
+
+bool has_tangent(const at::Tensor& t) { return t._fw_grad(0).defined(); }
+
+// The inputs of an operator without a derivative that one is asked of.  As of torch's own such operators: a tangent is refused
+// at the call; a gradient that is recorded is refused where it is asked for, by the results' backward pass.
+class Underived {
+ public:
+  Underived(const char* name, std::initializer_list<PyObject*> inputs) : name_(name) {
+    for (PyObject* o : inputs) add(o);
+  }
+  void add(PyObject* o) {
+    if (!is_tensor(o)) return;
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (has_tangent(t)) refuse(name_, " has no derivative: a tangent cannot pass through it");
+    if (c10::GradMode::is_enabled() && t.requires_grad()) inputs_.push_back(t);
+  }
+  bool any() const { return !inputs_.empty(); }
+  void mark(const at::Tensor& result) const {
+    using torch::autograd::NotImplemented;
+    if (inputs_.empty() || !torch::autograd::isDifferentiableType(result.scalar_type())) return;
+    const std::shared_ptr<NotImplemented> node(new NotImplemented(name_, torch::autograd::collect_next_edges(inputs_)),
+                                               torch::autograd::deleteNode);
+    torch::autograd::set_history(result, node);
+  }
+
+ private:
+  const char* name_;
+  std::vector<at::Tensor> inputs_;
+};
 
 int64_t integer(PyObject* o, const char* name) {
   const long long value = PyLong_AsLongLong(o);
@@ -212,7 +244,12 @@ PyObject* lookup(PyObject* const* args) {  // rows, ids, scale
   return THPVariable_Wrap(out);
 }
 
+PyObject* tangent(PyObject* const* args) {  // rows: whether they carry one
+  return PyBool_FromLong(is_tensor(args[0]) && has_tangent(THPVariable_Unpack(args[0])));
+}
+
 PyObject* lookup_grad(PyObject* const* args) {  // grad, ids, num_rows, scale, out or None, accumulate
+  const Underived underived("lookup_grad", {args[0]});
   const at::Tensor given = tensor(args[0], "grad");
   if (!given.is_cuda() || type_of(given) < 0) refuse("grad must be a float32, float16 or bfloat16 CUDA tensor");
   const at::Device device = given.device();
@@ -240,6 +277,7 @@ PyObject* lookup_grad(PyObject* const* args) {  // grad, ids, num_rows, scale, o
         out.size(0) != rows || out.size(1) != dims || !out.is_contiguous())
       refuse("out must be a dense [", rows, ", ", dims, "] tensor of ", grad.scalar_type(), " or float32 on ", device);
     if (out.requires_grad() && c10::GradMode::is_enabled()) refuse("out must not require a gradient");
+    if (underived.any()) refuse("out cannot be given for a grad that requires a gradient itself");
     if (out.is_neg()) refuse("out must not be a negated view");
     if (overlap(out, grad) || overlap(out, ids)) refuse("out must not overlap grad or the ids");
     out.unsafeGetTensorImpl()->bump_version();  // whoever keeps it for a backward pass learns that it has changed
@@ -252,6 +290,7 @@ PyObject* lookup_grad(PyObject* const* args) {  // grad, ids, num_rows, scale, o
                                        type_of(out), accumulate, space.mutable_data_ptr(), stream);
     });
   }
+  underived.mark(out);
   return THPVariable_Wrap(out);
 }
 
@@ -306,6 +345,7 @@ PyObject* check_packed(PyObject* const* args) {  // codes, scales, num_dims, gro
 }
 
 PyObject* unpack(PyObject* const* args) {  // codes, scales, num_dims, group, dtype
+  const Underived underived("PackedRows.unpack", {args[1]});
   const Packed p = packed_of(args);
   if (!THPDtype_Check(args[4])) refuse("dtype must be a torch.dtype");
   const at::ScalarType type = reinterpret_cast<THPDtype*>(args[4])->scalar_type;
@@ -315,6 +355,7 @@ PyObject* unpack(PyObject* const* args) {  // codes, scales, num_dims, group, dt
     return cuhnsw_unpack4_device(p.codes.const_data_ptr(), p.scales.const_data_ptr(), p.n, p.d, p.group,
                                  out.mutable_data_ptr(), type_of(out), stream);
   });
+  underived.mark(out);
   return THPVariable_Wrap(out);
 }
 
@@ -354,9 +395,12 @@ at::Tensor scores_of(const Packed& p, const Asked& asked, int64_t first, int64_t
 }
 
 PyObject* scores(PyObject* const* args) {  // codes, scales, num_dims, group, queries, bias or None
+  const Underived underived("PackedRows.scores", {args[1], args[4], args[5]});
   const Packed p = packed_of(args);
   const Asked asked = asked_of(p, args[4], args[5]);
-  return THPVariable_Wrap(scores_of(p, asked, 0, asked.queries.size(0)));
+  const at::Tensor out = scores_of(p, asked, 0, asked.queries.size(0));
+  underived.mark(out);
+  return THPVariable_Wrap(out);
 }
 
 // -- selection -----------------------------------------------------------------------------------------------------------
@@ -392,6 +436,7 @@ constexpr int64_t kSearchScores = 1ll << 30;  // scores of a search in memory at
 constexpr int64_t kSearchQueries = 32;        // but so many queries' at least
 
 PyObject* search(PyObject* const* args) {  // codes, scales, num_dims, group, queries, topk, bias or None
+  const Underived underived("PackedRows.search", {args[1], args[4], args[6]});
   const Packed p = packed_of(args);
   const int64_t topk = keep_of(integer(args[5], "topk"), "topk");
   const Asked asked = asked_of(p, args[4], args[6]);
@@ -410,10 +455,12 @@ PyObject* search(PyObject* const* args) {  // codes, scales, num_dims, group, qu
       select(all, p.n, p.n, some, 1, p.n, {}, topk, false, true, out, first);
     }
   }
+  underived.mark(out.totals);
   return tuple_of({out.ids, out.totals, out.found});
 }
 
 PyObject* select_beams(PyObject* const* args) {  // scores, totals or None, keep or None, log_softmax
+  const Underived underived("select_beams", {args[0], args[1]});
   const at::Tensor given = tensor(args[0], "scores");
   if (!given.is_cuda() || type_of(given) < 0) refuse("scores must be a float32, float16 or bfloat16 CUDA tensor");
   if (given.dim() != 3) refuse("scores must be [sequences, beams, vocabulary], not ", given.dim(), "-dimensional");
@@ -441,6 +488,7 @@ PyObject* select_beams(PyObject* const* args) {  // scores, totals or None, keep
     select(scores, scores.stride(0), scores.stride(1), sequences, beams, vocabulary, totals, keep, log_softmax, false, out,
            0);
   }
+  underived.mark(out.totals);
   return tuple_of({out.totals, out.beams, out.ids});
 }
 
@@ -483,6 +531,7 @@ PyObject* reorder(PyObject* const* args) {  // states, beams
   const at::Device device = beams.device();
   const int64_t sequences = beams.size(0), keep = beams.size(1);
   const Py_ssize_t count = several ? PySequence_Fast_GET_SIZE(args[0]) : 1;
+  std::vector<Underived> underived;
   std::vector<at::Tensor> inputs, outs;
   std::vector<cuhnsw_state> states;
   inputs.reserve(count);
@@ -491,6 +540,7 @@ PyObject* reorder(PyObject* const* args) {  // states, beams
   for (Py_ssize_t i = 0; i < count; ++i) {
     PyObject* o = several ? PySequence_Fast_GET_ITEM(args[0], i) : args[0];
     at::Tensor state;
+    underived.emplace_back("reorder", std::initializer_list<PyObject*>{o});
     if (is_tensor(o)) state = unpacked(o);
     if (!state.defined() || state.device() != device || state.dim() < 2)
       refuse("a state must be a tensor [sequences, beams, ...] on ", device);
@@ -517,6 +567,7 @@ PyObject* reorder(PyObject* const* args) {  // states, beams
       return cuhnsw_reorder_device(states.data(), (int32_t)count, beams.const_data_ptr<int32_t>(), sequences,
                                    inputs[0].size(1), keep, stream);
     });
+  for (Py_ssize_t i = 0; i < count; ++i) underived[i].mark(outs[i]);
   if (!several) return THPVariable_Wrap(outs[0]);
   PyObject* result = PyList_New(count);
   if (!result) throw std::bad_alloc();
@@ -533,9 +584,9 @@ PyObject* reorder(PyObject* const* args) {  // states, beams
       METH_FASTCALL, nullptr                                                             \
   }
 
-PyMethodDef kMethods[] = {FUNCTION(lookup, 3),  FUNCTION(lookup_grad, 6),  FUNCTION(pack, 2),         FUNCTION(check_packed, 4),
-                          FUNCTION(unpack, 5),  FUNCTION(scores, 6),       FUNCTION(search, 7),       FUNCTION(select_beams, 4),
-                          FUNCTION(pieces, 1),  FUNCTION(reorder, 2),      {nullptr, nullptr, 0, nullptr}};
+PyMethodDef kMethods[] = {FUNCTION(lookup, 3),  FUNCTION(tangent, 1),      FUNCTION(lookup_grad, 6),  FUNCTION(pack, 2),
+                          FUNCTION(check_packed, 4), FUNCTION(unpack, 5),  FUNCTION(scores, 6),       FUNCTION(search, 7),
+                          FUNCTION(select_beams, 4), FUNCTION(pieces, 1),  FUNCTION(reorder, 2),      {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_table", "The operators over a table of embeddings for torch tensors.",
                        -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

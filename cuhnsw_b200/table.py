@@ -11,7 +11,8 @@ next to the search:
 Everything is enqueued on torch's current stream of the tensors' device and not waited for.  Arguments that do not fit raise
 ``RuntimeError`` before anything is launched; contents (row numbers, beam numbers) are never read on the host, numbers outside
 the table stand for empty slots.  Captured into a CUDA graph, the calls allocate from the graph's pool, so that graphs do not share
-workspaces.  Only ``lookup`` is differentiable; the other results carry no gradient.
+workspaces.  Only ``lookup`` is differentiable.  The results of the others can be computed from tensors that require a gradient, but
+their backward pass raises ``RuntimeError``, as does a call with a forward-mode tangent; row numbers, and rows in 4 bits, are constants.
 
 The checks and the calls of the C ABI are compiled (csrc/table_torch.cpp).  No counterpart in the reference, which keeps its
 vectors on the host (cuhnsw/pyhnsw.py:48-58 there).
@@ -35,6 +36,7 @@ class _Lookup(torch.autograd.Function):
   @staticmethod
   def forward(ctx, rows, ids, scale):
     ctx.save_for_backward(ids)
+    ctx.save_for_forward(ids)
     ctx.num_rows, ctx.scale = rows.shape[0], scale
     return _table.lookup(rows, ids, scale)
 
@@ -44,15 +46,19 @@ class _Lookup(torch.autograd.Function):
     ids, = ctx.saved_tensors
     return _table.lookup_grad(grad, ids, ctx.num_rows, ctx.scale, None, False), None, None
 
+  @staticmethod
+  def jvp(ctx, rows, ids, scale):  # (the tangent of the rows; the others have none)
+    return _table.lookup(rows, *ctx.saved_tensors, ctx.scale)
+
 
 def lookup(rows, ids, scale=1.0):
   """``scale * rows[ids]``, rounded once to the rows' type: a tensor of ``ids.shape + (num_dims,)``.
 
   rows: float32, float16 or bfloat16 ``[num_rows, num_dims]``, rows any distance apart; ids: int32 or int64 of any shape.  An id
   outside ``0 .. num_rows-1`` gives zeros and gets no gradient: the -1 of an empty result slot of a search, or the padding of a
-  batch.  Differentiable in ``rows`` (once): see ``lookup_grad``.  The backward pass may be captured into a CUDA graph
+  batch.  Differentiable in ``rows`` (once, backward or forward): see ``lookup_grad``.  The backward pass may be captured into a CUDA graph
   as torch's own may: not while an eager graph of the same leaf lives, which torch answers with an error."""
-  if isinstance(rows, torch.Tensor) and rows.requires_grad and torch.is_grad_enabled():
+  if isinstance(rows, torch.Tensor) and (rows.requires_grad and torch.is_grad_enabled() or _table.tangent(rows)):
     return _Lookup.apply(rows, ids, scale)
   return _table.lookup(rows, ids, scale)
 

@@ -3,6 +3,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from cuhnsw_b200 import table
 from test_gpu_table import DEV, TYPES, check_select, gen, normal, plain_select
@@ -106,3 +107,63 @@ def test_what_is_not_finite_costs_its_group_alone(dtype, n, d, group):
   # no product of another row is touched
   scores, fine = got.scores(rows[:3]), want.scores(rows[:3])
   assert torch.equal(scores[:, ~lost.any(1)], fine[:, ~lost.any(1)]) and not scores[:, lost.any(1)].isfinite().any()
+
+
+# -- derivatives -----------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("recorded", [False, True])
+def test_a_tangent_passes_through_a_lookup(dtype, recorded):
+  rows = normal(1, 30, 12, dtype=TYPES[dtype]).requires_grad_(recorded)
+  tangent = normal(2, 30, 12, dtype=TYPES[dtype])
+  ids = torch.tensor([[3, -1, 29], [3, 30, 0]], device=DEV)
+  with forward_ad.dual_level():
+    for given in (rows, rows.t().contiguous().t()):
+      out, out_tangent = forward_ad.unpack_dual(table.lookup(forward_ad.make_dual(given, tangent), ids, -1.5))
+      assert torch.equal(out, table.lookup(rows.detach(), ids, -1.5)) and torch.equal(out_tangent, table.lookup(tangent, ids, -1.5))
+      assert out.requires_grad == recorded
+    assert forward_ad.unpack_dual(table.lookup(rows, ids)).tangent is None
+
+
+def underived(x):
+  """Results that depend on `x` [6, 32] through each operator without a derivative, by its name."""
+  rows = normal(1, 40, 32)
+  packed = table.pack_rows(rows, 32)
+  ids, beams = torch.arange(6, device=DEV), torch.tensor([[1, 0, -1], [0, 1, 1]], dtype=torch.int32, device=DEV)
+  with torch.no_grad():
+    scales = packed.scales.clone()
+  return {
+    "PackedRows.scores": lambda: [packed.scores(x), packed.scores(rows[:3], bias=x.reshape(-1)[:40])],
+    "PackedRows.search": lambda: [packed.search(x, 3)[1], packed.search(rows[:3], 3, bias=x.reshape(-1)[:40])[1]],
+    "PackedRows.unpack": lambda: [table.PackedRows(packed.codes, scales * x[0, 0].to(scales.dtype), 32, 32).unpack()],
+    "select_beams": lambda: [table.select_beams(x.view(2, 3, 32))[0], table.select_beams(rows[None, :6], x[:, 0].reshape(1, 6))[0]],
+    "reorder": lambda: [table.reorder(x.view(2, 3, 32), beams), table.reorder([ids.view(2, 3), x.view(2, 3, 4, 8)], beams)[1]],
+    "lookup_grad": lambda: [table.lookup_grad(x, ids, 9)],
+  }
+
+
+def test_derivatives_that_there_are_not_are_refused_where_they_are_asked_for():
+  x = normal(3, 6, 32)
+  plain = {name: call() for name, call in underived(x).items()}
+  x.requires_grad_()
+  for name, call in underived(x).items():
+    for out, want in zip(call(), plain[name]):
+      assert torch.equal(out, want) and out.requires_grad
+      with pytest.raises(RuntimeError, match=f"derivative for {name} is not implemented"):
+        (2 * out).sum().backward()
+    with torch.no_grad():
+      assert not any(out.requires_grad for out in call())
+  assert x.grad is None
+  nns, _, found = table.pack_rows(x, 32).search(x, 2)
+  _, beams, ids = table.select_beams(x[None])
+  assert not any(t.requires_grad for t in (nns, found, beams, ids, table.pack_rows(x, 32).scores(x.detach())))
+  assert not table.reorder([beams, x[None]], torch.zeros((1, 2), dtype=torch.int32, device=DEV))[0].requires_grad
+  with pytest.raises(RuntimeError, match="out cannot be given"):
+    table.lookup_grad(x, torch.arange(6, device=DEV), 9, out=torch.zeros((9, 32), device=DEV))
+  with torch.no_grad():
+    table.lookup_grad(x, torch.arange(6, device=DEV), 9, out=torch.zeros((9, 32), device=DEV))
+  with forward_ad.dual_level():
+    for name, call in underived(forward_ad.make_dual(x.detach(), torch.ones_like(x))).items():
+      with pytest.raises(RuntimeError, match=f"{name} has no derivative"):
+        call()
