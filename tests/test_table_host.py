@@ -1,7 +1,10 @@
 """The operators over a table of embeddings without a GPU: what the C ABI and the torch layer refuse, and the host's part of
 the beams' states."""
 import ctypes
+import importlib.util
 import re
+import subprocess
+import sys
 from pathlib import Path
 
 import pytest
@@ -10,6 +13,7 @@ import torch
 from conftest import has_gpu
 from cuhnsw_b200 import _table, cuhnsw_bind, table
 
+CSRC = Path(__file__).resolve().parent.parent / "cuhnsw_b200" / "csrc"
 INVALID = -1
 # addresses that are aligned but belong to nobody: a refused call must not touch them
 A, ODD = 0x10000, 0x10001
@@ -147,9 +151,27 @@ def test_fails_loudly_without_a_gpu():
 
 def test_kernels_that_start_early_read_by_ordinary_loads():
   """Read-only loads are for data that nobody writes while the kernel lives, and these live before the launch ahead of them ends."""
-  csrc = Path(__file__).resolve().parent.parent / "cuhnsw_b200" / "csrc"
-  launchers = [f for f in csrc.glob("*.cu") if "launch_early(" in f.read_text()]
+  launchers = [f for f in CSRC.glob("*.cu") if "launch_early(" in f.read_text()]
   assert len(launchers) >= 4
-  for f in launchers + list(csrc.glob("table_common.cuh")) + list(csrc.glob("scores4.cuh")):
+  for f in launchers + [CSRC / "table_common.cuh", CSRC / "scores4.cuh"]:
     code = re.sub(r"//[^\n]*", "", f.read_text())
     assert not re.search(r"__ldg\b|ld\.global(\.\w+)*\.nc|__restrict__|tex1Dfetch", code), f.name
+
+
+def test_the_library_builds_without_torch(tmp_path):
+  """Only the torch layer needs torch's headers."""
+  def wanted(python):
+    done = subprocess.run(["make", "-n", "-B", "-C", str(CSRC), f"PYTHON={python}"], capture_output=True, text=True, timeout=60)
+    assert done.returncode == 0, done.stderr
+    return done.stdout
+
+  without = tmp_path / "python"
+  without.write_text(f'#!/bin/sh\nexec {sys.executable} -S "$@"\n')  # (no installed packages)
+  without.chmod(0o755)
+  alone = wanted(without)
+  assert "libcuhnsw_b200.so" in alone and "table.cu" in alone
+  assert "table_torch" not in alone and "-o ../_table.so" not in alone and "_table.so, which only" in alone
+  nothing = wanted("/nonexistent/python")
+  assert "libcuhnsw_b200.so" in nothing and "table_torch" not in nothing
+  if importlib.util.find_spec("torch"):
+    assert "table_torch.cpp" in wanted(sys.executable)
