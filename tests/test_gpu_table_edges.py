@@ -6,7 +6,7 @@ import torch
 from torch.autograd import forward_ad
 
 from cuhnsw_b200 import table
-from test_gpu_table import DEV, TYPES, check_select, gen, normal, plain_select
+from test_gpu_table import DEV, TYPES, check_select, gen, ids_of, normal, plain_codes, plain_pack, plain_select
 
 pytestmark = pytest.mark.gpu
 
@@ -107,6 +107,147 @@ def test_what_is_not_finite_costs_its_group_alone(dtype, n, d, group):
   # no product of another row is touched
   scores, fine = got.scores(rows[:3]), want.scores(rows[:3])
   assert torch.equal(scores[:, ~lost.any(1)], fine[:, ~lost.any(1)]) and not scores[:, lost.any(1)].isfinite().any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [249, 250, 256])
+def test_pack_with_a_group_that_is_a_row(dtype, d):
+  rows = normal(d, 6001, d, dtype=TYPES[dtype])  # (rows of 32 words, four at a time)
+  rows[5, :] = 0
+  packed = table.pack_rows(rows, 256)
+  codes, scales = plain_pack(rows, 256)
+  assert torch.equal(packed.scales, scales) and torch.equal(plain_codes(packed), codes.double())
+  assert torch.equal(packed.unpack(), codes * scales.float())
+
+
+def packed_of(seed, n, d, group, values=range(-8, 8)):
+  """(packed rows with scales that are powers of two, the values that they stand for)"""
+  codes = torch.randint(0, len(values), (n, -(-d // 32) * 32), generator=gen(seed), device=DEV)
+  codes = torch.tensor(list(values), device=DEV)[codes] + 8
+  word, nibble = places(d)
+  raw = torch.zeros((n, codes.shape[1] // 8), dtype=torch.int64, device=DEV)  # words of eight codes
+  raw.index_add_(1, word, codes << nibble)
+  raw = torch.where(raw >= 1 << 31, raw - (1 << 32), raw).to(torch.int32)
+  scales = 2.0 ** torch.randint(0, 4, (n, -(-d // group)), generator=gen(seed + 1), device=DEV)
+  rows = table.PackedRows(raw.view(torch.uint8), scales.bfloat16(), d, group)
+  return rows, (codes[:, :d] - 8).double() * scales.double().repeat_interleave(group, 1)[:, :d]
+
+
+def places(d):
+  """Of every dimension (and those behind the last one in its block): its word in a row and the bit that its code begins at."""
+  dims = torch.arange(-(-d // 32) * 32, device=DEV)
+  block, four = dims // 32, dims // 128
+  m = torch.clamp(len(dims) // 32 - 4 * four, max=4)
+  t, j, k = dims % 32 // 8, block - 4 * four, dims % 8
+  return 16 * four + t * m + j, 4 * (k // 2 + 4 * (k % 2))
+
+
+SCORES = [(1, 129, 32), (15, 130, 64), (300, 257, 128), (64, 512, 256), (2000, 960, 128), (70, 1030, 384), (40, 4100, 1024), (5000, 200, 32),
+          (48, 8192, 64), (3, 20_000, 128), (2100, 16_500, 64), (17_000, 300, 32), (40_000, 260, 64), (3000, 5000, 32), (9000, 5000, 128)]
+
+
+@pytest.mark.parametrize("n, d, group", SCORES + [(100, 50, 32), (33, 128, 128), (31, 96, 64)])
+def test_fp32_queries_enter_with_all_their_bits(n, d, group):
+  """A query of one whole number of 24 bits: each of its parts, and their sum, is exact, and so is the product with 0 and powers of two."""
+  packed, rows = packed_of(n, n, d, group, (-8, -4, -2, -1, 0, 1, 2, 4))
+  for nq in (1, 7, 8, 9, 20):
+    dims = torch.randint(0, d, (nq,), generator=gen(nq), device=DEV)
+    dims[0], dims[-1] = d - 1, d // 2
+    number = torch.randint(1 << 22, 1 << 23, (nq,), generator=gen(nq + 1), device=DEV) * 2 + 1
+    queries = torch.zeros((nq, d), device=DEV)
+    queries[torch.arange(nq, device=DEV), dims] = torch.where(number % 3 == 0, -number, number).float()
+    want = queries[torch.arange(nq, device=DEV), dims].double()[:, None] * rows[:, dims].t()
+    assert torch.equal(packed.scores(queries).double(), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n, d, group", SCORES + [(100, 50, 32)])
+def test_scores_of_whole_numbers_are_exact(dtype, n, d, group):
+  """Every sum is a whole number below 2^24, in whatever order: nothing may be missing or counted twice."""
+  packed, rows = packed_of(n, n, d, group)
+  most = min(100, ((1 << 24) - 200) // (64 * d))
+  for nq in (1, 5, 8, 17, 33):
+    queries = torch.randint(-most, most + 1, (nq, d), generator=gen(nq), device=DEV).to(TYPES[dtype])
+    bias = torch.randint(-100, 101, (n,), generator=gen(3), device=DEV).float() if nq % 2 else None
+    want = queries.double() @ rows.t() + (0 if bias is None else bias.double())
+    assert torch.equal(packed.scores(queries, bias).double(), want)
+
+
+def test_scores_and_searches_beyond_32_bits():
+  n = 70_000_000
+  codes = torch.randint(0, 256, (n, 16), generator=gen(1), device=DEV, dtype=torch.uint8)
+  packed = table.PackedRows(codes, torch.ones((n, 1), dtype=torch.bfloat16, device=DEV), 32, 32)
+  queries = torch.randint(-3, 4, (32, 32), generator=gen(2), device=DEV).float()
+  scores = packed.scores(queries)  # 2.2 G scores
+  for first in (0, 67_108_860, n - 1000):
+    part = table.PackedRows(codes[first:first + 1000], packed.scales[first:first + 1000], 32, 32)
+    assert torch.equal(scores[:, first:first + 1000].double(), queries.double() @ part.unpack().double().t())
+  nns, distances, found = packed.search(queries, 5)
+  assert (found == 5).all()
+  for q in (0, 30, 31):
+    best = scores[q].topk(5).values
+    assert torch.equal(-distances[q], best) and torch.equal(scores[q][nns[q].long()], best)
+    for value in best.unique():  # the first places of each
+      mine = nns[q][best == value].long()
+      assert torch.equal(mine, (scores[q] == value).nonzero().view(-1)[:len(mine)])
+  del scores, codes, packed
+  n, d = 2_200_000, 4096  # 4.5 GB of codes
+  codes = torch.randint(0, 256, (n, d // 2), generator=gen(3), device=DEV, dtype=torch.uint8)
+  packed = table.PackedRows(codes, torch.ones((n, d // 128), dtype=torch.bfloat16, device=DEV), d, 128)
+  for dtype in (torch.float32, torch.bfloat16):
+    queries = torch.randint(-9, 10, (3, d), generator=gen(4), device=DEV).to(dtype)
+    scores = packed.scores(queries)
+    for first in (0, 1_048_570, 2_097_150, n - 100):
+      part = table.PackedRows(codes[first:first + 100], packed.scales[first:first + 100], d, 128)
+      assert torch.equal(scores[:, first:first + 100].double(), queries.double() @ part.unpack().double().t())
+
+
+def test_packing_beyond_32_bits():
+  n, d = 600_000, 4096  # 2.5 G values
+  rows = torch.randn((n, d), dtype=torch.bfloat16, generator=gen(1), device=DEV)
+  for group in (128, 512):
+    packed = table.pack_rows(rows, group)
+    out = packed.unpack(torch.bfloat16)
+    for first in (0, 524_280, n - 16):
+      part = table.pack_rows(rows[first:first + 16], group)
+      assert torch.equal(packed.codes[first:first + 16], part.codes) and torch.equal(packed.scales[first:first + 16], part.scales)
+      assert torch.equal(out[first:first + 16], part.unpack(torch.bfloat16))
+    del packed, out
+
+
+# -- gradient --------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype, out_type", [("f32", "f32"), ("bf16", "f32"), ("f16", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("count, n, d, kind", [
+  (2, 1, 1, "one"), (65, 1000, 96, "any"), (512, 5000, 500, "one"), (512, 5001, 100, "zipf"), (1025, 2, 257, "uniform"), (5000, 4097, 100, "zipf"),
+  (6144, 3, 33, "uniform"), (6145, 3, 33, "uniform"), (16_385, 70_000, 48, "any"), (20_000, 3, 2049, "any"), (40_961, 100_000, 8, "uniform"),
+  (50_000, 255, 66, "one"), (64_000, 9, 130, "blocks"), (120_003, 131_072, 40, "zipf"), (300_000, 5, 17, "uniform"), (1_000_000, 20, 7, "blocks")])
+def test_gradients_of_whole_numbers_are_exact(dtype, out_type, count, n, d, kind):
+  """Every sum is a whole number below 2^24, in whatever order: no token and no partial sum may be missing or counted twice."""
+  if kind == "blocks":  # a few long rows, one after another, of which none ends where a chunk does
+    ids = torch.arange(count, device=DEV) * n // (count + 3)
+  else:
+    ids = ids_of(count, count, n, kind)
+  grad = torch.randint(-8, 9, (count, d), generator=gen(count), device=DEV).to(TYPES[dtype])
+  there = (ids >= 0) & (ids < n)
+  sums = torch.zeros((n, d), dtype=torch.float64, device=DEV).index_add_(0, ids.clamp(0, n - 1), grad.double() * there[:, None])
+  out = torch.full((n, d), math.nan, dtype=TYPES[out_type], device=DEV)
+  assert torch.equal(table.lookup_grad(grad, ids, n, 0.25, out=out), (sums * 0.25).to(out.dtype))
+  before = torch.randint(-100, 101, (n, d), generator=gen(1), device=DEV).to(out.dtype)
+  added = table.lookup_grad(grad, ids, n, -2.0, out=before.clone(), accumulate=True)
+  assert torch.equal(added, (before.double() - 2 * sums).to(out.dtype))
+
+
+def test_gradients_beyond_32_bits():
+  count, n, d = 600_000, 560_000, 4096  # 2.5 G values, and 2.3 G of the table
+  grad = torch.randint(-8, 9, (count, d), generator=gen(1), device=DEV, dtype=torch.int8).to(torch.bfloat16)
+  ids = ids_of(2, count, n, "uniform", torch.int32)
+  ids[1000:200_000:7] = n - 1
+  out = table.lookup_grad(grad, ids, n)
+  for c in (0, 1, 2047, d - 1):
+    sums = torch.zeros(n, dtype=torch.float64, device=DEV).index_add_(0, ids, grad[:, c].double())
+    assert torch.equal(out[:, c], sums.to(torch.bfloat16))
 
 
 # -- derivatives -----------------------------------------------------------------------------------------------------
