@@ -701,27 +701,25 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(LookupGradParams 
 
 // ---- gradient: few tokens -------------------------------------------------------------------------------------------
 
-// Few tokens of a small table: one launch without a sort of all.  A CTA has kFewBytes of the result: it writes zeros, looks for its
+// Few tokens: one launch without a sort of all.  A CTA has kFewBytes of the result: it writes zeros, looks for its
 // rows among all ids, puts their tokens in order and writes the sums over the zeros.  Bound: latency.
-constexpr int kFewTokens = 512;
+constexpr int kFewTokens = 128;
 constexpr int kFewBytes = 16 * 1024;
 constexpr int kFewThreads = 256;
 constexpr int kFewAlone = 16;  // tokens of a row that one group of lanes adds up by itself
 constexpr int kFewLoads = 8;   // in flight per thread
 
-// Where that is better: rows short enough for a CTA to add up the most frequent one, zeros that do not take longer than the sort
-// would, and tokens that find many CTAs or are very few.  (511 tokens: 32 000 rows of 256 floats 12 us on the GPU, sorted 20;
-// 1 000 000 rows of 256, 1 GB, 176 and 150; 1000 rows of 8, two CTAs, 20 and 20.  512 tokens of two rows of 1024: 107 and 39.)
+// Where that is better: few tokens, in rows short enough for a CTA to add up the most frequent one.  (Caches cold, 128 tokens of
+// 32 000 rows of 256 floats 12 us, sorted 15, all of one row 16 and 17; of 1 000 000 rows 141 and 144; 256 frequent ones of 4000 rows
+// 20 and 15.  128 tokens of one row of 4096 bytes, 16 000 rows: 35 and 24.)
 bool few(const LookupGradParams& p, long long row_bytes) {
-  const long long bytes = p.n * row_bytes;
-  return !p.accumulate && p.tokens <= kFewTokens && row_bytes <= 2048 && bytes <= (64 << 20) &&
-         (p.tokens <= 32 || bytes >= (long long)kSMs * kFewBytes);
+  return !p.accumulate && p.tokens <= kFewTokens && row_bytes <= 2048;
 }
 
 template <class G, class O, int N>
 __global__ void __launch_bounds__(kFewThreads) few_kernel(LookupGradParams p, int rows_each, int lanes) {
-  __shared__ unsigned masks[kFewTokens / 32];
-  __shared__ unsigned short row_of[kFewTokens], list_row[kFewTokens], list_token[kFewTokens];
+  __shared__ unsigned masks[kFewThreads / 32];
+  __shared__ unsigned short list_row[kFewTokens], list_token[kFewTokens];
   __shared__ unsigned short sorted_row[kFewTokens], sorted_token[kFewTokens], long_rows[kFewTokens / kFewAlone];
   __shared__ int long_count;
   __shared__ __align__(16) float partial[kFewThreads * N];
@@ -737,39 +735,33 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(LookupGradParams p, in
     if ((int)threadIdx.x < head) to[threadIdx.x] = 0;
     if ((int)threadIdx.x < tail) to[head + 16 * words + threadIdx.x] = 0;
   }
-  bool any = false;
   if (threadIdx.x == 0) long_count = 0;
-  for (int base = 0; base < tokens; base += kFewThreads) {
-    const int t = base + threadIdx.x;
-    const long long id = t < tokens ? id_at(p.ids, p.ids64, t) : -1;
-    const bool mine = id >= row0 && id < row0 + rows;
-    const unsigned mask = __ballot_sync(FULL, mine);
-    if (lane_id() == 0) masks[t / 32] = mask;
-    if (mine) row_of[t] = (unsigned short)(id - row0);
-    any = any || mine;
-  }
-  if (!__syncthreads_or(any)) return;
+  static_assert(kFewTokens <= kFewThreads, "a token per thread");
+  const int t = threadIdx.x;
+  const long long id = t < tokens ? id_at(p.ids, p.ids64, t) : -1;
+  const bool mine = id >= row0 && id < row0 + rows;
+  const unsigned mask = __ballot_sync(FULL, mine);
+  if (lane_id() == 0) masks[t / 32] = mask;
+  if (!__syncthreads_or(mine)) return;
   // the tokens of its rows in their order, then by row
   int count = 0;
-  for (int base = 0; base < tokens; base += kFewThreads) {
-    const int t = base + threadIdx.x, word = t / 32;
-    int before = count;
-    for (int w = base / 32; w < word; ++w) before += __popc(masks[w]);
-    if (masks[word] >> (t & 31) & 1) {
-      const int at = before + __popc(masks[word] & ((1u << (t & 31)) - 1));
-      list_row[at] = row_of[t];
+#pragma unroll
+  for (int w = 0; w < kFewThreads / 32; ++w) {
+    if (mine && w == t / 32) {
+      const int at = count + __popc(mask & ((1u << (t & 31)) - 1));
+      list_row[at] = (unsigned short)(id - row0);
       list_token[at] = (unsigned short)t;
     }
-    for (int w = base / 32; w < (base + kFewThreads) / 32; ++w) count += __popc(masks[w]);
+    count += __popc(masks[w]);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < count; i += kFewThreads) {
-    const int row = list_row[i];
+  if (t < count) {
+    const int row = list_row[t];
     int rank = 0;
 #pragma unroll 8
-    for (int j = 0; j < count; ++j) rank += list_row[j] < row || (list_row[j] == row && j < i);
+    for (int j = 0; j < count; ++j) rank += list_row[j] < row || (list_row[j] == row && j < t);
     sorted_row[rank] = (unsigned short)row;
-    sorted_token[rank] = list_token[i];
+    sorted_token[rank] = list_token[t];
   }
   __syncthreads();
   const int group = threadIdx.x / lanes, lane = threadIdx.x % lanes, groups = kFewThreads / lanes;
@@ -809,10 +801,7 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(LookupGradParams p, in
   // rows of more tokens: a share for each group
   for (int i = 0; i < long_count; ++i) {
     const int s = long_rows[i], row = sorted_row[s];
-    int length = 0;
-    for (int base = s; base < count; base += kFewThreads)
-      length += __syncthreads_count(base + (int)threadIdx.x < count &&
-                                    sorted_row[min(base + (int)threadIdx.x, count - 1)] == row);
+    const int length = __syncthreads_count(s + t < count && sorted_row[min(s + t, count - 1)] == row);
     const int share = (length + groups - 1) / groups, from = min(length, group * share), to = min(length, from + share);
     for (int base = 0; base < d; base += lanes * N) {
       const int c = base + lane * N;

@@ -239,6 +239,15 @@ def test_gradients_of_whole_numbers_are_exact(dtype, out_type, count, n, d, kind
   assert torch.equal(added, (before.double() - 2 * sums).to(out.dtype))
 
 
+@pytest.mark.parametrize("dtype, out_type", [("f32", "f32"), ("bf16", "f32"), ("f16", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("count, n, d, kind", [
+  (1, 2_000_000, 30, "one"), (17, 1, 1, "one"), (64, 60_000, 24, "zipf"), (65, 20_000, 1, "zipf"), (96, 3, 511, "uniform"), (100, 100_000, 50, "ascending"),
+  (127, 300_000, 9, "empty"), (128, 5000, 500, "one"), (128, 5001, 512, "any"), (128, 1_000_003, 16, "any"), (128, 2_000_000, 100, "uniform"),
+  (128, 40, 1024, "zipf"), (128, 2, 300, "blocks"), (129, 5001, 300, "zipf"), (129, 2, 7, "blocks")])
+def test_gradients_of_few_whole_numbers_are_exact(dtype, out_type, count, n, d, kind):
+  test_gradients_of_whole_numbers_are_exact(dtype, out_type, count, n, d, kind)
+
+
 def test_gradients_beyond_32_bits():
   count, n, d = 600_000, 560_000, 4096  # 2.5 G values, and 2.3 G of the table
   grad = torch.randint(-8, 9, (count, d), generator=gen(1), device=DEV, dtype=torch.int8).to(torch.bfloat16)
