@@ -81,9 +81,11 @@ struct ColumnsF32 {
   using In = float;
   using Pairs = PairsBF16;
   static constexpr int kParts = 3;
-  // x = high + middle + low but for 2^-24 of it: each part is what the ones before leave, rounded to 8 bits
+  static constexpr float kLargest = 0x1.fep127f;  // of bfloat16
+  // x = high + middle + low: each part is what the ones before leave, rounded to 8 bits (below 2^-110 the last bits are lost)
   static __device__ __forceinline__ unsigned short part(float x, int which) {
-    const __nv_bfloat16 high = __float2bfloat16_rn(x);
+    // (the largest numbers would round to infinity)
+    const __nv_bfloat16 high = __float2bfloat16_rn(isfinite(x) ? fminf(fmaxf(x, -kLargest), kLargest) : x);
     if (which == 0) return __bfloat16_as_ushort(high);
     // (an infinity or NaN is all in the first part: its remainder would be a NaN)
     const float rest = isfinite(__bfloat162float(high)) ? x - __bfloat162float(high) : 0.0f;

@@ -224,7 +224,7 @@ int cuhnsw_unpack4_device(const void* d_codes, const void* d_scales, int64_t num
                           void* d_out, int32_t type, void* cuda_stream);
 /* d_out[q, r] = sum over the dimensions of query q times row r, plus d_bias[r] (fp32, may be NULL).  d_queries:
  * num_queries rows of num_dims values of `type`, query_stride values apart; d_out: num_queries x num_rows fp32, dense.
- * fp32 queries enter with their 24 bits. */
+ * fp32 queries enter with their 24 bits (of magnitudes from 2^-110 on; of smaller ones with those from 2^-133 on). */
 int cuhnsw_scores4_device(const void* d_codes, const void* d_scales, int64_t num_rows, int64_t num_dims, int64_t group,
                           const void* d_queries, int64_t query_stride, int32_t type, int64_t num_queries,
                           const float* d_bias, float* d_out, void* cuda_stream);

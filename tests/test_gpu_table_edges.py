@@ -160,6 +160,25 @@ def test_fp32_queries_enter_with_all_their_bits(n, d, group):
     assert torch.equal(packed.scores(queries).double(), want)
 
 
+@pytest.mark.parametrize("n, d", [(40, 1), (40, 100), (500, 200), (20_000, 300), (100, 5000)])
+def test_the_largest_and_smallest_fp32_queries(n, d):
+  packed, rows = packed_of(n, n, d, 32, (-1, 0, 1))
+  packed = table.PackedRows(packed.codes, torch.ones_like(packed.scales), d, 32)
+  rows = rows.sign()
+  top, least = torch.finfo(torch.float32).max, 2.0 ** -110
+  numbers = [top, -top, 3.396e38, 3.39617e38, 3.3962e38, 3.3895e38, least, least * (1 + 2 ** -23), -least * (2 - 2 ** -23), 2.0 ** -133]
+  queries = torch.zeros((len(numbers), d), device=DEV)
+  queries[:, d - 1] = torch.tensor(numbers, device=DEV)
+  want = queries[:, d - 1:].double() * rows[:, d - 1]
+  assert torch.equal(packed.scores(queries).double(), want)
+  for other in (math.inf, -math.inf, math.nan):
+    queries[0, d - 1] = other
+    scores = packed.scores(queries)
+    # (times 0 it is a NaN)
+    assert torch.equal(scores[0].isinf(), (rows[:, d - 1] != 0) & math.isinf(other)) and not scores[0].isfinite().any()
+    assert torch.equal(scores[1:].double(), want[1:])
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n, d, group", SCORES + [(100, 50, 32)])
 def test_scores_of_whole_numbers_are_exact(dtype, n, d, group):
