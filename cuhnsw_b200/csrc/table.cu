@@ -703,23 +703,29 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(LookupGradParams 
 
 // Few tokens: one launch without a sort of all.  A CTA has kFewBytes of the result: it writes zeros, looks for its
 // rows among all ids, puts their tokens in order and writes the sums over the zeros.  Bound: latency.
-constexpr int kFewTokens = 128;
+constexpr int kFewTokens = 512;
 constexpr int kFewBytes = 16 * 1024;
 constexpr int kFewThreads = 256;
 constexpr int kFewAlone = 16;  // tokens of a row that one group of lanes adds up by itself
 constexpr int kFewLoads = 8;   // in flight per thread
 
-// Where that is better: few tokens, in rows short enough for a CTA to add up the most frequent one.  (Caches cold, 128 tokens of
-// 32 000 rows of 256 floats 12 us, sorted 15, all of one row 16 and 17; of 1 000 000 rows 141 and 144; 256 frequent ones of 4000 rows
-// 20 and 15.  128 tokens of one row of 4096 bytes, 16 000 rows: 35 and 24.)
+// Where that is better: rows short enough for a CTA to add up the most frequent one, and very few tokens, or ones that find many CTAs
+// and zeros that do not take longer than the sort would.  (Caches cold.  128 tokens: 1000 rows of 8 floats 10 us, sorted 15; 32 000 of
+// 256 13 and 17; 524 288 of 256 78 and 83; one row of 4096 bytes of 16 000 35 and 24.  511 tokens: 1000 rows of 8 29 and 15; 8000 of 256 12
+// and 17; 32 000 16 and 17; 524 288 96 and 85.  It loses where many tokens are of rows next to each other: 511 of 32 000 rows
+// with the frequent ones in front 25 and 17.)
+constexpr int kFewAnywhere = 128;  // tokens
 bool few(const LookupGradParams& p, long long row_bytes) {
-  return !p.accumulate && p.tokens <= kFewTokens && row_bytes <= 2048;
+  const long long bytes = p.n * row_bytes;
+  return !p.accumulate && row_bytes <= 2048 &&
+         (p.tokens <= kFewAnywhere ||
+          (p.tokens <= kFewTokens && bytes <= (64 << 20) && bytes >= (long long)kSMs * kFewBytes));
 }
 
 template <class G, class O, int N>
 __global__ void __launch_bounds__(kFewThreads) few_kernel(LookupGradParams p, int rows_each, int lanes) {
-  __shared__ unsigned masks[kFewThreads / 32];
-  __shared__ unsigned short list_row[kFewTokens], list_token[kFewTokens];
+  __shared__ unsigned masks[kFewTokens / 32];
+  __shared__ unsigned short row_of[kFewTokens], list_row[kFewTokens], list_token[kFewTokens];
   __shared__ unsigned short sorted_row[kFewTokens], sorted_token[kFewTokens], long_rows[kFewTokens / kFewAlone];
   __shared__ int long_count;
   __shared__ __align__(16) float partial[kFewThreads * N];
@@ -735,33 +741,39 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(LookupGradParams p, in
     if ((int)threadIdx.x < head) to[threadIdx.x] = 0;
     if ((int)threadIdx.x < tail) to[head + 16 * words + threadIdx.x] = 0;
   }
+  bool any = false;
   if (threadIdx.x == 0) long_count = 0;
-  static_assert(kFewTokens <= kFewThreads, "a token per thread");
-  const int t = threadIdx.x;
-  const long long id = t < tokens ? id_at(p.ids, p.ids64, t) : -1;
-  const bool mine = id >= row0 && id < row0 + rows;
-  const unsigned mask = __ballot_sync(FULL, mine);
-  if (lane_id() == 0) masks[t / 32] = mask;
-  if (!__syncthreads_or(mine)) return;
+  for (int base = 0; base < tokens; base += kFewThreads) {
+    const int t = base + threadIdx.x;
+    const long long id = t < tokens ? id_at(p.ids, p.ids64, t) : -1;
+    const bool mine = id >= row0 && id < row0 + rows;
+    const unsigned mask = __ballot_sync(FULL, mine);
+    if (lane_id() == 0) masks[t / 32] = mask;
+    if (mine) row_of[t] = (unsigned short)(id - row0);
+    any = any || mine;
+  }
+  if (!__syncthreads_or(any)) return;
   // the tokens of its rows in their order, then by row
   int count = 0;
-#pragma unroll
-  for (int w = 0; w < kFewThreads / 32; ++w) {
-    if (mine && w == t / 32) {
-      const int at = count + __popc(mask & ((1u << (t & 31)) - 1));
-      list_row[at] = (unsigned short)(id - row0);
+  for (int base = 0; base < tokens; base += kFewThreads) {
+    const int t = base + threadIdx.x, word = t / 32;
+    int before = count;
+    for (int w = base / 32; w < word; ++w) before += __popc(masks[w]);
+    if (masks[word] >> (t & 31) & 1) {
+      const int at = before + __popc(masks[word] & ((1u << (t & 31)) - 1));
+      list_row[at] = row_of[t];
       list_token[at] = (unsigned short)t;
     }
-    count += __popc(masks[w]);
+    for (int w = base / 32; w < (base + kFewThreads) / 32; ++w) count += __popc(masks[w]);
   }
   __syncthreads();
-  if (t < count) {
-    const int row = list_row[t];
+  for (int i = threadIdx.x; i < count; i += kFewThreads) {
+    const int row = list_row[i];
     int rank = 0;
 #pragma unroll 8
-    for (int j = 0; j < count; ++j) rank += list_row[j] < row || (list_row[j] == row && j < t);
+    for (int j = 0; j < count; ++j) rank += list_row[j] < row || (list_row[j] == row && j < i);
     sorted_row[rank] = (unsigned short)row;
-    sorted_token[rank] = list_token[t];
+    sorted_token[rank] = list_token[i];
   }
   __syncthreads();
   const int group = threadIdx.x / lanes, lane = threadIdx.x % lanes, groups = kFewThreads / lanes;
@@ -801,7 +813,10 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(LookupGradParams p, in
   // rows of more tokens: a share for each group
   for (int i = 0; i < long_count; ++i) {
     const int s = long_rows[i], row = sorted_row[s];
-    const int length = __syncthreads_count(s + t < count && sorted_row[min(s + t, count - 1)] == row);
+    int length = 0;
+    for (int base = s; base < count; base += kFewThreads)
+      length += __syncthreads_count(base + (int)threadIdx.x < count &&
+                                    sorted_row[min(base + (int)threadIdx.x, count - 1)] == row);
     const int share = (length + groups - 1) / groups, from = min(length, group * share), to = min(length, from + share);
     for (int base = 0; base < d; base += lanes * N) {
       const int c = base + lane * N;
