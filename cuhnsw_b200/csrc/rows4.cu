@@ -97,7 +97,7 @@ __device__ __forceinline__ unsigned codes_of_any(const T (&v)[8], float step) {
 }
 
 // `lanes` lanes (a power of two, at most a warp) take the words of eight dimensions of kAt rows at once.  Bound: instructions, some
-// 20 per value (1 183 514 rows of 50 floats in 60 us, 4.9 TB/s).
+// 20 per value (1 183 514 rows of 50 floats in 60 us, 4.7 TB/s).
 template <class T, int N, int kAt>
 __global__ void __launch_bounds__(kPackThreads, 4) pack_kernel(const T* rows, long long row_stride, long long n, int d,
                                                                int group_shift, int groups, unsigned char* codes,
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kPackThreads, 4) pack_kernel(const T* rows, lo
 }
 
 // Rows of more than 32 words: a warp has a row, and 4 x 32 words of it at a time, whole ones without a question (50 000 rows of 2048
-// bfloat16 in 66 us, 3.9 TB/s; with a question at each word 80).  Bound: instructions.
+// bfloat16 in 58 us, 4.2 TB/s; as it was at 66, with a question at each word 80).  Bound: instructions, issue slots 0.76 in use.
 template <class T, int N>
 __global__ void __launch_bounds__(kPackThreads) pack_long_kernel(const T* rows, long long row_stride, long long n, int d,
                                                                  int group_shift, int groups, unsigned char* codes,
@@ -261,7 +261,8 @@ __global__ void __launch_bounds__(kPackThreads) pack_wide_kernel(const T* rows, 
 
 // `lanes` threads share `each` rows, V neighbouring values of each (V divides 8): where they are in a row is worked out once.  kRows
 // rows are on their way at a time.
-// Bound: HBM bytes (50 000 rows of 2048 to fp32 in 84 us, 5.5 TB/s; with 4 rows on their way instead of 8 96 us, with 16 101).
+// Bound: HBM bytes (50 000 rows of 2048 to fp32 in 77 us, 6.0 TB/s).  Eight rows on their way: 1 000 000 of 51 floats, caches cold, 74 us,
+// with 4 102, with 16 88; 50 000 of 2048 80, 82 and 78.
 template <class T, int V, int kRows>
 __global__ void __launch_bounds__(kPackThreads) unpack_kernel(const unsigned char* codes, const __nv_bfloat16* scales,
                                                               long long n, int d, int group, int group_shift, T* out,
@@ -352,7 +353,7 @@ template <class T, int V>
 cudaError_t unpack_v(const unsigned char* codes, const __nv_bfloat16* scales, long long n, int d, int group, T* out,
                      cudaStream_t stream) {
   const int lanes = next_pow2((d + V - 1) / V, kPackThreads);
-  // 16 rows, fewer while there are not four CTAs per SM (1 183 514 rows of 50 dimensions 63 us, one at a time 246)
+  // 16 rows, fewer while there are not four CTAs per SM (1 183 514 rows of 50 dimensions 59 us, one at a time 246)
   int each = 16;
   while (each > 1 && n / ((long long)(kPackThreads / lanes) * each) < 4 * kSMs) each /= 2;
   const long long per = (long long)(kPackThreads / lanes) * each, blocks = (n + per - 1) / per;

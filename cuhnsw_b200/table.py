@@ -52,7 +52,7 @@ class _Lookup(torch.autograd.Function):
 
 
 def lookup(rows, ids, scale=1.0):
-  """``scale * rows[ids]``, rounded once to the rows' type: a tensor of ``ids.shape + (num_dims,)``.
+  """``scale * rows[ids]``, the product in float32 rounded to the rows' type: a tensor of ``ids.shape + (num_dims,)``.
 
   rows: float32, float16 or bfloat16 ``[num_rows, num_dims]``, rows any distance apart; ids: int32 or int64 of any shape.  An id
   outside ``0 .. num_rows-1`` gives zeros and gets no gradient: the -1 of an empty result slot of a search, or the padding of a
@@ -78,7 +78,8 @@ def lookup_grad(grad, ids, num_rows, scale=1.0, out=None, accumulate=False):
 
 def pack_rows(rows, group=64):
   """``PackedRows`` of a float32, float16 or bfloat16 ``[num_rows, num_dims]`` tensor: a code of 4 bits per value and a
-  bfloat16 scale per ``group`` consecutive dimensions (32, 64 or a multiple of 128).  A group with a NaN becomes NaN altogether; in one
+  bfloat16 scale per ``group`` consecutive dimensions (32, 64 or a multiple of 128): the group's largest magnitude times float32(1/7),
+  rounded, and codes that are the values over it, rounded.  A group with a NaN becomes NaN altogether; in one
   with an infinity the infinities stay and the rest becomes NaN."""
   codes, scales = _table.pack(rows, group)
   return PackedRows(codes, scales, rows.shape[1], group)
@@ -135,7 +136,9 @@ def select_beams(scores, totals=None, keep=None, log_softmax=True):
   (without the last term if ``log_softmax`` is false); equal ones by smaller beam, then smaller id.  scores: float32, float16 or
   bfloat16 ``[sequences, beams, vocabulary]``; totals: float32 ``[sequences, beams]``, default zeros; keep: 1 to 256, default
   the number of beams.  A total of -inf or NaN is never chosen (a beam that has ended or an id that may not follow is -inf);
-  slots that stay empty hold -inf, -1, -1."""
+  slots that stay empty hold -inf, -1, -1.  Totals are compared in 64 bits.  The log's sum is one of float32 exponentials: within some
+  3e-7, and the same for the same scores, so that equal beams are ties; totals of different beams closer than that may come in
+  either order."""
   return _table.select_beams(scores, totals, keep, log_softmax)
 
 

@@ -191,7 +191,7 @@ int cuhnsw_merge_topk_gathered_device(const int32_t* d_gathered, const int32_t* 
 /* element types; all sums are fp32 whatever the type */
 enum { CUHNSW_F32 = 0, CUHNSW_F16 = 1, CUHNSW_BF16 = 2 };
 
-/* d_out[t] = scale * d_rows[d_ids[t]], rounded once to the rows' type (scale 1: copied).  d_rows: num_rows rows of num_dims
+/* d_out[t] = scale * d_rows[d_ids[t]], the product in fp32, rounded to the rows' type (scale 1: copied).  d_rows: num_rows rows of num_dims
  * values, row_stride values apart; d_ids: num_ids int32 or (ids64) int64; d_out: num_ids x num_dims, dense.  An id outside
  * 0..num_rows-1, e.g. the -1 of an empty result slot, gives zeros.  num_rows up to 2^31 - 2. */
 int cuhnsw_lookup_device(const void* d_rows, int64_t row_stride, int64_t num_rows, int64_t num_dims, int32_t type,
@@ -235,7 +235,9 @@ int cuhnsw_scores4_device(const void* d_codes, const void* d_scales, int64_t num
  * sequences seq_stride and beams beam_stride values apart; d_totals: sequences x beams fp32, or NULL for zeros.  Totals of
  * -inf or NaN are not chosen; what is left of the `keep` slots holds -inf, -1, -1.  d_out_*: sequences x keep; d_out_beams and
  * d_out_found (slots in use, per sequence) may be NULL.  negate: the totals are written with the other sign (+inf in empty
- * slots), the distances of the dot metric.  Totals are compared in 64 bits.  vocabulary below 2^31, beams up to 16384. */
+ * slots), the distances of the dot metric.  Totals are sums in 64 bits and compared so (one below fp32's range is written as -inf).
+ * The log is of a sum of fp32 exponentials, within some 3e-7 and the same for the same scores wherever they lie: totals of
+ * two beams closer than that may come in either order.  vocabulary below 2^31, beams up to 16384. */
 int64_t cuhnsw_select_workspace(int64_t sequences, int64_t beams, int64_t vocabulary, int32_t keep);
 int cuhnsw_select_device(const void* d_scores, int64_t seq_stride, int64_t beam_stride, int32_t type,
                          const float* d_totals, int64_t sequences, int64_t beams, int64_t vocabulary, int32_t keep,
