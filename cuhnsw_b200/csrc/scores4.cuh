@@ -32,6 +32,8 @@ __device__ __forceinline__ unsigned in_register(unsigned x) {
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                                                             \
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1))
 
+// Codes as values, in the way that is common for small whole numbers: their bits under the mantissa of a power of two, which is then
+// taken away.
 struct PairsF16 {
   unsigned magic = in_register(0x64006400u);  // 1024, the last bit of whose mantissa is one
   unsigned minus_low = in_register(0xe408e408u), sixteenth = in_register(0x2c002c00u), minus_high = in_register(0xd480d480u);

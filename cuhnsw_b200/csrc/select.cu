@@ -131,7 +131,8 @@ struct Pool {
 // the `keep`-th is a bound that as many scores reach; the scores of the few threads whose largest one reaches it are looked at again,
 // and what is not below goes into a pool, the pool in order.  Also the piece's largest score and its sum of
 // exponentials, in fp32, which a score's place among its own beam's does not depend on: the log of a row's sum is within 3e-7 (rows of
-// 1000 to 1 000 000 scores, deviations 0.01 to 30), and the same for equal rows.  Bound: latency (256 x 131 072 floats in 38 us, 3.5 TB/s,
+// 1000 to 1 000 000 scores, deviations 0.01 to 30), and the same for equal rows.  (In 64 bits, by a table and a series, it is within 3e-14:
+// a selection from 256 x 131 072 floats, caches cold, 69 us instead of 52.)  Bound: latency (256 x 131 072 floats in 38 us, 3.5 TB/s,
 // issue slots 0.54 in use; per instruction 3.5 warps wait for loads, and 2.5 at barriers, where a CTA has no load on its way).
 constexpr int kPoolScores = 4096;
 constexpr int kWarps = kThreads / 32;
